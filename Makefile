@@ -4,7 +4,7 @@
 #   make ref        -> oracle/_ref/*.so           (needs /root/reference; this container only)
 HIPCC   ?= /opt/rocm/bin/hipcc
 ARCH    ?= gfx950
-HIPFLAGS = -O3 --offload-arch=$(ARCH) -std=c++17 -fPIC -Iinclude -Wno-unused-value
+HIPFLAGS = -O3 --offload-arch=$(ARCH) -std=c++17 -fPIC -Iinclude -Wno-unused-value -Xclang -target-feature -Xclang -packed-fp32-ops
 
 LIB = geot_amd/libgeot_hip.so
 SRC = geot_amd/csrc/seg_reduce.hip geot_amd/csrc/seg_reduce_f32.hip geot_amd/csrc/seg_reduce_f64.hip geot_amd/csrc/seg_reduce_f16.hip \
@@ -27,7 +27,7 @@ devlib:
 
 tools: tools/kbench
 tools/kbench: tools/kbench.cpp $(LIB) include/geot_hip.h
-	$(HIPCC) -O2 --offload-arch=$(ARCH) -std=c++17 -Iinclude tools/kbench.cpp -Lgeot_amd -lgeot_hip \
+	$(HIPCC) -O2 --offload-arch=$(ARCH) -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -Iinclude tools/kbench.cpp -Lgeot_amd -lgeot_hip \
 	  -Wl,-rpath,'$$ORIGIN/../geot_amd' -o $@
 
 # the PyTorch dispatcher plugin over the C ABI (the host side of the drop-in): geot_amd/_C.so

@@ -72,7 +72,7 @@ def hipcc() -> str:
 
 def _digest(paths) -> str:
     import hashlib
-    h = hashlib.sha256()
+    h = hashlib.sha256(" ".join(f for f in HIPFLAGS if not os.path.isabs(f)).encode())     # (other flags are another binary)
     for p in paths:
         with open(p, "rb") as f:
             h.update(f.read())
@@ -107,7 +107,10 @@ def needs_build(dev: bool = False) -> bool:
 
 
 OBJ_DIR = os.path.join(_HERE, "csrc", ".obj")        # per-source objects (git-ignored; they do not travel with a snapshot)
-HIPFLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-Wno-unused-value", "-I", os.path.join(_ROOT, "include")]
+# (no packed float32 arithmetic: some forms of v_pk_{add,mul,fma}_f32 have returned wrong values on this hardware now and then; the
+# host pass warns that it does not know the feature)
+HIPFLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-Wno-unused-value", "-Xclang", "-target-feature", "-Xclang",
+            "-packed-fp32-ops", "-I", os.path.join(_ROOT, "include")]
 
 
 def build(force: bool = False, verbose: bool = False, jobs: int = 0, dev: bool = False) -> str:
