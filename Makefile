@@ -9,7 +9,7 @@ HIPFLAGS = -O3 --offload-arch=$(ARCH) -std=c++17 -fPIC -Iinclude -Wno-unused-val
 LIB = geot_amd/libgeot_hip.so
 SRC = geot_amd/csrc/seg_reduce.hip geot_amd/csrc/seg_reduce_f32.hip geot_amd/csrc/seg_reduce_f64.hip geot_amd/csrc/seg_reduce_f16.hip \
       geot_amd/csrc/seg_reduce_bf16.hip geot_amd/csrc/seg_slab.hip geot_amd/csrc/seg_sort.hip geot_amd/csrc/seg_plan.hip \
-      geot_amd/csrc/seg_guard.hip
+      geot_amd/csrc/seg_guard.hip geot_amd/csrc/dense_mm.hip geot_amd/csrc/row_norm.hip
 
 .PHONY: all lib devlib tools shim oracle ref clean
 all: lib tools
@@ -33,7 +33,7 @@ tools/kbench: tools/kbench.cpp $(LIB) include/geot_hip.h
 # the PyTorch dispatcher plugin over the C ABI (the host side of the drop-in): geot_amd/_C.so
 shim: geot_amd/_C.so
 # (geot_amd/_lib.py holds the recipe: g++ -c csrc/torch_ops.cpp csrc/host_*.cpp side by side, one link against libtorch + libgeot_hip)
-geot_amd/_C.so: geot_amd/csrc/torch_ops.cpp geot_amd/csrc/host_state.cpp geot_amd/csrc/host_cache.cpp geot_amd/csrc/host_plan.cpp geot_amd/csrc/host.h $(LIB) include/geot_hip.h
+geot_amd/_C.so: geot_amd/csrc/torch_ops.cpp geot_amd/csrc/host_state.cpp geot_amd/csrc/host_cache.cpp geot_amd/csrc/host_plan.cpp geot_amd/csrc/host_dense.cpp geot_amd/csrc/host.h $(LIB) include/geot_hip.h
 	python3 geot_amd/_lib.py plugin
 
 oracle:

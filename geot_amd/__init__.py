@@ -23,9 +23,12 @@ from .ops import (  # noqa: E402
     gather_weight_scatter_impl,
     get_reduction_enum,
     index_scatter,
+    layer_norm,
+    linear,
     mh_spmm,
     mh_spmm_transposed,
     sddmm_coo_impl,
+    segment_matmul,
 )
 
 from .graph import Graph, PlanOrdered  # noqa: E402
@@ -36,5 +39,5 @@ __all__ = [
     "index_scatter", "gather_scatter", "gather_weight_scatter", "mh_spmm", "mh_spmm_transposed",
     "csr_gws", "coo_to_csr", "csr_gws_impl",
     "gather_scatter_impl", "gather_weight_scatter_impl", "sddmm_coo_impl", "get_reduction_enum", "hip",
-    "Graph", "PlanOrdered",
+    "Graph", "PlanOrdered", "linear", "segment_matmul", "layer_norm",
 ]

@@ -24,12 +24,12 @@ DEV = os.environ.get("GEOT_HIP_LIB", "") == "dev"
 # (the longest compiles first; seg_reduce_<type>.hip are seg_reduce.hip's kernels of one storage type each - they #include it)
 SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("seg_reduce_f32.hip", "seg_plan.hip", "seg_reduce_f16.hip", "seg_reduce_bf16.hip",
                                                      "seg_reduce_f64.hip", "seg_slab.hip", "seg_reduce.hip", "seg_sort.hip",
-                                                     "seg_guard.hip")]
+                                                     "seg_guard.hip", "dense_mm.hip", "row_norm.hip")]
 SEG_REDUCE = os.path.join(_HERE, "csrc", "seg_reduce.hip")
 HEADER = os.path.join(_ROOT, "include", "geot_hip.h")
 DEV_HEADER = os.path.join(_ROOT, "include", "geot_hip_dev.h")     # measurement hooks + experiment switches (not the stable ABI)
 PLUGIN_PATH = os.path.join(_HERE, "_C.so")                       # the torch dispatcher plugin (csrc/torch_ops.cpp)
-PLUGIN_SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("torch_ops.cpp", "host_state.cpp", "host_cache.cpp", "host_plan.cpp")]
+PLUGIN_SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("torch_ops.cpp", "host_state.cpp", "host_cache.cpp", "host_plan.cpp", "host_dense.cpp")]
 PLUGIN_HEADER = os.path.join(_HERE, "csrc", "host.h")
 LIB_INPUTS = SOURCES + [HEADER, DEV_HEADER, os.path.join(_HERE, "csrc", "internal.h")]
 PLUGIN_INPUTS = PLUGIN_SOURCES + [PLUGIN_HEADER, HEADER]
@@ -48,6 +48,9 @@ SYMBOLS = [
     "geot_csr_workspace_bytes", "geot_csr_gws", "geot_coo_to_csr",
     "geot_slab_units", "geot_slab_full_chip", "geot_slab_rows_per_group", "geot_slab_rows_per_group_dtype", "geot_slab_units_for", "geot_slab_rows_per_group_shape", "geot_slab_workspace_bytes", "geot_slab_workspace_bytes_staged", "geot_slab_spmm", "geot_slab_sddmm", "geot_slab_sddmm_staged", "geot_slab_mh_sddmm", "geot_slab_to_plan_order",
     "geot_slab_plan_scratch_bytes", "geot_slab_plan_rows", "geot_slab_plan_groups", "geot_slab_plan_edges",
+    "geot_linear", "geot_activation_backward", "geot_linear_grad_input", "geot_linear_grad_weight_workspace_bytes", "geot_linear_grad_weight",
+    "geot_segment_matmul", "geot_segment_matmul_grad_input", "geot_segment_matmul_grad_weight_workspace_bytes", "geot_segment_matmul_grad_weight",
+    "geot_layer_norm", "geot_layer_norm_backward_workspace_bytes", "geot_layer_norm_backward",
     "geot_profile_enable", "geot_profile_reset", "geot_profile_read", "geot_profile_box", "geot_profile_box_rows", "geot_tune", "geot_set_option", "geot_last_kernel",
 ]
 
@@ -266,6 +269,22 @@ def load() -> ctypes.CDLL:
     L.geot_slab_sddmm_staged.argtypes = [ctypes.POINTER(SlabPlan), c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_vp, c_sz, c_vp]
     L.geot_slab_to_plan_order.argtypes = [ctypes.POINTER(SlabPlan), c_vp, c_vp, c_i64, c_int, c_vp]
     L.geot_slab_mh_sddmm.argtypes = [ctypes.POINTER(SlabPlan), c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_sz, c_vp]
+    c_f = ctypes.c_float
+    L.geot_linear.argtypes = [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_int, c_vp]
+    L.geot_activation_backward.argtypes = [c_vp, c_vp, c_vp, c_i64, c_int, c_int, c_vp]
+    L.geot_linear_grad_input.argtypes = [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_vp]
+    L.geot_linear_grad_weight_workspace_bytes.restype = c_sz
+    L.geot_linear_grad_weight_workspace_bytes.argtypes = [c_i64, c_i64, c_i64]
+    L.geot_linear_grad_weight.argtypes = [c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_vp, c_sz, c_vp]
+    L.geot_segment_matmul.argtypes = [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp]
+    L.geot_segment_matmul_grad_input.argtypes = [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp]
+    L.geot_segment_matmul_grad_weight_workspace_bytes.restype = c_sz
+    L.geot_segment_matmul_grad_weight_workspace_bytes.argtypes = [c_i64, c_i64, c_i64, c_i64]
+    L.geot_segment_matmul_grad_weight.argtypes = [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_sz, c_vp]
+    L.geot_layer_norm.argtypes = [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_f, c_int, c_int, c_vp]
+    L.geot_layer_norm_backward_workspace_bytes.restype = c_sz
+    L.geot_layer_norm_backward_workspace_bytes.argtypes = [c_i64, c_i64]
+    L.geot_layer_norm_backward.argtypes = [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_int, c_vp, c_sz, c_vp]
     L.geot_profile_enable.argtypes = [c_int]
     L.geot_profile_enable.restype = None
     L.geot_profile_reset.restype = None

@@ -1,0 +1,900 @@
+// dense_mm.hip -- the matrix products of a layer's node and edge rows: geot_linear, geot_segment_matmul and their gradients.
+//
+// One tile kernel per shape of product, on the matrix cores:
+//   mm_rows_kernel     y[i, :] = act(a[i, :] . B(group of i) + bias) + residual      rows grouped by a pointer array (or one group)
+//   mm_weight_kernel   dW(group) = p_rows^T q_rows, the sum running over the group's rows, split into chunks of rows
+//   mm_join_kernel     adds the chunks' partial products (32 bits, in chunk order: the same bits every run)
+//
+// Arithmetic.  16-bit operands go to v_mfma_f32_32x32x16 as they are, sums in float32.  float32 operands are split exactly into three
+// bfloat16 parts, x = x1 + x2 + x3 (8 significant bits each, round to nearest), and a product takes the six partial products whose
+// weight is above 2^-24 of it: x1y1, x1y2, x2y1, x2y2, x1y3, x3y1.  What is left out (x2y3, x3y2, x3y3) is at most 2^-23 of |xy| and
+// 2^-26 of it on average - below the float32 rounding of the sum itself - while the bfloat16 cores run 16 times faster than the
+// float32 ones (dense peaks 2.5 PFLOP/s against 0.157): six products there cost less than half of one here.  A split of an infinity
+// (inf - inf) or of a value that rounds up to one is not a number: any non-finite sum is computed again, element by element, in plain
+// float32 (element_again), so infinities and NaN come out as in an ordinary float32 product.
+//
+// Layout in LDS.  A tile holds chunks of 8 reduction values (16 bytes) - the operand of one MFMA lane - as
+// [part][chunk][row ^ ((row >> 3) & 7)], each chunk column padded: fragment reads are contiguous, and the writes of both staging forms
+// hit 8 different 16-byte banks.  An operand whose reduction index is contiguous in memory is staged chunk by chunk; one whose OUTPUT
+// index is contiguous is staged in blocks of 8 reduction values by VR columns that a thread transposes in its registers, so one compute
+// loop serves x W^T, dz W, and x^T dz.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "geot_hip.h"
+#include "internal.h"
+
+namespace {
+
+using bf16 = __bf16;
+using f16 = _Float16;
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8), may_alias));
+typedef f16 f16x8 __attribute__((ext_vector_type(8), may_alias));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4), may_alias));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4), may_alias));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2), may_alias));
+
+constexpr int kThreads = 256; // four waves, two by two over the tile
+
+// loads and stores of 16 / 8 bytes at the element's own alignment (rows of any width, views of any offset)
+template <int SIZE> struct Packed;
+template <> struct Packed<2> {
+  typedef u32x4 x16 __attribute__((aligned(2), may_alias));
+  typedef u32x2 x8 __attribute__((aligned(2), may_alias));
+};
+template <> struct Packed<4> {
+  typedef u32x4 x16 __attribute__((aligned(4), may_alias));
+  typedef u32x2 x8 __attribute__((aligned(4), may_alias));
+};
+template <typename T> using Packed16 = typename Packed<sizeof(T)>::x16;
+template <typename T> using Packed8 = typename Packed<sizeof(T)>::x8;
+
+template <typename T> struct Elem;
+template <> struct Elem<bf16> {
+  static constexpr int PARTS = 1, BK = 64, VR = 4;
+  typedef bf16x8 Frag;
+  static __device__ f32x16 mfma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Elem<f16> {
+  static constexpr int PARTS = 1, BK = 64, VR = 4;
+  typedef f16x8 Frag;
+  static __device__ f32x16 mfma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Elem<float> {
+  static constexpr int PARTS = 3, BK = 32, VR = 2;
+  typedef bf16x8 Frag;
+  static __device__ f32x16 mfma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+
+template <typename T> __device__ inline float as_float(T v) { return (float)v; }
+
+__device__ inline int swizzled(int row) { return row ^ ((row >> 3) & 7); }
+
+// ---- a tile of R rows (output index) by BK reduction values -------------------------------------------------------------------
+template <typename T, int R> struct Tile {
+  using E = Elem<T>;
+  static constexpr int CK = E::BK / 8;        // chunks along the reduction
+  static constexpr int PAD = 8 / CK;          // chunk columns 16 * PAD bytes apart in their banks
+  static constexpr int COL = R + PAD;         // 16-byte slots of a chunk column
+  static constexpr int BYTES = E::PARTS * CK * COL * 16;
+  static __device__ int slot(int part, int chunk, int row) { return (part * CK + chunk) * COL + swizzled(row); }
+};
+
+// three bfloat16 parts of 8 floats
+__device__ inline void split8(const float (&v)[8], bf16x8 (&p)[3]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bf16 a = (bf16)v[j];
+    const float r = v[j] - (float)a;
+    const bf16 b = (bf16)r;
+    p[0][j] = a;
+    p[1][j] = b;
+    p[2][j] = (bf16)(r - (float)b);
+  }
+}
+
+// Staging, reduction index contiguous: element (row, k) at base[row * ld + k].
+template <typename T, int R> struct StageK {
+  using E = Elem<T>;
+  using L = Tile<T, R>;
+  static constexpr int N = (R * L::CK + kThreads - 1) / kThreads;
+  static constexpr bool WHOLE = (R * L::CK) % kThreads == 0;
+  static constexpr int W = 8 * sizeof(T) / 16; // 16-byte pieces of a chunk
+  u32x4 reg[N][W];
+  const T *base;
+  int64_t ld;
+  int rows;     // rows that exist (>= 1); the others read the last one and are not stored
+  int64_t k_end;
+
+  __device__ void open(const T *b, int64_t ld_, int64_t first, int64_t rows_left, int64_t k_begin, int64_t k_end_) {
+    ld = ld_;
+    rows = (int)(rows_left < R ? rows_left : R);
+    base = b + first * ld_ + k_begin;
+    k_end = k_end_ - k_begin;
+  }
+  __device__ void load(int64_t k0, int tid) {
+    const bool inside = k0 + E::BK <= k_end;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = tid + i * kThreads;
+      const int chunk = idx % L::CK;
+      int row = idx / L::CK;
+      row = row < rows ? row : rows - 1;
+      const int64_t k = k0 + chunk * 8;
+      const T *p = base + row * ld + k;
+      if (inside || k + 8 <= k_end) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) reg[i][w] = reinterpret_cast<const Packed16<T> *>(p)[w];
+      } else {
+        alignas(16) T tmp[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) tmp[j] = k + j < k_end ? p[j] : (T)0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) reg[i][w] = reinterpret_cast<const u32x4 *>(tmp)[w];
+      }
+    }
+  }
+  __device__ void store(char *lds, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = tid + i * kThreads;
+      if (!WHOLE && idx >= R * L::CK) continue;
+      const int chunk = idx % L::CK, row = idx / L::CK;
+      if constexpr (E::PARTS == 1) {
+        reinterpret_cast<u32x4 *>(lds)[L::slot(0, chunk, row)] = reg[i][0];
+      } else {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(reg[i][j / 4][j % 4]);
+        bf16x8 p[3];
+        split8(v, p);
+#pragma unroll
+        for (int s = 0; s < 3; ++s) reinterpret_cast<bf16x8 *>(lds)[L::slot(s, chunk, row)] = p[s];
+      }
+    }
+  }
+};
+
+// Staging, output index contiguous: element (row, k) at base[k * ld + row].  SUM: also adds up what it stages, per row.
+template <typename T, int R, bool SUM> struct StageR {
+  using E = Elem<T>;
+  using L = Tile<T, R>;
+  static constexpr int VR = E::VR; // rows of a thread's block: 8 bytes
+  static constexpr int BLOCKS = (R / VR) * L::CK;
+  static constexpr int N = (BLOCKS + kThreads - 1) / kThreads;
+  static constexpr bool WHOLE = BLOCKS % kThreads == 0;
+  u32x2 reg[N][8];
+  float sum[SUM ? N : 1][VR];
+  const T *base;
+  int64_t ld, k_end;
+  int rows;
+  bool add = false; // (SUM: this workgroup is the one that adds them up)
+
+  __device__ void open(const T *b, int64_t ld_, int64_t first, int64_t rows_left, int64_t k_begin, int64_t k_end_) {
+    ld = ld_;
+    rows = (int)(rows_left < R ? rows_left : R);
+    base = b + k_begin * ld_ + first;
+    k_end = k_end_ - k_begin;
+    if constexpr (SUM) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < VR; ++j) sum[i][j] = 0.0f;
+    }
+  }
+  __device__ void load(int64_t k0, int tid) {
+    const bool inside = k0 + E::BK <= k_end && rows == R;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = tid + i * kThreads;
+      const int row = (idx % (R / VR)) * VR, chunk = idx / (R / VR);
+      const T *p = base + (k0 + chunk * 8) * ld + row;
+      if (!WHOLE && idx >= BLOCKS) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) reg[i][j] = u32x2{0, 0};
+      } else if (inside) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) reg[i][j] = *reinterpret_cast<const Packed8<T> *>(p + j * ld);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          alignas(8) T tmp[VR];
+          const bool in_k = k0 + chunk * 8 + j < k_end;
+#pragma unroll
+          for (int r = 0; r < VR; ++r) tmp[r] = in_k && row + r < rows ? p[j * ld + r] : (T)0.0f;
+          reg[i][j] = *reinterpret_cast<const u32x2 *>(tmp);
+        }
+      }
+    }
+  }
+  __device__ float value(int i, int j, int r) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(reg[i][j][r]);
+    } else {
+      const uint32_t half = (r & 1) ? reg[i][j][r / 2] >> 16 : reg[i][j][r / 2] & 0xffffu;
+      return (float)__builtin_bit_cast(T, (uint16_t)half);
+    }
+  }
+  __device__ void store(char *lds, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = tid + i * kThreads;
+      const int row = (idx % (R / VR)) * VR, chunk = idx / (R / VR);
+      if (WHOLE || idx < BLOCKS) {
+#pragma unroll
+        for (int r = 0; r < VR; ++r) {
+          if constexpr (E::PARTS == 1) {
+            u32x4 out; // two of 8 reduction values a word: the halves of two neighbouring loads
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              out[j] = __builtin_amdgcn_perm(reg[i][2 * j + 1][r / 2], reg[i][2 * j][r / 2], (r & 1) ? 0x07060302u : 0x05040100u);
+            reinterpret_cast<u32x4 *>(lds)[L::slot(0, chunk, row + r)] = out;
+          } else {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = value(i, j, r);
+            bf16x8 p[3];
+            split8(v, p);
+#pragma unroll
+            for (int s = 0; s < 3; ++s) reinterpret_cast<bf16x8 *>(lds)[L::slot(s, chunk, row + r)] = p[s];
+          }
+        }
+      }
+      if constexpr (SUM) {
+        if (add) {
+#pragma unroll
+          for (int r = 0; r < VR; ++r)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[i][r] += value(i, j, r);
+        }
+      }
+    }
+  }
+};
+
+// ---- the products of one staged pair of tiles -----------------------------------------------------------------------------------
+template <typename T, int BM, int BN> struct Accum {
+  using E = Elem<T>;
+  static constexpr int FM = BM / 64, FN = BN / 64; // 32 x 32 fragments of a wave (the four waves sit two by two)
+  f32x16 acc[FM][FN];
+
+  __device__ void clear() {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+  }
+  __device__ void step(const char *la, const char *lb, int wm, int wn, int lane) {
+    using F = typename E::Frag;
+    using LA = Tile<T, BM>;
+    using LB = Tile<T, BN>;
+#pragma unroll
+    for (int s = 0; s < E::BK / 16; ++s) {
+      const int chunk = 2 * s + lane / 32;
+      F a[E::PARTS][FM], b[E::PARTS][FN];
+#pragma unroll
+      for (int p = 0; p < E::PARTS; ++p) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) a[p][i] = reinterpret_cast<const F *>(la)[LA::slot(p, chunk, wm * (BM / 2) + i * 32 + lane % 32)];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) b[p][j] = reinterpret_cast<const F *>(lb)[LB::slot(p, chunk, wn * (BN / 2) + j * 32 + lane % 32)];
+      }
+      // the smallest partial products first
+      constexpr int NP = E::PARTS == 1 ? 1 : 6;
+      constexpr int PA[6] = {E::PARTS == 1 ? 0 : 2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) acc[i][j] = E::mfma(a[PA[p]][i], b[PB[p]][j], acc[i][j]);
+    }
+  }
+  // element e of a fragment: row 8 * (e / 4) + 4 * (lane / 32) + e % 4, column lane % 32
+  static __device__ int row_of(int e, int lane) { return 8 * (e / 4) + 4 * (lane / 32) + e % 4; }
+  // fragments of row block i of every wave -> lds[64][BN + 4] floats (rows wm * 32 + ..)
+  __device__ void put(float *lds, int i, int wm, int wn, int lane) const {
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) lds[(wm * 32 + row_of(e, lane)) * (BN + 4) + wn * (BN / 2) + j * 32 + lane % 32] = acc[i][j][e];
+  }
+};
+
+// One element in plain float32: the way of an infinity, a NaN or an overflow through a product of split operands.  A NaN ends it.
+__device__ float element_again(const float *a, int64_t stride_a, const float *b, int64_t stride_b, int64_t k) {
+  float s = 0.0f;
+  for (int64_t i = 0; i < k && s == s; ++i) s = fmaf(a[i * stride_a], b[i * stride_b], s);
+  return s;
+}
+__device__ inline bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+
+__device__ inline float activate(float z, int act) {
+  if (act == GEOT_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
+  if (act == GEOT_ACT_GELU) return 0.5f * z * erfcf(-0.70710678118654752f * z);
+  if (act == GEOT_ACT_SILU) return z / (1.0f + expf(-z));
+  return z;
+}
+__device__ inline float activation_slope(float z, int act) {
+  if (act == GEOT_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
+  if (act == GEOT_ACT_GELU) return 0.5f * erfcf(-0.70710678118654752f * z) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+  if (act == GEOT_ACT_SILU) {
+    const float s = 1.0f / (1.0f + expf(-z));
+    return s * (1.0f + z * (1.0f - s));
+  }
+  return 1.0f;
+}
+
+// ---- groups of rows --------------------------------------------------------------------------------------------------------------
+// Rows are cut at the boundaries q_0 = 0, q_1 = ptr[0], ..., q_{G+1} = ptr[G], q_{G+2} = rows (each clamped into [0, rows]): G groups,
+// and the rows in front of and behind them, whose results are zero.  Piece j starts at slot floor(q_j / unit) + j of the launch: that
+// leaves it at least ceil(len / unit) slots and makes the slot of a workgroup a binary search in ptr - no scan, no table, no second
+// launch; at most G + 2 slots stay empty.  Without a pointer array there is one group, all rows.
+struct Groups {
+  const int64_t *ptr;
+  int64_t groups, rows;
+  __device__ int64_t bound(int64_t j) const { // q_j
+    if (j <= 0) return 0;
+    if (j >= groups + 2) return rows;
+    const int64_t q = ptr[j - 1];
+    return q < 0 ? 0 : (q > rows ? rows : q);
+  }
+};
+struct Piece {
+  int64_t group;      // 0 .. G-1; -1: rows outside every group
+  int64_t begin, end; // the piece's rows
+  int64_t index;      // which unit of the piece this slot is (may lie behind its end)
+  int64_t start;      // the piece's first slot
+};
+__device__ inline Piece piece_of(const Groups &g, int64_t unit, int64_t slot) {
+  if (!g.ptr) return {0, 0, g.rows, slot, 0};
+  int64_t lo = 0, hi = g.groups + 1; // the last piece whose first slot is <= slot
+  while (lo < hi) {
+    const int64_t mid = (lo + hi + 1) / 2;
+    if (g.bound(mid) / unit + mid <= slot) lo = mid;
+    else hi = mid - 1;
+  }
+  const int64_t q0 = g.bound(lo), q1 = g.bound(lo + 1), start = q0 / unit + lo;
+  return {lo >= 1 && lo <= g.groups ? lo - 1 : -1, q0, q1, slot - start, start};
+}
+int64_t slots_of(int64_t rows, int64_t groups, bool with_ptr, int64_t unit) {
+  if (!with_ptr) return (rows + unit - 1) / unit;
+  return rows / unit + groups + 2;
+}
+
+// Workgroups go to the 8 XCDs round robin; tiles that share an operand should share an L2: XCD x takes the x-th eighth of the tiles.
+__device__ inline int64_t xcd_contiguous(int64_t block, int64_t blocks) {
+  const int64_t x = block % 8, q = blocks / 8, r = blocks % 8;
+  return x * q + (x < r ? x : r) + block / 8;
+}
+
+struct RowsArgs {
+  const void *a, *b, *bias, *residual;
+  void *z, *y;
+  int64_t lda, ldb, ldr, ldy, b_group, bias_group; // strides in elements
+  Groups groups;
+  int64_t n, k;
+  int64_t tiles_n;
+  int act;
+};
+
+// y rows.  BR: B's output index is contiguous (element (n, k) at b[k * ldb + n]), otherwise its reduction index (b[n * ldb + k]).
+template <typename T, int BM, int BN, bool BR, int NBUF>
+__global__ __launch_bounds__(kThreads, 2) void mm_rows_kernel(const RowsArgs g) {
+  using E = Elem<T>;
+  using LA = Tile<T, BM>;
+  using LB = Tile<T, BN>;
+  constexpr int STAGE = LA::BYTES + LB::BYTES;
+  constexpr int EPI = 64 * (BN + 4) * 4;
+  __shared__ __attribute__((aligned(16))) char lds[NBUF * STAGE > EPI ? NBUF * STAGE : EPI];
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, wm = wave / 2, wn = wave % 2;
+  const int64_t tile = xcd_contiguous(blockIdx.x, gridDim.x);
+  const int64_t slot = tile / g.tiles_n, n0 = (tile % g.tiles_n) * BN;
+  const Piece piece = piece_of(g.groups, BM, slot);
+  const int64_t r0 = piece.begin + piece.index * BM;
+  if (r0 >= piece.end) return;
+  const int64_t rows = piece.end - r0 < BM ? piece.end - r0 : BM;
+  const bool real = piece.group >= 0;
+  const int64_t k_len = real ? g.k : 0;
+  const T *A = static_cast<const T *>(g.a);
+  const T *B = static_cast<const T *>(g.b) + (real ? piece.group * g.b_group : 0);
+
+  Accum<T, BM, BN> acc;
+  acc.clear();
+  StageK<T, BM> sa;
+  typename std::conditional<BR, StageR<T, BN, false>, StageK<T, BN>>::type sb;
+  sa.open(A, g.lda, r0, rows, 0, k_len);
+  sb.open(B, g.ldb, n0, g.n - n0, 0, k_len);
+  if (k_len > 0) {
+    sa.load(0, tid);
+    sb.load(0, tid);
+    if constexpr (NBUF == 2) {
+      sa.store(lds, tid);
+      sb.store(lds + LA::BYTES, tid);
+      if (E::BK < k_len) {
+        sa.load(E::BK, tid);
+        sb.load(E::BK, tid);
+      }
+      __syncthreads();
+      int cur = 0;
+      for (int64_t k0 = 0; k0 < k_len; k0 += E::BK) {
+        char *now = lds + cur * STAGE, *next = lds + (cur ^ 1) * STAGE;
+        acc.step(now, now + LA::BYTES, wm, wn, lane);
+        if (k0 + E::BK < k_len) {
+          sa.store(next, tid);
+          sb.store(next + LA::BYTES, tid);
+          if (k0 + 2 * E::BK < k_len) {
+            sa.load(k0 + 2 * E::BK, tid);
+            sb.load(k0 + 2 * E::BK, tid);
+          }
+        }
+        __syncthreads();
+        cur ^= 1;
+      }
+    } else {
+      for (int64_t k0 = 0; k0 < k_len; k0 += E::BK) {
+        sa.store(lds, tid);
+        sb.store(lds + LA::BYTES, tid);
+        if (k0 + E::BK < k_len) {
+          sa.load(k0 + E::BK, tid);
+          sb.load(k0 + E::BK, tid);
+        }
+        __syncthreads();
+        acc.step(lds, lds + LA::BYTES, wm, wn, lane);
+        __syncthreads();
+      }
+    }
+  }
+
+  // epilogue: 64 rows at a time through LDS, so that every access to memory is whole rows; V consecutive columns a thread
+  constexpr int V = 16 / sizeof(T), TPR = BN / V, RPP = kThreads / TPR;
+  using Vec = Packed16<T>;
+  const int col = (tid % TPR) * V;
+  const int64_t nc = n0 + col;
+  const int cols = nc + V <= g.n ? V : (nc < g.n ? (int)(g.n - nc) : 0);
+  float bias[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    bias[v] = g.bias && real && v < cols ? as_float(static_cast<const T *>(g.bias)[piece.group * g.bias_group + nc + v]) : 0.0f;
+  float *out = reinterpret_cast<float *>(lds);
+#pragma unroll
+  for (int i = 0; i < BM / 64; ++i) {
+    if (i) __syncthreads();
+    acc.put(out, i, wm, wn, lane);
+    __syncthreads();
+    if (cols > 0) {
+#pragma unroll 2
+      for (int lr = tid / TPR; lr < 64; lr += RPP) {
+        const int64_t tr = (lr / 32) * (BM / 2) + i * 32 + lr % 32;
+        if (tr >= rows) continue;
+        const int64_t row = r0 + tr;
+        float v[V];
+#pragma unroll
+        for (int c = 0; c < V; c += 4) {
+          const f32x4 q = *reinterpret_cast<const f32x4 *>(out + lr * (BN + 4) + col + c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[c + e] = q[e];
+        }
+        if constexpr (E::PARTS == 3) {
+#pragma unroll
+          for (int c = 0; c < V; ++c)
+            if (!finite(v[c]) && c < cols)
+              v[c] = element_again(reinterpret_cast<const float *>(A) + row * g.lda, 1,
+                                   reinterpret_cast<const float *>(B) + (BR ? nc + c : (nc + c) * g.ldb), BR ? g.ldb : 1, k_len);
+        }
+        alignas(16) T tmp[V];
+#pragma unroll
+        for (int c = 0; c < V; ++c) v[c] += bias[c];
+        if (g.z) {
+          T *zp = static_cast<T *>(g.z) + row * g.n + nc;
+#pragma unroll
+          for (int c = 0; c < V; ++c) tmp[c] = (T)v[c];
+          if (cols == V) *reinterpret_cast<Vec *>(zp) = *reinterpret_cast<const u32x4 *>(tmp);
+          else
+            for (int c = 0; c < cols; ++c) zp[c] = tmp[c];
+        }
+        if (g.act != GEOT_ACT_NONE) {
+#pragma unroll
+          for (int c = 0; c < V; ++c) v[c] = activate(v[c], g.act);
+        }
+        if (g.residual) {
+          const T *rp = static_cast<const T *>(g.residual) + row * g.ldr + nc;
+          if (cols == V) {
+            *reinterpret_cast<u32x4 *>(tmp) = *reinterpret_cast<const Vec *>(rp);
+#pragma unroll
+            for (int c = 0; c < V; ++c) v[c] += as_float(tmp[c]);
+          } else {
+            for (int c = 0; c < cols; ++c) v[c] += as_float(rp[c]);
+          }
+        }
+        T *yp = static_cast<T *>(g.y) + row * g.ldy + nc;
+#pragma unroll
+        for (int c = 0; c < V; ++c) tmp[c] = (T)v[c];
+        if (cols == V) *reinterpret_cast<Vec *>(yp) = *reinterpret_cast<const u32x4 *>(tmp);
+        else
+          for (int c = 0; c < cols; ++c) yp[c] = tmp[c];
+      }
+    }
+  }
+}
+
+// ---- gradient of the weight ---------------------------------------------------------------------------------------------------------
+struct WeightArgs {
+  const void *p, *q;   // [rows, np], [rows, nq]: out(i, j) = sum over rows of p[r, i] q[r, j]
+  void *out, *colsum;  // [G, np, nq] in T; column sums of p (sum_p) or q [G, np or nq], may be null
+  float *part;         // partial products of the chunks of groups that have several: [slots][np * nq + (colsum ? ns : 0)]
+  int64_t ldp, ldq, np, nq, ns;
+  Groups groups;
+  int64_t unit;        // rows of a chunk
+  int64_t tiles_p, tiles_q;
+  int sum_p;
+};
+
+template <typename T, int BM, int BN, int NBUF>
+__global__ __launch_bounds__(kThreads, 2) void mm_weight_kernel(const WeightArgs g) {
+  using E = Elem<T>;
+  using LA = Tile<T, BM>;
+  using LB = Tile<T, BN>;
+  constexpr int STAGE = LA::BYTES + LB::BYTES;
+  constexpr int EPI = 64 * (BN + 4) * 4;
+  __shared__ __attribute__((aligned(16))) char lds[NBUF * STAGE > EPI ? NBUF * STAGE : EPI];
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, wm = wave / 2, wn = wave % 2;
+  const int64_t tile = xcd_contiguous(blockIdx.x, gridDim.x), tiles = g.tiles_p * g.tiles_q;
+  const int64_t slot = tile / tiles, t = tile % tiles, i0 = (t / g.tiles_q) * BM, j0 = (t % g.tiles_q) * BN;
+  const Piece piece = piece_of(g.groups, g.unit, slot);
+  if (piece.group < 0) return;
+  const int64_t len = piece.end - piece.begin, r0 = piece.begin + piece.index * g.unit;
+  if (len > 0 ? r0 >= piece.end : piece.index > 0) return;   // (a group without rows still writes its zeros, once)
+  const int64_t r1 = len <= 0 ? r0 : (r0 + g.unit < piece.end ? r0 + g.unit : piece.end);
+  const bool whole = len <= g.unit;                          // this chunk is all of its group
+  const T *P = static_cast<const T *>(g.p), *Q = static_cast<const T *>(g.q);
+  const bool sums = g.colsum && (g.sum_p ? j0 == 0 : i0 == 0);
+
+  Accum<T, BM, BN> acc;
+  acc.clear();
+  StageR<T, BM, true> sa;
+  StageR<T, BN, true> sb;
+  sa.open(P, g.ldp, i0, g.np - i0, r0, r1);
+  sb.open(Q, g.ldq, j0, g.nq - j0, r0, r1);
+  sa.add = sums && g.sum_p;
+  sb.add = sums && !g.sum_p;
+  const int64_t k_len = r1 - r0;
+  if (k_len > 0) {
+    sa.load(0, tid);
+    sb.load(0, tid);
+    if constexpr (NBUF == 2) {
+      sa.store(lds, tid);
+      sb.store(lds + LA::BYTES, tid);
+      if (E::BK < k_len) {
+        sa.load(E::BK, tid);
+        sb.load(E::BK, tid);
+      }
+      __syncthreads();
+      int cur = 0;
+      for (int64_t k0 = 0; k0 < k_len; k0 += E::BK) {
+        char *now = lds + cur * STAGE, *next = lds + (cur ^ 1) * STAGE;
+        acc.step(now, now + LA::BYTES, wm, wn, lane);
+        if (k0 + E::BK < k_len) {
+          sa.store(next, tid);
+          sb.store(next + LA::BYTES, tid);
+          if (k0 + 2 * E::BK < k_len) {
+            sa.load(k0 + 2 * E::BK, tid);
+            sb.load(k0 + 2 * E::BK, tid);
+          }
+        }
+        __syncthreads();
+        cur ^= 1;
+      }
+    } else {
+      for (int64_t k0 = 0; k0 < k_len; k0 += E::BK) {
+        sa.store(lds, tid);
+        sb.store(lds + LA::BYTES, tid);
+        if (k0 + E::BK < k_len) {
+          sa.load(k0 + E::BK, tid);
+          sb.load(k0 + E::BK, tid);
+        }
+        __syncthreads();
+        acc.step(lds, lds + LA::BYTES, wm, wn, lane);
+        __syncthreads();
+      }
+    }
+  }
+
+  const int64_t per_slot = g.np * g.nq + (g.colsum ? g.ns : 0);
+  float *out = reinterpret_cast<float *>(lds);
+  const int col = (tid % (BN / 4)) * 4;
+#pragma unroll
+  for (int i = 0; i < BM / 64; ++i) {
+    if (i) __syncthreads();
+    acc.put(out, i, wm, wn, lane);
+    __syncthreads();
+    for (int lr = tid / (BN / 4); lr < 64; lr += kThreads / (BN / 4)) {
+      const int64_t row = i0 + (lr / 32) * (BM / 2) + i * 32 + lr % 32;
+      if (row >= g.np) continue;
+      const f32x4 q = *reinterpret_cast<const f32x4 *>(out + lr * (BN + 4) + col);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int64_t cc = j0 + col + c;
+        if (cc >= g.nq) break;
+        float v = q[c];
+        if constexpr (E::PARTS == 3) {
+          if (!finite(v))
+            v = element_again(reinterpret_cast<const float *>(P) + r0 * g.ldp + row, g.ldp, reinterpret_cast<const float *>(Q) + r0 * g.ldq + cc, g.ldq,
+                              k_len);
+        }
+        if (whole) static_cast<T *>(g.out)[(piece.group * g.np + row) * g.nq + cc] = (T)v;
+        else g.part[slot * per_slot + row * g.nq + cc] = v;
+      }
+    }
+  }
+
+  if (sums) { // (uniform over the workgroup) column sums: CK threads hold each column's share
+    __syncthreads();
+    auto fold = [&](auto &st, int R, int64_t first, int64_t n) {
+      using S = typename std::remove_reference<decltype(st)>::type;
+#pragma unroll
+      for (int i = 0; i < S::N; ++i) {
+        const int idx = tid + i * kThreads;
+        if (idx < S::BLOCKS) {
+          const int row = (idx % (R / S::VR)) * S::VR, chunk = idx / (R / S::VR);
+#pragma unroll
+          for (int r = 0; r < S::VR; ++r) out[chunk * R + row + r] = st.sum[i][r];
+        }
+      }
+      __syncthreads();
+      for (int c = tid; c < R && first + c < n; c += kThreads) {
+        float s = 0.0f;
+        for (int k = 0; k < E::BK / 8; ++k) s += out[k * R + c];
+        if (whole) static_cast<T *>(g.colsum)[piece.group * g.ns + first + c] = (T)s;
+        else g.part[slot * per_slot + g.np * g.nq + first + c] = s;
+      }
+    };
+    if (g.sum_p) fold(sa, BM, i0, g.np);
+    else fold(sb, BN, j0, g.nq);
+  }
+}
+
+// The chunks of a group, added in their order by 16 threads an element (each every 16th chunk, then the 16 by halves).
+template <typename T> __global__ __launch_bounds__(kThreads) void mm_join_kernel(const WeightArgs g) {
+  __shared__ float part[kThreads];
+  const int64_t group = blockIdx.y;
+  Piece piece;
+  if (!g.groups.ptr) piece = {0, 0, g.groups.rows, 0, 0};
+  else {
+    const int64_t q0 = g.groups.bound(group + 1), q1 = g.groups.bound(group + 2);
+    piece = {group, q0, q1, 0, q0 / g.unit + group + 1};
+  }
+  const int64_t len = piece.end - piece.begin;
+  if (len <= g.unit) return;
+  const int64_t chunks = (len + g.unit - 1) / g.unit;
+  const int64_t size = g.np * g.nq, per_slot = size + (g.colsum ? g.ns : 0);
+  const int lane = threadIdx.x % 16, way = threadIdx.x / 16;
+  for (int64_t base = (int64_t)blockIdx.x * 16; base < per_slot; base += (int64_t)gridDim.x * 16) {
+    const int64_t i = base + lane;
+    float s = 0.0f;
+    if (i < per_slot) {
+#pragma unroll 4
+      for (int64_t c = way; c < chunks; c += 16) s += g.part[(piece.start + c) * per_slot + i];
+    }
+    part[threadIdx.x] = s;
+    __syncthreads();
+#pragma unroll
+    for (int h = 128; h >= 16; h /= 2) {
+      if ((int)threadIdx.x < h) part[threadIdx.x] += part[threadIdx.x + h];
+      __syncthreads();
+    }
+    if (way == 0 && i < per_slot) {
+      if (i < size) static_cast<T *>(g.out)[group * size + i] = (T)part[lane];
+      else static_cast<T *>(g.colsum)[group * g.ns + i - size] = (T)part[lane];
+    }
+    __syncthreads();
+  }
+}
+
+// ---- the activation's gradient: dz = dy * act'(z) -----------------------------------------------------------------------------------
+template <typename T> __global__ __launch_bounds__(kThreads) void act_backward_kernel(const T *dy, const T *z, T *dz, int64_t n, int act) {
+  constexpr int V = 16 / sizeof(T);
+  using Vec = Packed16<T>;
+  const int64_t step = (int64_t)gridDim.x * kThreads * V;
+  for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * V; i < n; i += step) {
+    if (i + V <= n) {
+      alignas(16) T a[V], b[V];
+      *reinterpret_cast<u32x4 *>(a) = *reinterpret_cast<const Vec *>(dy + i);
+      *reinterpret_cast<u32x4 *>(b) = *reinterpret_cast<const Vec *>(z + i);
+#pragma unroll
+      for (int v = 0; v < V; ++v) a[v] = (T)(as_float(a[v]) * activation_slope(as_float(b[v]), act));
+      *reinterpret_cast<Vec *>(dz + i) = *reinterpret_cast<const u32x4 *>(a);
+    } else {
+      for (int64_t j = i; j < n; ++j) dz[j] = (T)(as_float(dy[j]) * activation_slope(as_float(z[j]), act));
+    }
+  }
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------------------------
+int launched(const char *name) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return geot_internal_fail(GEOT_ELAUNCH, hipGetErrorString(e));
+  if (name) geot_internal_note_kernel(name);
+  return GEOT_OK;
+}
+
+constexpr int64_t kMaxBlocks = ((int64_t)1 << 31) - 1;
+
+template <typename T, int BM, int BN, bool BR> int run_rows(RowsArgs &g, hipStream_t st) {
+  constexpr int NBUF = Elem<T>::PARTS == 1 ? 2 : 1;
+  g.tiles_n = (g.n + BN - 1) / BN;
+  const int64_t slots = slots_of(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, BM);
+  if (slots > kMaxBlocks / g.tiles_n) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
+  hipLaunchKernelGGL((mm_rows_kernel<T, BM, BN, BR, NBUF>), dim3((unsigned)(slots * g.tiles_n)), dim3(kThreads), 0, st, g);
+  return launched("mm_rows_kernel");
+}
+template <typename T, bool BR> int rows_typed(RowsArgs &g, hipStream_t st) {
+  return g.n <= 64 ? run_rows<T, 128, 64, BR>(g, st) : run_rows<T, 128, 128, BR>(g, st);
+}
+int rows_product(RowsArgs &g, bool br, int dtype, hipStream_t st) {
+  if (g.groups.rows == 0 || g.n == 0) return GEOT_OK;
+  switch (dtype) {
+  case GEOT_F32: return br ? rows_typed<float, true>(g, st) : rows_typed<float, false>(g, st);
+  case GEOT_F16: return br ? rows_typed<f16, true>(g, st) : rows_typed<f16, false>(g, st);
+  case GEOT_BF16: return br ? rows_typed<bf16, true>(g, st) : rows_typed<bf16, false>(g, st);
+  }
+  return geot_internal_fail(GEOT_EUNSUPPORTED, "matrix products take float32, float16 and bfloat16");
+}
+
+// Chunks of rows.  Enough workgroups to fill the chip (kWeightBlocks), and no chunk below 256 rows.
+constexpr int64_t kWeightBlocks = 1024;
+struct WeightPlan {
+  int64_t tiles_p, tiles_q, unit, slots;
+};
+WeightPlan weight_plan(int64_t rows, int64_t groups, bool with_ptr, int64_t np, int64_t nq) {
+  WeightPlan w;
+  const int64_t bm = np <= 64 ? 64 : 128, bn = nq <= 64 ? 64 : 128;
+  w.tiles_p = np > 0 ? (np + bm - 1) / bm : 1; // (a side of width 0 still has its column sums)
+  w.tiles_q = nq > 0 ? (nq + bn - 1) / bn : 1;
+  const int64_t tiles = w.tiles_p * w.tiles_q;
+  const int64_t want = kWeightBlocks / tiles > 1 ? kWeightBlocks / tiles : 1;
+  w.unit = (rows + want - 1) / want;
+  w.unit = w.unit < 256 ? 256 : (w.unit + 63) / 64 * 64;
+  w.slots = with_ptr ? rows / w.unit + groups + 2 : (rows + w.unit - 1) / w.unit;
+  if (w.slots < 1) w.slots = 1;
+  return w;
+}
+template <typename T, int BM, int BN> int run_weight(WeightArgs &g, int64_t slots, hipStream_t st) {
+  constexpr int NBUF = Elem<T>::PARTS == 1 ? 2 : 1;
+  const int64_t tiles = g.tiles_p * g.tiles_q;
+  if (slots > kMaxBlocks / tiles) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
+  hipLaunchKernelGGL((mm_weight_kernel<T, BM, BN, NBUF>), dim3((unsigned)(slots * tiles)), dim3(kThreads), 0, st, g);
+  if (const int rc = launched("mm_weight_kernel")) return rc;
+  if (g.groups.rows > g.unit) { // some group may have several chunks
+    const int64_t per = (g.np * g.nq + (g.colsum ? g.ns : 0) + 15) / 16;
+    hipLaunchKernelGGL((mm_join_kernel<T>), dim3((unsigned)(per < 2048 ? per : 2048), (unsigned)g.groups.groups), dim3(kThreads), 0, st, g);
+    return launched(nullptr);
+  }
+  return GEOT_OK;
+}
+template <typename T> int weight_typed(WeightArgs &g, int64_t slots, hipStream_t st) {
+  if (g.np <= 64) return g.nq <= 64 ? run_weight<T, 64, 64>(g, slots, st) : run_weight<T, 64, 128>(g, slots, st);
+  return g.nq <= 64 ? run_weight<T, 128, 64>(g, slots, st) : run_weight<T, 128, 128>(g, slots, st);
+}
+int weight_product(WeightArgs &g, int dtype, void *workspace, size_t workspace_bytes, hipStream_t st) {
+  if (g.groups.groups == 0 || (g.np * g.nq == 0 && !(g.colsum && g.ns > 0))) return GEOT_OK;
+  const WeightPlan w = weight_plan(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, g.np, g.nq);
+  g.unit = w.unit;
+  g.tiles_p = w.tiles_p;
+  g.tiles_q = w.tiles_q;
+  g.part = static_cast<float *>(workspace);
+  if (g.groups.rows > w.unit) {
+    const size_t need = (size_t)w.slots * (size_t)(g.np * g.nq + (g.colsum ? g.ns : 0)) * sizeof(float);
+    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) return geot_internal_fail(GEOT_EWORKSPACE, "weight gradient: workspace too small or misaligned");
+  }
+  switch (dtype) {
+  case GEOT_F32: return weight_typed<float>(g, w.slots, st);
+  case GEOT_F16: return weight_typed<f16>(g, w.slots, st);
+  case GEOT_BF16: return weight_typed<bf16>(g, w.slots, st);
+  }
+  return geot_internal_fail(GEOT_EUNSUPPORTED, "matrix products take float32, float16 and bfloat16");
+}
+
+bool bad_size(int64_t a, int64_t b, int64_t c) {
+  constexpr int64_t lim = (int64_t)1 << 40;
+  return a < 0 || b < 0 || c < 0 || a > lim || b > lim || c > lim;
+}
+
+} // namespace
+
+extern "C" {
+
+int geot_linear(const void *x, int64_t ldx, const void *weight, const void *bias, const void *residual, int64_t ld_residual, void *z, void *y,
+                int64_t rows, int64_t in, int64_t out, int activation, int dtype, void *stream) {
+  if (bad_size(rows, in, out) || ldx < 0 || ld_residual < 0) return geot_internal_fail(GEOT_EINVAL, "geot_linear: negative size");
+  if (activation < GEOT_ACT_NONE || activation > GEOT_ACT_SILU) return geot_internal_fail(GEOT_EINVAL, "geot_linear: unknown activation");
+  if (rows > 0 && out > 0 && (!y || (in > 0 && (!x || !weight)))) return geot_internal_fail(GEOT_EINVAL, "geot_linear: null pointer");
+  RowsArgs g{};
+  g.a = x; g.lda = ldx; g.b = weight; g.ldb = in; g.bias = bias; g.residual = residual; g.ldr = ld_residual; g.z = z; g.y = y; g.ldy = out;
+  g.groups = {nullptr, 1, rows}; g.n = out; g.k = in; g.act = activation;
+  return rows_product(g, false, dtype, static_cast<hipStream_t>(stream));
+}
+
+int geot_linear_grad_input(const void *dz, const void *weight, void *dx, int64_t rows, int64_t in, int64_t out, int dtype, void *stream) {
+  if (bad_size(rows, in, out)) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_input: negative size");
+  if (rows > 0 && in > 0 && (!dx || (out > 0 && (!dz || !weight)))) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_input: null pointer");
+  RowsArgs g{};
+  g.a = dz; g.lda = out; g.b = weight; g.ldb = in; g.y = dx; g.ldy = in;
+  g.groups = {nullptr, 1, rows}; g.n = in; g.k = out; g.act = GEOT_ACT_NONE;
+  return rows_product(g, true, dtype, static_cast<hipStream_t>(stream));
+}
+
+size_t geot_linear_grad_weight_workspace_bytes(int64_t rows, int64_t in, int64_t out) {
+  if (bad_size(rows, in, out)) return 0;
+  const WeightPlan w = weight_plan(rows, 1, false, out, in);
+  return rows > w.unit ? (size_t)w.slots * (size_t)(in * out + out) * sizeof(float) : 0;
+}
+
+int geot_linear_grad_weight(const void *dz, const void *x, int64_t ldx, void *dweight, void *dbias, int64_t rows, int64_t in, int64_t out, int dtype,
+                            void *workspace, size_t workspace_bytes, void *stream) {
+  if (bad_size(rows, in, out) || ldx < 0) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_weight: negative size");
+  if (in > 0 && out > 0 && (!dweight || (rows > 0 && (!dz || !x)))) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_weight: null pointer");
+  WeightArgs g{};
+  g.p = dz; g.ldp = out; g.np = out; g.q = x; g.ldq = ldx; g.nq = in; g.out = dweight; g.colsum = dbias; g.ns = out; g.sum_p = 1;
+  g.groups = {nullptr, 1, rows};
+  return weight_product(g, dtype, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+int geot_activation_backward(const void *dy, const void *z, void *dz, int64_t n, int activation, int dtype, void *stream) {
+  if (n < 0 || (n > 0 && (!dy || !z || !dz))) return geot_internal_fail(GEOT_EINVAL, "geot_activation_backward: bad argument");
+  if (activation < GEOT_ACT_NONE || activation > GEOT_ACT_SILU) return geot_internal_fail(GEOT_EINVAL, "geot_activation_backward: unknown activation");
+  if (n == 0) return GEOT_OK;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t vec = dtype == GEOT_F32 ? 4 : 8, want = (n + vec * kThreads - 1) / (vec * kThreads);
+  const unsigned blocks = (unsigned)(want < 8192 ? want : 8192);
+  switch (dtype) {
+  case GEOT_F32: hipLaunchKernelGGL(act_backward_kernel<float>, dim3(blocks), dim3(kThreads), 0, st, (const float *)dy, (const float *)z, (float *)dz, n, activation); break;
+  case GEOT_F16: hipLaunchKernelGGL(act_backward_kernel<f16>, dim3(blocks), dim3(kThreads), 0, st, (const f16 *)dy, (const f16 *)z, (f16 *)dz, n, activation); break;
+  case GEOT_BF16: hipLaunchKernelGGL(act_backward_kernel<bf16>, dim3(blocks), dim3(kThreads), 0, st, (const bf16 *)dy, (const bf16 *)z, (bf16 *)dz, n, activation); break;
+  default: return geot_internal_fail(GEOT_EUNSUPPORTED, "geot_activation_backward: float32, float16 and bfloat16");
+  }
+  return launched("act_backward_kernel");
+}
+
+int geot_segment_matmul(const void *x, int64_t ldx, const int64_t *ptr, const void *weight, const void *bias, void *y, int64_t rows, int64_t groups,
+                        int64_t in, int64_t out, int dtype, void *stream) {
+  if (bad_size(rows, in, out) || groups < 0 || groups > 65535 || ldx < 0) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul: negative size, or more than 65535 groups");
+  if (rows > 0 && out > 0 && (!y || !ptr || (in > 0 && groups > 0 && (!x || !weight)))) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul: null pointer");
+  RowsArgs g{};
+  g.a = x; g.lda = ldx; g.b = weight; g.ldb = out; g.b_group = in * out; g.bias = bias; g.bias_group = out; g.y = y; g.ldy = out;
+  g.groups = {ptr, groups, rows}; g.n = out; g.k = in; g.act = GEOT_ACT_NONE;
+  return rows_product(g, true, dtype, static_cast<hipStream_t>(stream));
+}
+
+int geot_segment_matmul_grad_input(const void *dy, const int64_t *ptr, const void *weight, void *dx, int64_t rows, int64_t groups, int64_t in, int64_t out,
+                                   int dtype, void *stream) {
+  if (bad_size(rows, in, out) || groups < 0 || groups > 65535) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul_grad_input: negative size, or more than 65535 groups");
+  if (rows > 0 && in > 0 && (!dx || !ptr || (out > 0 && groups > 0 && (!dy || !weight)))) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul_grad_input: null pointer");
+  RowsArgs g{};
+  g.a = dy; g.lda = out; g.b = weight; g.ldb = out; g.b_group = in * out; g.y = dx; g.ldy = in;
+  g.groups = {ptr, groups, rows}; g.n = in; g.k = out; g.act = GEOT_ACT_NONE;
+  return rows_product(g, false, dtype, static_cast<hipStream_t>(stream));
+}
+
+size_t geot_segment_matmul_grad_weight_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out) {
+  if (bad_size(rows, in, out) || groups < 0 || groups > 65535) return 0;
+  const WeightPlan w = weight_plan(rows, groups, true, in, out);
+  return rows > w.unit ? (size_t)w.slots * (size_t)(in * out + out) * sizeof(float) : 0;
+}
+
+int geot_segment_matmul_grad_weight(const void *x, int64_t ldx, const int64_t *ptr, const void *dy, void *dweight, void *dbias, int64_t rows, int64_t groups,
+                                    int64_t in, int64_t out, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+  if (bad_size(rows, in, out) || groups < 0 || groups > 65535 || ldx < 0) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul_grad_weight: negative size, or more than 65535 groups");
+  if (groups > 0 && in > 0 && out > 0 && (!ptr || !dweight || (rows > 0 && (!x || !dy)))) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul_grad_weight: null pointer");
+  WeightArgs g{};
+  g.p = x; g.ldp = ldx; g.np = in; g.q = dy; g.ldq = out; g.nq = out; g.out = dweight; g.colsum = dbias; g.ns = out; g.sum_p = 0;
+  g.groups = {ptr, groups, rows};
+  return weight_product(g, dtype, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+} // extern "C"

@@ -439,6 +439,139 @@ torch.library.register_autograd("geot::index_scatter", _is_backward, setup_conte
 
 
 # --------------------------------------------------------------------------------------------------
+# dense rows (csrc/host_dense.cpp): fake-tensor rules and autograd formulas of the differentiable forms
+# --------------------------------------------------------------------------------------------------
+def _fake_linear(x, weight, bias, residual, activation, save=True):
+    y = x.new_empty([*x.shape[:-1], weight.shape[0]])
+    keep = save and activation != "none" and not (activation == "relu" and residual is None)
+    return y, (torch.empty_like(y) if keep else x.new_empty([0]))
+
+
+torch.library.register_fake("geot::linear_forward")(_fake_linear)
+
+
+@torch.library.register_fake("geot::linear_train")
+def _(x, weight, bias, residual, activation):
+    return _fake_linear(x, weight, bias, residual, activation)
+
+
+@torch.library.register_fake("geot::linear_backward")
+def _(grad, x, weight, z, activation, need_x, need_weight, need_bias):
+    return (x.new_empty(x.shape if need_x else [0]), weight.new_empty(weight.shape if need_weight else [0]),
+            weight.new_empty([weight.shape[0] if need_bias else 0]))
+
+
+def _fake_segment_matmul(x, ptr, weight, bias):
+    return x.new_empty([x.shape[0], weight.shape[2]])
+
+
+torch.library.register_fake("geot::segment_matmul_forward")(_fake_segment_matmul)
+torch.library.register_fake("geot::segment_matmul_train")(_fake_segment_matmul)
+
+
+@torch.library.register_fake("geot::segment_matmul_backward")
+def _(grad, x, ptr, weight, need_x, need_weight, need_bias):
+    return (x.new_empty(x.shape if need_x else [0]), weight.new_empty(weight.shape if need_weight else [0]),
+            weight.new_empty([weight.shape[0], weight.shape[2]] if need_bias else [0]))
+
+
+def _fake_layer_norm(x, weight, bias, eps, save=True):
+    rows = 1
+    for n in x.shape[:-1]:
+        rows = rows * n
+    return x.new_empty(x.shape), x.new_empty([3 if save else 0, rows], dtype=torch.float32)
+
+
+torch.library.register_fake("geot::layer_norm_forward")(_fake_layer_norm)
+
+
+@torch.library.register_fake("geot::layer_norm_train")
+def _(x, weight, bias, eps):
+    return _fake_layer_norm(x, weight, bias, eps)
+
+
+@torch.library.register_fake("geot::layer_norm_backward")
+def _(grad, x, weight, bias, stats, need_params):
+    dtype = next((p.dtype for p in (weight, bias) if p is not None), x.dtype)
+    n = x.shape[-1] if need_params else 0
+    return x.new_empty(x.shape), x.new_empty([n], dtype=dtype), x.new_empty([n], dtype=dtype)
+
+
+def _once(name: str) -> None:
+    """These backward passes have no gradient of their own; a caller that asks for one (create_graph) is told so."""
+    if torch.is_grad_enabled():
+        raise NotImplementedError(f"{name}: the backward pass is not differentiable (create_graph=True is not supported)")
+
+
+def _linear_setup(ctx, inputs, output):
+    x, weight, bias, residual, activation = inputs
+    y, z = output
+    ctx.activation = activation
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(z)
+    # relu without a residual: y has z's sign, nothing else is kept
+    ctx.save_for_backward(x, weight, y if activation == "relu" and residual is None else z)
+
+
+def _linear_backward(ctx, grad, _grad_z):
+    """y = act(z) + residual, z = x W^T + b:  dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = column sums of dz;  dresidual = dy."""
+    if grad is None:
+        return None, None, None, None, None
+    _once("linear")
+    x, weight, z = ctx.saved_tensors
+    need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+    dx = dw = db = None
+    if need_x or need_w or need_b:
+        dx, dw, db = torch.ops.geot.linear_backward(grad, x, weight, z, ctx.activation, need_x, need_w, need_b)
+    return dx if need_x else None, dw if need_w else None, db if need_b else None, grad if need_r else None, None
+
+
+torch.library.register_autograd("geot::linear_train", _linear_backward, setup_context=_linear_setup)
+
+
+def _segment_matmul_setup(ctx, inputs, output):
+    x, ptr, weight, _bias = inputs
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(x, ptr, weight)
+
+
+def _segment_matmul_backward(ctx, grad):
+    """Per group g:  dx = dy W[g]^T;  dW[g] = x_g^T dy_g;  db[g] = column sums of dy_g."""
+    if grad is None:
+        return None, None, None, None
+    _once("segment_matmul")
+    x, ptr, weight = ctx.saved_tensors
+    need_x, _, need_w, need_b = ctx.needs_input_grad
+    dx, dw, db = torch.ops.geot.segment_matmul_backward(grad, x, ptr, weight, need_x, need_w, need_b)
+    return dx if need_x else None, None, dw if need_w else None, db if need_b else None
+
+
+torch.library.register_autograd("geot::segment_matmul_train", _segment_matmul_backward, setup_context=_segment_matmul_setup)
+
+
+def _layer_norm_setup(ctx, inputs, output):
+    x, weight, bias, _eps = inputs
+    _y, stats = output
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(stats)
+    ctx.save_for_backward(x, weight, bias, stats)
+
+
+def _layer_norm_backward(ctx, grad, _grad_stats):
+    """h = (x - mean) rstd, g = dy w:  dx = rstd (g - mean g - h mean(g h));  dw = sum over rows of dy h;  db = sum over rows of dy."""
+    if grad is None:
+        return None, None, None, None
+    _once("layer_norm")
+    x, weight, bias, stats = ctx.saved_tensors
+    need_x, need_w, need_b, _ = ctx.needs_input_grad
+    dx, dw, db = torch.ops.geot.layer_norm_backward(grad, x, weight, bias, stats, need_w or need_b)
+    return dx if need_x else None, dw if need_w else None, db if need_b else None, None
+
+
+torch.library.register_autograd("geot::layer_norm_train", _layer_norm_backward, setup_context=_layer_norm_setup)
+
+
+# --------------------------------------------------------------------------------------------------
 # public functions (geot/*.py)
 # --------------------------------------------------------------------------------------------------
 def index_scatter(dim: int, src: torch.Tensor, index: torch.Tensor, reduce: str = "sum",
@@ -530,3 +663,33 @@ def coo_to_csr(coo_row: torch.Tensor) -> torch.Tensor:
 def _(coo_row):
     ctx = torch.library.get_ctx()
     return coo_row.new_empty([ctx.new_dynamic_size()], dtype=torch.int32)
+
+
+# --------------------------------------------------------------------------------------------------
+# dense rows: what stands around the aggregations in a layer (the reference's models use torch.nn.Linear there)
+# --------------------------------------------------------------------------------------------------
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+           activation: str = "none") -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual`` in one kernel: x [..., in], weight [out, in] (torch.nn.Linear's layout), bias [out],
+    residual [..., out]; ``activation``: 'none', 'relu', 'gelu' (the error-function form) or 'silu'.
+
+    float32, float16 or bfloat16, one dtype for all operands; sums in float32, one rounding.  Differentiable in every tensor (the
+    backward pass itself is not).  A training call keeps the pre-activation in the operands' dtype ('none', and 'relu' without a
+    residual, keep nothing)."""
+    return torch.ops.geot.linear(x, weight, bias, residual, activation)
+
+
+def segment_matmul(x: torch.Tensor, ptr: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Row groups times their own matrices: ``out[i] = x[i] @ weight[g] (+ bias[g])`` for ``ptr[g] <= i < ptr[g + 1]`` - the typed
+    transform of a heterogeneous graph, the products of routed experts (call shape of pyg_lib's ``segment_matmul``).
+
+    x [rows, in], ptr int64 [groups + 1] ascending, on the GPU (never read back: the call does not synchronise), weight
+    [groups, in, out], bias [groups, out]; float32, float16 or bfloat16.  Groups may be empty; rows in front of ptr[0] and behind ptr[-1]
+    come out 0.  Entries of ptr that do not ascend leave the result unspecified.  Differentiable in x, weight and bias."""
+    return torch.ops.geot.segment_matmul(x, ptr, weight, bias)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """Normalisation of the last dimension: ``(x - mean) / sqrt(var + eps) * weight + bias``; weight / bias [x.shape[-1]], of x's dtype or
+    float32.  float32, float16 or bfloat16 rows, statistics in float32.  Differentiable in x, weight and bias."""
+    return torch.ops.geot.layer_norm(x, weight, bias, eps)

@@ -381,6 +381,51 @@ int geot_slab_mh_sddmm(const geot_slab_plan *plan, const void *mat_1, const void
  * sorted = 1 on faith for reductions other than sum (probe first: geot_index_probe).  The reference tolerates a wrong
  * `sorted` promise for sum only (its kernels ignore `reduce` on the GPU): this is a documented difference. */
 
+/* ---- dense rows: the products and the normalisation of a layer's node / edge rows ------------------------------------------------
+ * Operators the reference does not have (its models call torch.nn.Linear and LayerNorm around the aggregations).  dtype: GEOT_F32,
+ * GEOT_F16 or GEOT_BF16 for every operand; sums in float32, one rounding at the end.  Matrices are row-major; `ldx` / `ld_residual` is
+ * the distance of two rows in elements (>= the row's width, or 0 for one repeated row), every other operand is dense.  Operands need no alignment beyond their
+ * element's.  No call allocates or synchronises; results do not depend on the launch (no atomics).
+ *
+ * geot_linear:  y = act(x weight^T + bias) + residual     x [rows, in], weight [out, in], bias [out] or NULL, residual [rows, out] or
+ * NULL, y [rows, out]; z [rows, out] or NULL receives x weight^T + bias (what the backward pass of the activation needs). */
+enum { GEOT_ACT_NONE = 0, GEOT_ACT_RELU = 1, GEOT_ACT_GELU = 2 /* z * Phi(z), the error-function form */, GEOT_ACT_SILU = 3 };
+int geot_linear(const void *x, int64_t ldx, const void *weight, const void *bias, const void *residual, int64_t ld_residual, void *z,
+                void *y, int64_t rows, int64_t in, int64_t out, int activation, int dtype, void *stream);
+/* dz[i] = dy[i] * act'(z[i]); dz may be dy.  For relu z may be y (they have one sign). */
+int geot_activation_backward(const void *dy, const void *z, void *dz, int64_t n, int activation, int dtype, void *stream);
+/* dx = dz weight   [rows, in] */
+int geot_linear_grad_input(const void *dz, const void *weight, void *dx, int64_t rows, int64_t in, int64_t out, int dtype, void *stream);
+/* dweight = dz^T x [out, in]; dbias = column sums of dz [out] or NULL.  The rows are split over workgroups and the parts joined in a
+ * fixed order; `workspace`: geot_linear_grad_weight_workspace_bytes, 16-byte aligned, no content expected, free after the call. */
+size_t geot_linear_grad_weight_workspace_bytes(int64_t rows, int64_t in, int64_t out);
+int geot_linear_grad_weight(const void *dz, const void *x, int64_t ldx, void *dweight, void *dbias, int64_t rows, int64_t in, int64_t out,
+                            int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/* geot_segment_matmul:  y[i] = x[i] weight[g] + bias[g]  for ptr[g] <= i < ptr[g + 1]     ptr [groups + 1] ascending, weight
+ * [groups, in, out], bias [groups, out] or NULL (groups <= 65535).  Rows in front of ptr[0] and behind ptr[groups] come out 0, as do
+ * their gradients; a group without rows has gradient 0.  Entries of ptr are clamped into [0, rows]; with entries that do not ascend the
+ * result is unspecified, but nothing outside the operands is touched. */
+int geot_segment_matmul(const void *x, int64_t ldx, const int64_t *ptr, const void *weight, const void *bias, void *y, int64_t rows,
+                        int64_t groups, int64_t in, int64_t out, int dtype, void *stream);
+/* dx[i] = dy[i] weight[g]^T   [rows, in] */
+int geot_segment_matmul_grad_input(const void *dy, const int64_t *ptr, const void *weight, void *dx, int64_t rows, int64_t groups, int64_t in,
+                                   int64_t out, int dtype, void *stream);
+/* dweight[g] = x_g^T dy_g [groups, in, out]; dbias[g] = column sums of dy_g [groups, out] or NULL */
+size_t geot_segment_matmul_grad_weight_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out);
+int geot_segment_matmul_grad_weight(const void *x, int64_t ldx, const int64_t *ptr, const void *dy, void *dweight, void *dbias, int64_t rows,
+                                    int64_t groups, int64_t in, int64_t out, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/* geot_layer_norm:  y = (x - mean) * rstd * weight + bias over each row of x [rows, feat]; weight / bias [feat] or NULL, of `dtype` or
+ * float32 (param_dtype).  stats [3, rows] float32 or NULL receives what the backward pass needs: the mean as two parts whose sum it is, and
+ * rstd = 1 / sqrt(var + eps).  dx [rows, feat], dweight / dbias [feat] in param_dtype, both or neither. */
+int geot_layer_norm(const void *x, int64_t ldx, const void *weight, const void *bias, void *y, float *stats, int64_t rows, int64_t feat,
+                    float eps, int dtype, int param_dtype, void *stream);
+size_t geot_layer_norm_backward_workspace_bytes(int64_t rows, int64_t feat);
+int geot_layer_norm_backward(const void *x, int64_t ldx, const void *weight, const float *stats, const void *dy, void *dx, void *dweight,
+                             void *dbias, int64_t rows, int64_t feat, int dtype, int param_dtype, void *workspace, size_t workspace_bytes,
+                             void *stream);
+
 #ifdef __cplusplus
 }
 #endif
