@@ -1,10 +1,11 @@
-// host_dense.cpp -- the geot::* operators on dense rows: linear, segment_matmul, layer_norm (kernels: csrc/dense_mm.hip, csrc/row_norm.hip).
+// host_dense.cpp -- the geot_dense::* operators on dense rows: linear, segment_matmul, layer_norm (kernels: csrc/dense_mm.hip, csrc/row_norm.hip).
 //
-// The reference has no such operators (its models call torch.nn.Linear and torch.nn.LayerNorm around the aggregations).  Each comes as
-//   geot::<op>            what a user calls: looks whether a gradient is asked for and goes to one of
-//   geot::<op>_forward    the kernel, nothing kept for a backward pass (inference stays out of Python altogether)
-//   geot::<op>_train      the differentiable form; its fake-tensor rule and autograd formula are in geot_amd/ops.py, over
-//   geot::<op>_backward   the gradients
+// The reference has no such operators (its models call torch.nn.Linear and torch.nn.LayerNorm around the aggregations); they live in a
+// dispatcher namespace of their own, so that `geot` holds what the reference's layers define and expect there.  Each comes as
+//   geot_dense::<op>            what a user calls: looks whether a gradient is asked for and goes to one of
+//   geot_dense::<op>_forward    the kernel, nothing kept for a backward pass (inference stays out of Python altogether)
+//   geot_dense::<op>_train      the differentiable form; its fake-tensor rule and autograd formula are in geot_amd/ops.py, over
+//   geot_dense::<op>_backward   the gradients
 // Every call runs on its tensors' device and that device's current stream, allocates what it needs from torch's caching allocator (under
 // capture: from the graph's own pool, so two captured graphs share no scratch) and neither synchronises nor remembers anything.
 #include "host.h"
@@ -105,7 +106,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward_op(const at::Tens
   check_linear(x_in, w_in, c10::nullopt, grad_in);
   const int act = activation_code(activation);
   TORCH_CHECK(act == GEOT_ACT_NONE || (z_in.sizes() == grad_in.sizes() && z_in.scalar_type() == grad_in.scalar_type()),
-              "linear: the backward pass of '", activation, "' needs what the differentiable forward (geot::linear_train) saved");
+              "linear: the backward pass of '", activation, "' needs what the differentiable forward (geot_dense::linear_train) saved");
   require_gpu("linear", {&grad_in, &x_in, &w_in, &z_in});
   const int dt = dense_dtype(x_in, "linear");
   GEOT_DEVICE_GUARD(x_in);
@@ -139,10 +140,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward_op(const at::Tens
 at::Tensor linear_op(const at::Tensor &x, const at::Tensor &w, const c10::optional<at::Tensor> &bias, const c10::optional<at::Tensor> &residual,
                      c10::string_view activation) {
   if (wants_grad({&x, &w, ptr_of(bias), ptr_of(residual)})) {
-    static const auto train = c10::Dispatcher::singleton().findSchemaOrThrow("geot::linear_train", "").typed<decltype(linear_train_op)>();
+    static const auto train = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::linear_train", "").typed<decltype(linear_train_op)>();
     return std::get<0>(train.call(x, w, bias, residual, activation));
   }
-  static const auto fwd = c10::Dispatcher::singleton().findSchemaOrThrow("geot::linear_forward", "").typed<decltype(linear_forward_op)>();
+  static const auto fwd = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::linear_forward", "").typed<decltype(linear_forward_op)>();
   return std::get<0>(fwd.call(x, w, bias, residual, activation, false));
 }
 
@@ -205,8 +206,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> segment_matmul_backward_op(const 
 }
 
 at::Tensor segment_matmul_op(const at::Tensor &x, const at::Tensor &ptr, const at::Tensor &w, const c10::optional<at::Tensor> &bias) {
-  static const auto train = c10::Dispatcher::singleton().findSchemaOrThrow("geot::segment_matmul_train", "").typed<decltype(segment_matmul_forward_op)>();
-  static const auto fwd = c10::Dispatcher::singleton().findSchemaOrThrow("geot::segment_matmul_forward", "").typed<decltype(segment_matmul_forward_op)>();
+  static const auto train = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::segment_matmul_train", "").typed<decltype(segment_matmul_forward_op)>();
+  static const auto fwd = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::segment_matmul_forward", "").typed<decltype(segment_matmul_forward_op)>();
   return wants_grad({&x, &w, ptr_of(bias)}) ? train.call(x, ptr, w, bias) : fwd.call(x, ptr, w, bias);
 }
 
@@ -265,16 +266,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_backward_op(const at::
 
 at::Tensor layer_norm_op(const at::Tensor &x, const c10::optional<at::Tensor> &w, const c10::optional<at::Tensor> &b, double eps) {
   if (wants_grad({&x, ptr_of(w), ptr_of(b)})) {
-    static const auto train = c10::Dispatcher::singleton().findSchemaOrThrow("geot::layer_norm_train", "").typed<decltype(layer_norm_train_op)>();
+    static const auto train = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::layer_norm_train", "").typed<decltype(layer_norm_train_op)>();
     return std::get<0>(train.call(x, w, b, eps));
   }
-  static const auto fwd = c10::Dispatcher::singleton().findSchemaOrThrow("geot::layer_norm_forward", "").typed<decltype(layer_norm_forward_op)>();
+  static const auto fwd = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::layer_norm_forward", "").typed<decltype(layer_norm_forward_op)>();
   return std::get<0>(fwd.call(x, w, b, eps, false));
 }
 
 } // namespace
 
-TORCH_LIBRARY_FRAGMENT(geot, m) {
+TORCH_LIBRARY_FRAGMENT(geot_dense, m) {
   m.def("linear(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, str activation) -> Tensor", linear_op);
   m.def("linear_forward(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, str activation, bool save) -> (Tensor, Tensor)");
   m.def("linear_train(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, str activation) -> (Tensor, Tensor)");
@@ -300,5 +301,5 @@ TORCH_LIBRARY_FRAGMENT(geot, m) {
   m.impl("layer_norm_forward", layer_norm_forward_op);                 \
   m.impl("layer_norm_train", layer_norm_train_op);                     \
   m.impl("layer_norm_backward", layer_norm_backward_op)
-TORCH_LIBRARY_IMPL(geot, CUDA, m) { GEOT_DENSE_IMPLS(m); }
-TORCH_LIBRARY_IMPL(geot, CPU, m) { GEOT_DENSE_IMPLS(m); }
+TORCH_LIBRARY_IMPL(geot_dense, CUDA, m) { GEOT_DENSE_IMPLS(m); }
+TORCH_LIBRARY_IMPL(geot_dense, CPU, m) { GEOT_DENSE_IMPLS(m); }

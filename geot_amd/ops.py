@@ -447,15 +447,15 @@ def _fake_linear(x, weight, bias, residual, activation, save=True):
     return y, (torch.empty_like(y) if keep else x.new_empty([0]))
 
 
-torch.library.register_fake("geot::linear_forward")(_fake_linear)
+torch.library.register_fake("geot_dense::linear_forward")(_fake_linear)
 
 
-@torch.library.register_fake("geot::linear_train")
+@torch.library.register_fake("geot_dense::linear_train")
 def _(x, weight, bias, residual, activation):
     return _fake_linear(x, weight, bias, residual, activation)
 
 
-@torch.library.register_fake("geot::linear_backward")
+@torch.library.register_fake("geot_dense::linear_backward")
 def _(grad, x, weight, z, activation, need_x, need_weight, need_bias):
     return (x.new_empty(x.shape if need_x else [0]), weight.new_empty(weight.shape if need_weight else [0]),
             weight.new_empty([weight.shape[0] if need_bias else 0]))
@@ -465,11 +465,11 @@ def _fake_segment_matmul(x, ptr, weight, bias):
     return x.new_empty([x.shape[0], weight.shape[2]])
 
 
-torch.library.register_fake("geot::segment_matmul_forward")(_fake_segment_matmul)
-torch.library.register_fake("geot::segment_matmul_train")(_fake_segment_matmul)
+torch.library.register_fake("geot_dense::segment_matmul_forward")(_fake_segment_matmul)
+torch.library.register_fake("geot_dense::segment_matmul_train")(_fake_segment_matmul)
 
 
-@torch.library.register_fake("geot::segment_matmul_backward")
+@torch.library.register_fake("geot_dense::segment_matmul_backward")
 def _(grad, x, ptr, weight, need_x, need_weight, need_bias):
     return (x.new_empty(x.shape if need_x else [0]), weight.new_empty(weight.shape if need_weight else [0]),
             weight.new_empty([weight.shape[0], weight.shape[2]] if need_bias else [0]))
@@ -482,15 +482,15 @@ def _fake_layer_norm(x, weight, bias, eps, save=True):
     return x.new_empty(x.shape), x.new_empty([3 if save else 0, rows], dtype=torch.float32)
 
 
-torch.library.register_fake("geot::layer_norm_forward")(_fake_layer_norm)
+torch.library.register_fake("geot_dense::layer_norm_forward")(_fake_layer_norm)
 
 
-@torch.library.register_fake("geot::layer_norm_train")
+@torch.library.register_fake("geot_dense::layer_norm_train")
 def _(x, weight, bias, eps):
     return _fake_layer_norm(x, weight, bias, eps)
 
 
-@torch.library.register_fake("geot::layer_norm_backward")
+@torch.library.register_fake("geot_dense::layer_norm_backward")
 def _(grad, x, weight, bias, stats, need_params):
     dtype = next((p.dtype for p in (weight, bias) if p is not None), x.dtype)
     n = x.shape[-1] if need_params else 0
@@ -522,11 +522,11 @@ def _linear_backward(ctx, grad, _grad_z):
     need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
     dx = dw = db = None
     if need_x or need_w or need_b:
-        dx, dw, db = torch.ops.geot.linear_backward(grad, x, weight, z, ctx.activation, need_x, need_w, need_b)
+        dx, dw, db = torch.ops.geot_dense.linear_backward(grad, x, weight, z, ctx.activation, need_x, need_w, need_b)
     return dx if need_x else None, dw if need_w else None, db if need_b else None, grad if need_r else None, None
 
 
-torch.library.register_autograd("geot::linear_train", _linear_backward, setup_context=_linear_setup)
+torch.library.register_autograd("geot_dense::linear_train", _linear_backward, setup_context=_linear_setup)
 
 
 def _segment_matmul_setup(ctx, inputs, output):
@@ -542,11 +542,11 @@ def _segment_matmul_backward(ctx, grad):
     _once("segment_matmul")
     x, ptr, weight = ctx.saved_tensors
     need_x, _, need_w, need_b = ctx.needs_input_grad
-    dx, dw, db = torch.ops.geot.segment_matmul_backward(grad, x, ptr, weight, need_x, need_w, need_b)
+    dx, dw, db = torch.ops.geot_dense.segment_matmul_backward(grad, x, ptr, weight, need_x, need_w, need_b)
     return dx if need_x else None, None, dw if need_w else None, db if need_b else None
 
 
-torch.library.register_autograd("geot::segment_matmul_train", _segment_matmul_backward, setup_context=_segment_matmul_setup)
+torch.library.register_autograd("geot_dense::segment_matmul_train", _segment_matmul_backward, setup_context=_segment_matmul_setup)
 
 
 def _layer_norm_setup(ctx, inputs, output):
@@ -564,11 +564,11 @@ def _layer_norm_backward(ctx, grad, _grad_stats):
     _once("layer_norm")
     x, weight, bias, stats = ctx.saved_tensors
     need_x, need_w, need_b, _ = ctx.needs_input_grad
-    dx, dw, db = torch.ops.geot.layer_norm_backward(grad, x, weight, bias, stats, need_w or need_b)
+    dx, dw, db = torch.ops.geot_dense.layer_norm_backward(grad, x, weight, bias, stats, need_w or need_b)
     return dx if need_x else None, dw if need_w else None, db if need_b else None, None
 
 
-torch.library.register_autograd("geot::layer_norm_train", _layer_norm_backward, setup_context=_layer_norm_setup)
+torch.library.register_autograd("geot_dense::layer_norm_train", _layer_norm_backward, setup_context=_layer_norm_setup)
 
 
 # --------------------------------------------------------------------------------------------------
@@ -676,7 +676,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     float32, float16 or bfloat16, one dtype for all operands; sums in float32, one rounding.  Differentiable in every tensor (the
     backward pass itself is not).  A training call keeps the pre-activation in the operands' dtype ('none', and 'relu' without a
     residual, keep nothing)."""
-    return torch.ops.geot.linear(x, weight, bias, residual, activation)
+    return torch.ops.geot_dense.linear(x, weight, bias, residual, activation)
 
 
 def segment_matmul(x: torch.Tensor, ptr: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -686,10 +686,10 @@ def segment_matmul(x: torch.Tensor, ptr: torch.Tensor, weight: torch.Tensor, bia
     x [rows, in], ptr int64 [groups + 1] ascending, on the GPU (never read back: the call does not synchronise), weight
     [groups, in, out], bias [groups, out]; float32, float16 or bfloat16.  Groups may be empty; rows in front of ptr[0] and behind ptr[-1]
     come out 0.  Entries of ptr that do not ascend leave the result unspecified.  Differentiable in x, weight and bias."""
-    return torch.ops.geot.segment_matmul(x, ptr, weight, bias)
+    return torch.ops.geot_dense.segment_matmul(x, ptr, weight, bias)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """Normalisation of the last dimension: ``(x - mean) / sqrt(var + eps) * weight + bias``; weight / bias [x.shape[-1]], of x's dtype or
     float32.  float32, float16 or bfloat16 rows, statistics in float32.  Differentiable in x, weight and bias."""
-    return torch.ops.geot.layer_norm(x, weight, bias, eps)
+    return torch.ops.geot_dense.layer_norm(x, weight, bias, eps)

@@ -169,10 +169,10 @@ def test_fake_shapes():
         x = torch.empty(3, 4, 8, dtype=torch.bfloat16, device="cuda")
         w = torch.empty(6, 8, dtype=torch.bfloat16, device="cuda")
         assert geot.linear(x, w, activation="gelu").shape == (3, 4, 6)
-        y, z = torch.ops.geot.linear_train(x, w, None, None, "gelu")
-        assert z.shape == y.shape and torch.ops.geot.linear_train(x, w, None, None, "relu")[1].numel() == 0
+        y, z = torch.ops.geot_dense.linear_train(x, w, None, None, "gelu")
+        assert z.shape == y.shape and torch.ops.geot_dense.linear_train(x, w, None, None, "relu")[1].numel() == 0
         assert geot.layer_norm(x, w[0].float()).shape == x.shape
-        assert torch.ops.geot.layer_norm_train(x, w[0].float(), None, 1e-5)[1].shape == (3, 12)
+        assert torch.ops.geot_dense.layer_norm_train(x, w[0].float(), None, 1e-5)[1].shape == (3, 12)
         assert geot.segment_matmul(x[0], torch.empty(3, dtype=torch.int64, device="cuda"), torch.empty(2, 8, 5, dtype=torch.bfloat16, device="cuda")).shape == (4, 5)
 
 
