@@ -37,7 +37,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4), may_alias));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4), may_alias));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2), may_alias));
 
-constexpr int kThreads = 256; // four waves, two by two over the tile
+constexpr int kThreads = 256; // of the kernels beside the tile kernels
 
 // loads and stores of 16 / 8 bytes at the element's own alignment (rows of any width, views of any offset)
 template <int SIZE> struct Packed;
@@ -97,11 +97,11 @@ __device__ inline void split8(const float (&v)[8], bf16x8 (&p)[3]) {
 }
 
 // Staging, reduction index contiguous: element (row, k) at base[row * ld + k].
-template <typename T, int R> struct StageK {
+template <typename T, int R, int NT> struct StageK {
   using E = Elem<T>;
   using L = Tile<T, R>;
-  static constexpr int N = (R * L::CK + kThreads - 1) / kThreads;
-  static constexpr bool WHOLE = (R * L::CK) % kThreads == 0;
+  static constexpr int N = (R * L::CK + NT - 1) / NT;
+  static constexpr bool WHOLE = (R * L::CK) % NT == 0;
   static constexpr int W = 8 * sizeof(T) / 16; // 16-byte pieces of a chunk
   u32x4 reg[N][W];
   const T *base;
@@ -119,7 +119,7 @@ template <typename T, int R> struct StageK {
     const bool inside = k0 + E::BK <= k_end;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = tid + i * kThreads;
+      const int idx = tid + i * NT;
       const int chunk = idx % L::CK;
       int row = idx / L::CK;
       row = row < rows ? row : rows - 1;
@@ -140,7 +140,7 @@ template <typename T, int R> struct StageK {
   __device__ void store(char *lds, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = tid + i * kThreads;
+      const int idx = tid + i * NT;
       if (!WHOLE && idx >= R * L::CK) continue;
       const int chunk = idx % L::CK, row = idx / L::CK;
       if constexpr (E::PARTS == 1) {
@@ -159,13 +159,13 @@ template <typename T, int R> struct StageK {
 };
 
 // Staging, output index contiguous: element (row, k) at base[k * ld + row].  SUM: also adds up what it stages, per row.
-template <typename T, int R, bool SUM> struct StageR {
+template <typename T, int R, int NT, bool SUM> struct StageR {
   using E = Elem<T>;
   using L = Tile<T, R>;
   static constexpr int VR = E::VR; // rows of a thread's block: 8 bytes
   static constexpr int BLOCKS = (R / VR) * L::CK;
-  static constexpr int N = (BLOCKS + kThreads - 1) / kThreads;
-  static constexpr bool WHOLE = BLOCKS % kThreads == 0;
+  static constexpr int N = (BLOCKS + NT - 1) / NT;
+  static constexpr bool WHOLE = BLOCKS % NT == 0;
   u32x2 reg[N][8];
   float sum[SUM ? N : 1][VR];
   const T *base;
@@ -189,7 +189,7 @@ template <typename T, int R, bool SUM> struct StageR {
     const bool inside = k0 + E::BK <= k_end && rows == R;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = tid + i * kThreads;
+      const int idx = tid + i * NT;
       const int row = (idx % (R / VR)) * VR, chunk = idx / (R / VR);
       const T *p = base + (k0 + chunk * 8) * ld + row;
       if (!WHOLE && idx >= BLOCKS) {
@@ -221,7 +221,7 @@ template <typename T, int R, bool SUM> struct StageR {
   __device__ void store(char *lds, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = tid + i * kThreads;
+      const int idx = tid + i * NT;
       const int row = (idx % (R / VR)) * VR, chunk = idx / (R / VR);
       if (WHOLE || idx < BLOCKS) {
 #pragma unroll
@@ -256,9 +256,10 @@ template <typename T, int R, bool SUM> struct StageR {
 };
 
 // ---- the products of one staged pair of tiles -----------------------------------------------------------------------------------
-template <typename T, int BM, int BN> struct Accum {
+// WM x WN waves over a BM x BN tile
+template <typename T, int BM, int BN, int WM, int WN> struct Accum {
   using E = Elem<T>;
-  static constexpr int FM = BM / 64, FN = BN / 64; // 32 x 32 fragments of a wave (the four waves sit two by two)
+  static constexpr int FM = BM / WM / 32, FN = BN / WN / 32; // 32 x 32 fragments of a wave
   f32x16 acc[FM][FN];
 
   __device__ void clear() {
@@ -268,6 +269,17 @@ template <typename T, int BM, int BN> struct Accum {
       for (int j = 0; j < FN; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+  }
+  __device__ void products(const typename E::Frag (&a)[E::PARTS][FM], const typename E::Frag (&b)[E::PARTS][FN]) {
+    // the smallest partial products first
+    constexpr int NP = E::PARTS == 1 ? 1 : 6;
+    constexpr int PA[6] = {E::PARTS == 1 ? 0 : 2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = E::mfma(a[PA[p]][i], b[PB[p]][j], acc[i][j]);
   }
   __device__ void step(const char *la, const char *lb, int wm, int wn, int lane) {
     using F = typename E::Frag;
@@ -280,30 +292,23 @@ template <typename T, int BM, int BN> struct Accum {
 #pragma unroll
       for (int p = 0; p < E::PARTS; ++p) {
 #pragma unroll
-        for (int i = 0; i < FM; ++i) a[p][i] = reinterpret_cast<const F *>(la)[LA::slot(p, chunk, wm * (BM / 2) + i * 32 + lane % 32)];
+        for (int i = 0; i < FM; ++i) a[p][i] = reinterpret_cast<const F *>(la)[LA::slot(p, chunk, wm * (BM / WM) + i * 32 + lane % 32)];
 #pragma unroll
-        for (int j = 0; j < FN; ++j) b[p][j] = reinterpret_cast<const F *>(lb)[LB::slot(p, chunk, wn * (BN / 2) + j * 32 + lane % 32)];
+        for (int j = 0; j < FN; ++j) b[p][j] = reinterpret_cast<const F *>(lb)[LB::slot(p, chunk, wn * (BN / WN) + j * 32 + lane % 32)];
       }
-      // the smallest partial products first
-      constexpr int NP = E::PARTS == 1 ? 1 : 6;
-      constexpr int PA[6] = {E::PARTS == 1 ? 0 : 2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-          for (int j = 0; j < FN; ++j) acc[i][j] = E::mfma(a[PA[p]][i], b[PB[p]][j], acc[i][j]);
+      products(a, b);
     }
   }
   // element e of a fragment: row 8 * (e / 4) + 4 * (lane / 32) + e % 4, column lane % 32
   static __device__ int row_of(int e, int lane) { return 8 * (e / 4) + 4 * (lane / 32) + e % 4; }
-  // fragments of row block i of every wave -> lds[64][BN + 4] floats (rows wm * 32 + ..)
+  // row block i of every wave -> lds[32 * WM][BN + 4] floats (rows wm * 32 + ..); row lr of it is row tile_row(lr, i) of the tile
   __device__ void put(float *lds, int i, int wm, int wn, int lane) const {
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) lds[(wm * 32 + row_of(e, lane)) * (BN + 4) + wn * (BN / 2) + j * 32 + lane % 32] = acc[i][j][e];
+      for (int e = 0; e < 16; ++e) lds[(wm * 32 + row_of(e, lane)) * (BN + 4) + wn * (BN / WN) + j * 32 + lane % 32] = acc[i][j][e];
   }
+  static __device__ int tile_row(int lr, int i) { return (lr / 32) * (BM / WM) + i * 32 + lr % 32; }
 };
 
 // One element in plain float32: the way of an infinity, a NaN or an overflow through a product of split operands.  A NaN ends it.
@@ -314,20 +319,70 @@ __device__ float element_again(const float *a, int64_t stride_a, const float *b,
 }
 __device__ inline bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 
-__device__ inline float activate(float z, int act) {
-  if (act == GEOT_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
-  if (act == GEOT_ACT_GELU) return 0.5f * z * erfcf(-0.70710678118654752f * z);
-  if (act == GEOT_ACT_SILU) return z / (1.0f + expf(-z));
-  return z;
-}
-__device__ inline float activation_slope(float z, int act) {
-  if (act == GEOT_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-  if (act == GEOT_ACT_GELU) return 0.5f * erfcf(-0.70710678118654752f * z) + z * 0.39894228040143268f * expf(-0.5f * z * z);
-  if (act == GEOT_ACT_SILU) {
-    const float s = 1.0f / (1.0f + expf(-z));
-    return s * (1.0f + z * (1.0f - s));
+// The normal distribution's tail, Phi(-a) = exp(-a^2 / 2) R(a) for a >= 0: R is smooth (Mills' ratio times the density's constant) and
+// is taken as a polynomial in t = 1 / (1 + 0.26 a), fitted by least squares reweighted to equal ripple on [0, 14.2] (3e-8; 4e-7 with its
+// float32 rounding).  The same exponential serves the density in the slope.  erfcf + expf instead bound the kernels by their vector
+// instructions: a gelu layer of 2.4 M x 128 -> 256 bf16 took 1527 us forward and 1064 us for its dz, 640 and 760 us of memory time.
+struct Normal {
+  float cdf, bell; // Phi(z), exp(-z^2 / 2)
+};
+template <bool EXACT> __device__ inline Normal normal_of(float z) {
+  const float a = fminf(fabsf(z), 20.0f); // (exp(-200) is 0 in float32: nothing changes behind; a NaN goes on in z)
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.26f, a, 1.0f));
+  constexpr float half_log2e = 0.72134752044448170f;
+  const float sq = a * a, arg = sq * half_log2e;
+  float bell = __builtin_amdgcn_exp2f(-arg);
+  if constexpr (EXACT) { // what the two products above rounded away (up to 24 x 2^-24 in the argument)
+    const float rest = fmaf(sq, half_log2e, -arg) + fmaf(a, a, -sq) * half_log2e;
+    bell = fmaf(bell * rest, -0.69314718055994531f, bell);
   }
-  return 1.0f;
+  float r = 0.030395518988370895f;
+  r = fmaf(r, t, -0.15229645371437073f);
+  r = fmaf(r, t, 0.25038889050483704f);
+  r = fmaf(r, t, -0.14968349039554596f);
+  r = fmaf(r, t, 0.160069078207016f);
+  r = fmaf(r, t, 0.051404859870672226f);
+  r = fmaf(r, t, 0.10293274372816086f);
+  r = fmaf(r, t, 0.10303061455488205f);
+  r = fmaf(r, t, 0.10375823080539703f);
+  const float tail = r * t * bell;
+  return {z < 0.0f ? tail : 1.0f - tail, bell};
+}
+template <bool EXACT> __device__ inline float logistic(float z) {
+  constexpr float log2e = 1.44269504088896341f;
+  const float arg = z * log2e;
+  float e = __builtin_amdgcn_exp2f(-arg);
+  if constexpr (EXACT) {
+    const float rest = fmaf(z, log2e, -arg);
+    if (fabsf(z) < 80.0f) e = fmaf(e * rest, -0.69314718055994531f, e);
+  }
+  return __builtin_amdgcn_rcpf(1.0f + e);
+}
+// ACT is a compile-time choice inside the loops over elements.  T: float operands take the exact forms.
+template <typename T, int ACT> __device__ inline float activate(float z) {
+  if constexpr (ACT == GEOT_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
+  else if constexpr (ACT == GEOT_ACT_GELU) return z * normal_of<sizeof(T) == 4>(z).cdf;
+  else if constexpr (ACT == GEOT_ACT_SILU) return z * logistic<sizeof(T) == 4>(z);
+  else return z;
+}
+template <typename T, int ACT> __device__ inline float activation_slope(float z) {
+  if constexpr (ACT == GEOT_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
+  else if constexpr (ACT == GEOT_ACT_GELU) {
+    const Normal n = normal_of<sizeof(T) == 4>(z);
+    return fmaf(z * 0.39894228040143268f, n.bell, n.cdf);
+  } else if constexpr (ACT == GEOT_ACT_SILU) {
+    const float s = logistic<sizeof(T) == 4>(z);
+    return s * fmaf(z, 1.0f - s, 1.0f);
+  } else return 1.0f;
+}
+template <int V> using Const = std::integral_constant<int, V>;
+template <typename F> __device__ __host__ inline void by_activation(int act, F f) {
+  switch (act) {
+  case GEOT_ACT_RELU: f(Const<GEOT_ACT_RELU>()); break;
+  case GEOT_ACT_GELU: f(Const<GEOT_ACT_GELU>()); break;
+  case GEOT_ACT_SILU: f(Const<GEOT_ACT_SILU>()); break;
+  default: f(Const<GEOT_ACT_NONE>());
+  }
 }
 
 // ---- groups of rows --------------------------------------------------------------------------------------------------------------
@@ -373,28 +428,119 @@ __device__ inline int64_t xcd_contiguous(int64_t block, int64_t blocks) {
   return x * q + (x < r ? x : r) + block / 8;
 }
 
+// The reduction: the next step's operands are on their way from memory while this one's are multiplied.  NBUF 2: a barrier a step.
+template <typename T, int BM, int BN, int WM, int WN, int NBUF, typename SA, typename SB>
+__device__ inline void staged_products(SA &sa, SB &sb, Accum<T, BM, BN, WM, WN> &acc, char *lds, int64_t k_len, int tid, int wm, int wn, int lane) {
+  constexpr int A_BYTES = Tile<T, BM>::BYTES, STAGE = A_BYTES + Tile<T, BN>::BYTES, BK = Elem<T>::BK;
+  if (k_len <= 0) return;
+  sa.load(0, tid);
+  sb.load(0, tid);
+  if constexpr (NBUF == 2) {
+    sa.store(lds, tid);
+    sb.store(lds + A_BYTES, tid);
+    if (BK < k_len) {
+      sa.load(BK, tid);
+      sb.load(BK, tid);
+    }
+    __syncthreads();
+    int cur = 0;
+    for (int64_t k0 = 0; k0 < k_len; k0 += BK) {
+      char *now = lds + cur * STAGE, *next = lds + (cur ^ 1) * STAGE;
+      acc.step(now, now + A_BYTES, wm, wn, lane);
+      if (k0 + BK < k_len) {
+        sa.store(next, tid);
+        sb.store(next + A_BYTES, tid);
+        if (k0 + 2 * BK < k_len) {
+          sa.load(k0 + 2 * BK, tid);
+          sb.load(k0 + 2 * BK, tid);
+        }
+      }
+      __syncthreads();
+      cur ^= 1;
+    }
+  } else {
+    for (int64_t k0 = 0; k0 < k_len; k0 += BK) {
+      sa.store(lds, tid);
+      sb.store(lds + A_BYTES, tid);
+      if (k0 + BK < k_len) {
+        sa.load(k0 + BK, tid);
+        sb.load(k0 + BK, tid);
+      }
+      __syncthreads();
+      acc.step(lds, lds + A_BYTES, wm, wn, lane);
+      __syncthreads();
+    }
+  }
+}
+
 struct RowsArgs {
   const void *a, *b, *bias, *residual;
   void *z, *y;
   int64_t lda, ldb, ldr, ldy, b_group, bias_group; // strides in elements
   Groups groups;
   int64_t n, k;
-  int64_t tiles_n;
+  int64_t slots, tiles_n;
   int act;
 };
 
+// V consecutive columns of one row: bias, z, activation, residual, y.  cols of them exist.
+template <typename T, int V, int ACT>
+__device__ inline void finish_row(const RowsArgs &g, int64_t row, int64_t col, int cols, float (&v)[V], const float (&bias)[V]) {
+  using Vec = Packed16<T>;
+  alignas(16) T tmp[V];
+#pragma unroll
+  for (int c = 0; c < V; ++c) v[c] += bias[c];
+  if (g.z) {
+    T *zp = static_cast<T *>(g.z) + row * g.n + col;
+#pragma unroll
+    for (int c = 0; c < V; ++c) tmp[c] = (T)v[c];
+    if (cols == V) *reinterpret_cast<Vec *>(zp) = *reinterpret_cast<const u32x4 *>(tmp);
+    else
+      for (int c = 0; c < V; ++c)
+        if (c < cols) zp[c] = tmp[c];
+  }
+#pragma unroll
+  for (int c = 0; c < V; ++c) v[c] = activate<T, ACT>(v[c]);
+  if (g.residual) {
+    const T *rp = static_cast<const T *>(g.residual) + row * g.ldr + col;
+    if (cols == V) *reinterpret_cast<u32x4 *>(tmp) = *reinterpret_cast<const Vec *>(rp);
+    else
+#pragma unroll
+      for (int c = 0; c < V; ++c) tmp[c] = c < cols ? rp[c] : (T)0.0f;
+#pragma unroll
+    for (int c = 0; c < V; ++c) v[c] += as_float(tmp[c]);
+  }
+  T *yp = static_cast<T *>(g.y) + row * g.ldy + col;
+#pragma unroll
+  for (int c = 0; c < V; ++c) tmp[c] = (T)v[c];
+  if (cols == V) *reinterpret_cast<Vec *>(yp) = *reinterpret_cast<const u32x4 *>(tmp);
+  else
+    for (int c = 0; c < V; ++c)
+      if (c < cols) yp[c] = tmp[c];
+}
+
+// A workgroup's tile: groups of 8 row tiles, inside a group the column tiles one after the other with the 8 row tiles fastest - what runs
+// at one time on an XCD shares both operands (8 + 8 panels for 64 tiles instead of 2 + 32 in plain order at 32 column tiles).
+constexpr int64_t kGroupRows = 8;
+__device__ inline void tile_of(int64_t id, int64_t slots, int64_t tiles_n, int64_t &slot, int64_t &tile) {
+  const int64_t per = kGroupRows * tiles_n, group = id / per, in = id % per, first = group * kGroupRows;
+  const int64_t height = slots - first < kGroupRows ? slots - first : kGroupRows;
+  slot = first + in % height;
+  tile = in / height;
+}
+
 // y rows.  BR: B's output index is contiguous (element (n, k) at b[k * ldb + n]), otherwise its reduction index (b[n * ldb + k]).
-template <typename T, int BM, int BN, bool BR, int NBUF>
-__global__ __launch_bounds__(kThreads, 2) void mm_rows_kernel(const RowsArgs g) {
+template <typename T, int BM, int BN, int WM, int WN, bool BR, int NBUF>
+__global__ __launch_bounds__(64 * WM * WN, 2) void mm_rows_kernel(const RowsArgs g) {
   using E = Elem<T>;
   using LA = Tile<T, BM>;
   using LB = Tile<T, BN>;
-  constexpr int STAGE = LA::BYTES + LB::BYTES;
-  constexpr int EPI = 64 * (BN + 4) * 4;
+  constexpr int NT = 64 * WM * WN, STAGE = LA::BYTES + LB::BYTES, EPI = 32 * WM * (BN + 4) * 4;
   __shared__ __attribute__((aligned(16))) char lds[NBUF * STAGE > EPI ? NBUF * STAGE : EPI];
-  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, wm = wave / 2, wn = wave % 2;
-  const int64_t tile = xcd_contiguous(blockIdx.x, gridDim.x);
-  const int64_t slot = tile / g.tiles_n, n0 = (tile % g.tiles_n) * BN;
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, wm = wave / WN, wn = wave % WN;
+  int64_t slot, tile;
+  tile_of(xcd_contiguous(blockIdx.x, gridDim.x), g.slots, g.tiles_n, slot, tile);
+  const int64_t n0 = tile * BN;
   const Piece piece = piece_of(g.groups, BM, slot);
   const int64_t r0 = piece.begin + piece.index * BM;
   if (r0 >= piece.end) return;
@@ -404,56 +550,16 @@ __global__ __launch_bounds__(kThreads, 2) void mm_rows_kernel(const RowsArgs g) 
   const T *A = static_cast<const T *>(g.a);
   const T *B = static_cast<const T *>(g.b) + (real ? piece.group * g.b_group : 0);
 
-  Accum<T, BM, BN> acc;
+  Accum<T, BM, BN, WM, WN> acc;
   acc.clear();
-  StageK<T, BM> sa;
-  typename std::conditional<BR, StageR<T, BN, false>, StageK<T, BN>>::type sb;
+  StageK<T, BM, NT> sa;
+  typename std::conditional<BR, StageR<T, BN, NT, false>, StageK<T, BN, NT>>::type sb;
   sa.open(A, g.lda, r0, rows, 0, k_len);
   sb.open(B, g.ldb, n0, g.n - n0, 0, k_len);
-  if (k_len > 0) {
-    sa.load(0, tid);
-    sb.load(0, tid);
-    if constexpr (NBUF == 2) {
-      sa.store(lds, tid);
-      sb.store(lds + LA::BYTES, tid);
-      if (E::BK < k_len) {
-        sa.load(E::BK, tid);
-        sb.load(E::BK, tid);
-      }
-      __syncthreads();
-      int cur = 0;
-      for (int64_t k0 = 0; k0 < k_len; k0 += E::BK) {
-        char *now = lds + cur * STAGE, *next = lds + (cur ^ 1) * STAGE;
-        acc.step(now, now + LA::BYTES, wm, wn, lane);
-        if (k0 + E::BK < k_len) {
-          sa.store(next, tid);
-          sb.store(next + LA::BYTES, tid);
-          if (k0 + 2 * E::BK < k_len) {
-            sa.load(k0 + 2 * E::BK, tid);
-            sb.load(k0 + 2 * E::BK, tid);
-          }
-        }
-        __syncthreads();
-        cur ^= 1;
-      }
-    } else {
-      for (int64_t k0 = 0; k0 < k_len; k0 += E::BK) {
-        sa.store(lds, tid);
-        sb.store(lds + LA::BYTES, tid);
-        if (k0 + E::BK < k_len) {
-          sa.load(k0 + E::BK, tid);
-          sb.load(k0 + E::BK, tid);
-        }
-        __syncthreads();
-        acc.step(lds, lds + LA::BYTES, wm, wn, lane);
-        __syncthreads();
-      }
-    }
-  }
+  staged_products<T, BM, BN, WM, WN, NBUF>(sa, sb, acc, lds, k_len, tid, wm, wn, lane);
 
-  // epilogue: 64 rows at a time through LDS, so that every access to memory is whole rows; V consecutive columns a thread
-  constexpr int V = 16 / sizeof(T), TPR = BN / V, RPP = kThreads / TPR;
-  using Vec = Packed16<T>;
+  // epilogue: 32 * WM rows at a time through LDS, so that every access to memory is whole rows; V consecutive columns a thread
+  constexpr int V = 16 / sizeof(T), TPR = BN / V, RPP = NT / TPR;
   const int col = (tid % TPR) * V;
   const int64_t nc = n0 + col;
   const int cols = nc + V <= g.n ? V : (nc < g.n ? (int)(g.n - nc) : 0);
@@ -462,64 +568,134 @@ __global__ __launch_bounds__(kThreads, 2) void mm_rows_kernel(const RowsArgs g) 
   for (int v = 0; v < V; ++v)
     bias[v] = g.bias && real && v < cols ? as_float(static_cast<const T *>(g.bias)[piece.group * g.bias_group + nc + v]) : 0.0f;
   float *out = reinterpret_cast<float *>(lds);
+  by_activation(g.act, [&](auto act) {
 #pragma unroll
-  for (int i = 0; i < BM / 64; ++i) {
-    if (i) __syncthreads();
-    acc.put(out, i, wm, wn, lane);
-    __syncthreads();
-    if (cols > 0) {
+    for (int i = 0; i < acc.FM; ++i) {
+      if (i) __syncthreads();
+      acc.put(out, i, wm, wn, lane);
+      __syncthreads();
+      if (cols > 0) {
 #pragma unroll 2
-      for (int lr = tid / TPR; lr < 64; lr += RPP) {
-        const int64_t tr = (lr / 32) * (BM / 2) + i * 32 + lr % 32;
-        if (tr >= rows) continue;
-        const int64_t row = r0 + tr;
-        float v[V];
+        for (int lr = tid / TPR; lr < 32 * WM; lr += RPP) {
+          const int64_t tr = acc.tile_row(lr, i);
+          if (tr >= rows) continue;
+          const int64_t row = r0 + tr;
+          float v[V];
 #pragma unroll
-        for (int c = 0; c < V; c += 4) {
-          const f32x4 q = *reinterpret_cast<const f32x4 *>(out + lr * (BN + 4) + col + c);
+          for (int c = 0; c < V; c += 4) {
+            const f32x4 q = *reinterpret_cast<const f32x4 *>(out + lr * (BN + 4) + col + c);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[c + e] = q[e];
-        }
-        if constexpr (E::PARTS == 3) {
-#pragma unroll
-          for (int c = 0; c < V; ++c)
-            if (!finite(v[c]) && c < cols)
-              v[c] = element_again(reinterpret_cast<const float *>(A) + row * g.lda, 1,
-                                   reinterpret_cast<const float *>(B) + (BR ? nc + c : (nc + c) * g.ldb), BR ? g.ldb : 1, k_len);
-        }
-        alignas(16) T tmp[V];
-#pragma unroll
-        for (int c = 0; c < V; ++c) v[c] += bias[c];
-        if (g.z) {
-          T *zp = static_cast<T *>(g.z) + row * g.n + nc;
-#pragma unroll
-          for (int c = 0; c < V; ++c) tmp[c] = (T)v[c];
-          if (cols == V) *reinterpret_cast<Vec *>(zp) = *reinterpret_cast<const u32x4 *>(tmp);
-          else
-            for (int c = 0; c < cols; ++c) zp[c] = tmp[c];
-        }
-        if (g.act != GEOT_ACT_NONE) {
-#pragma unroll
-          for (int c = 0; c < V; ++c) v[c] = activate(v[c], g.act);
-        }
-        if (g.residual) {
-          const T *rp = static_cast<const T *>(g.residual) + row * g.ldr + nc;
-          if (cols == V) {
-            *reinterpret_cast<u32x4 *>(tmp) = *reinterpret_cast<const Vec *>(rp);
-#pragma unroll
-            for (int c = 0; c < V; ++c) v[c] += as_float(tmp[c]);
-          } else {
-            for (int c = 0; c < cols; ++c) v[c] += as_float(rp[c]);
+            for (int e = 0; e < 4; ++e) v[c + e] = q[e];
           }
-        }
-        T *yp = static_cast<T *>(g.y) + row * g.ldy + nc;
+          if constexpr (E::PARTS == 3) {
 #pragma unroll
-        for (int c = 0; c < V; ++c) tmp[c] = (T)v[c];
-        if (cols == V) *reinterpret_cast<Vec *>(yp) = *reinterpret_cast<const u32x4 *>(tmp);
-        else
-          for (int c = 0; c < cols; ++c) yp[c] = tmp[c];
+            for (int c = 0; c < V; ++c)
+              if (!finite(v[c]) && c < cols)
+                v[c] = element_again(reinterpret_cast<const float *>(A) + row * g.lda, 1,
+                                     reinterpret_cast<const float *>(B) + (BR ? nc + c : (nc + c) * g.ldb), BR ? g.ldb : 1, k_len);
+          }
+          finish_row<T, V, decltype(act)::value>(g, row, nc, cols, v, bias);
+        }
       }
     }
+  });
+}
+
+// Few rows (or few columns): too few tiles to fill the chip, and the time of a call is that of reading one operand - for a single row of
+// a 4096 x 4096 product, 32 tiles walking 64 steps each took 56 us where the weight is read in 7.  Here a workgroup takes 32 FM rows by 32
+// columns, its eight waves take every eighth step of the reduction each, straight from memory into the operand registers of the matrix
+// instructions (lane = row, 8 consecutive values), U steps in flight, and the eight partial tiles are added through LDS.
+template <typename T, int FM> __global__ __launch_bounds__(512, 2) void mm_few_rows_kernel(const RowsArgs g) {
+  using E = Elem<T>;
+  using F = typename E::Frag;
+  constexpr int W = 8, U = 4 / FM < 1 ? 1 : 4 / FM, P16 = 8 * sizeof(T) / 16;
+  __shared__ __attribute__((aligned(16))) float part[W][32 * FM][36];
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  const int64_t tile = blockIdx.x % g.tiles_n, r0 = (int64_t)(blockIdx.x / g.tiles_n) * 32 * FM, n0 = tile * 32;
+  const T *rows[FM + 1]; // of A, then of B: rows that do not exist read the last one
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int64_t r = r0 + i * 32 + lane % 32;
+    rows[i] = static_cast<const T *>(g.a) + (r < g.groups.rows ? r : g.groups.rows - 1) * g.lda;
+  }
+  const int64_t n = n0 + lane % 32;
+  rows[FM] = static_cast<const T *>(g.b) + (n < g.n ? n : g.n - 1) * g.ldb;
+
+  Accum<T, 32 * FM, 32, 1, 1> acc;
+  acc.clear();
+  for (int64_t k0 = wave * 16 * U; k0 < g.k; k0 += W * 16 * U) {
+    u32x4 reg[U][FM + 1][P16];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = k0 + u * 16 + (lane / 32) * 8;
+#pragma unroll
+      for (int i = 0; i <= FM; ++i) {
+        if (k + 8 <= g.k) {
+#pragma unroll
+          for (int w = 0; w < P16; ++w) reg[u][i][w] = reinterpret_cast<const Packed16<T> *>(rows[i] + k)[w];
+        } else {
+          alignas(16) T tmp[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) tmp[j] = k + j < g.k ? rows[i][k + j] : (T)0.0f;
+#pragma unroll
+          for (int w = 0; w < P16; ++w) reg[u][i][w] = reinterpret_cast<const u32x4 *>(tmp)[w];
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      F a[E::PARTS][FM], b[E::PARTS][1];
+#pragma unroll
+      for (int i = 0; i <= FM; ++i) {
+        if constexpr (E::PARTS == 1) {
+          const F f = *reinterpret_cast<const F *>(&reg[u][i][0]);
+          if (i < FM) a[0][i < FM ? i : 0] = f;
+          else b[0][0] = f;
+        } else {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(reg[u][i][j / 4][j % 4]);
+          bf16x8 p[3];
+          split8(v, p);
+#pragma unroll
+          for (int s = 0; s < 3; ++s) (i < FM ? a[s][i < FM ? i : 0] : b[s][0]) = p[s];
+        }
+      }
+      acc.products(a, b);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) part[wave][i * 32 + acc.row_of(e, lane)][lane % 32] = acc.acc[i][0][e];
+  __syncthreads();
+  constexpr int V = 16 / sizeof(T), TPR = 32 / V;
+  const int col = (tid % TPR) * V;
+  const int64_t nc = n0 + col;
+  const int cols = nc + V <= g.n ? V : (nc < g.n ? (int)(g.n - nc) : 0);
+  if (cols == 0) return;
+  float bias[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) bias[v] = g.bias && v < cols ? as_float(static_cast<const T *>(g.bias)[nc + v]) : 0.0f;
+  for (int lr = tid / TPR; lr < 32 * FM && r0 + lr < g.groups.rows; lr += 512 / TPR) {
+    float v[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) v[c] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int c = 0; c < V; c += 4) {
+        const f32x4 q = *reinterpret_cast<const f32x4 *>(&part[w][lr][col + c]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[c + e] += q[e];
+      }
+    if constexpr (E::PARTS == 3) {
+#pragma unroll
+      for (int c = 0; c < V; ++c)
+        if (!finite(v[c]) && c < cols)
+          v[c] = element_again(static_cast<const float *>(g.a) + (r0 + lr) * g.lda, 1, static_cast<const float *>(g.b) + (nc + c) * g.ldb, 1, g.k);
+    }
+    by_activation(g.act, [&](auto act) { finish_row<T, V, decltype(act)::value>(g, r0 + lr, nc, cols, v, bias); });
   }
 }
 
@@ -535,15 +711,14 @@ struct WeightArgs {
   int sum_p;
 };
 
-template <typename T, int BM, int BN, int NBUF>
-__global__ __launch_bounds__(kThreads, 2) void mm_weight_kernel(const WeightArgs g) {
+template <typename T, int BM, int BN, int WM, int WN, int NBUF>
+__global__ __launch_bounds__(64 * WM * WN, 2) void mm_weight_kernel(const WeightArgs g) {
   using E = Elem<T>;
   using LA = Tile<T, BM>;
   using LB = Tile<T, BN>;
-  constexpr int STAGE = LA::BYTES + LB::BYTES;
-  constexpr int EPI = 64 * (BN + 4) * 4;
+  constexpr int NT = 64 * WM * WN, STAGE = LA::BYTES + LB::BYTES, EPI = 32 * WM * (BN + 4) * 4;
   __shared__ __attribute__((aligned(16))) char lds[NBUF * STAGE > EPI ? NBUF * STAGE : EPI];
-  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, wm = wave / 2, wn = wave % 2;
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, wm = wave / WN, wn = wave % WN;
   const int64_t tile = xcd_contiguous(blockIdx.x, gridDim.x), tiles = g.tiles_p * g.tiles_q;
   const int64_t slot = tile / tiles, t = tile % tiles, i0 = (t / g.tiles_q) * BM, j0 = (t % g.tiles_q) * BN;
   const Piece piece = piece_of(g.groups, g.unit, slot);
@@ -555,66 +730,27 @@ __global__ __launch_bounds__(kThreads, 2) void mm_weight_kernel(const WeightArgs
   const T *P = static_cast<const T *>(g.p), *Q = static_cast<const T *>(g.q);
   const bool sums = g.colsum && (g.sum_p ? j0 == 0 : i0 == 0);
 
-  Accum<T, BM, BN> acc;
+  Accum<T, BM, BN, WM, WN> acc;
   acc.clear();
-  StageR<T, BM, true> sa;
-  StageR<T, BN, true> sb;
+  StageR<T, BM, NT, true> sa;
+  StageR<T, BN, NT, true> sb;
   sa.open(P, g.ldp, i0, g.np - i0, r0, r1);
   sb.open(Q, g.ldq, j0, g.nq - j0, r0, r1);
   sa.add = sums && g.sum_p;
   sb.add = sums && !g.sum_p;
   const int64_t k_len = r1 - r0;
-  if (k_len > 0) {
-    sa.load(0, tid);
-    sb.load(0, tid);
-    if constexpr (NBUF == 2) {
-      sa.store(lds, tid);
-      sb.store(lds + LA::BYTES, tid);
-      if (E::BK < k_len) {
-        sa.load(E::BK, tid);
-        sb.load(E::BK, tid);
-      }
-      __syncthreads();
-      int cur = 0;
-      for (int64_t k0 = 0; k0 < k_len; k0 += E::BK) {
-        char *now = lds + cur * STAGE, *next = lds + (cur ^ 1) * STAGE;
-        acc.step(now, now + LA::BYTES, wm, wn, lane);
-        if (k0 + E::BK < k_len) {
-          sa.store(next, tid);
-          sb.store(next + LA::BYTES, tid);
-          if (k0 + 2 * E::BK < k_len) {
-            sa.load(k0 + 2 * E::BK, tid);
-            sb.load(k0 + 2 * E::BK, tid);
-          }
-        }
-        __syncthreads();
-        cur ^= 1;
-      }
-    } else {
-      for (int64_t k0 = 0; k0 < k_len; k0 += E::BK) {
-        sa.store(lds, tid);
-        sb.store(lds + LA::BYTES, tid);
-        if (k0 + E::BK < k_len) {
-          sa.load(k0 + E::BK, tid);
-          sb.load(k0 + E::BK, tid);
-        }
-        __syncthreads();
-        acc.step(lds, lds + LA::BYTES, wm, wn, lane);
-        __syncthreads();
-      }
-    }
-  }
+  staged_products<T, BM, BN, WM, WN, NBUF>(sa, sb, acc, lds, k_len, tid, wm, wn, lane);
 
   const int64_t per_slot = g.np * g.nq + (g.colsum ? g.ns : 0);
   float *out = reinterpret_cast<float *>(lds);
   const int col = (tid % (BN / 4)) * 4;
 #pragma unroll
-  for (int i = 0; i < BM / 64; ++i) {
+  for (int i = 0; i < acc.FM; ++i) {
     if (i) __syncthreads();
     acc.put(out, i, wm, wn, lane);
     __syncthreads();
-    for (int lr = tid / (BN / 4); lr < 64; lr += kThreads / (BN / 4)) {
-      const int64_t row = i0 + (lr / 32) * (BM / 2) + i * 32 + lr % 32;
+    for (int lr = tid / (BN / 4); lr < 32 * WM; lr += NT / (BN / 4)) {
+      const int64_t row = i0 + acc.tile_row(lr, i);
       if (row >= g.np) continue;
       const f32x4 q = *reinterpret_cast<const f32x4 *>(out + lr * (BN + 4) + col);
 #pragma unroll
@@ -639,7 +775,7 @@ __global__ __launch_bounds__(kThreads, 2) void mm_weight_kernel(const WeightArgs
       using S = typename std::remove_reference<decltype(st)>::type;
 #pragma unroll
       for (int i = 0; i < S::N; ++i) {
-        const int idx = tid + i * kThreads;
+        const int idx = tid + i * NT;
         if (idx < S::BLOCKS) {
           const int row = (idx % (R / S::VR)) * S::VR, chunk = idx / (R / S::VR);
 #pragma unroll
@@ -647,7 +783,7 @@ __global__ __launch_bounds__(kThreads, 2) void mm_weight_kernel(const WeightArgs
         }
       }
       __syncthreads();
-      for (int c = tid; c < R && first + c < n; c += kThreads) {
+      for (int c = tid; c < R && first + c < n; c += NT) {
         float s = 0.0f;
         for (int k = 0; k < E::BK / 8; ++k) s += out[k * R + c];
         if (whole) static_cast<T *>(g.colsum)[piece.group * g.ns + first + c] = (T)s;
@@ -697,7 +833,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void mm_join_kernel
 }
 
 // ---- the activation's gradient: dz = dy * act'(z) -----------------------------------------------------------------------------------
-template <typename T> __global__ __launch_bounds__(kThreads) void act_backward_kernel(const T *dy, const T *z, T *dz, int64_t n, int act) {
+template <typename T, int ACT> __global__ __launch_bounds__(kThreads) void act_backward_kernel(const T *dy, const T *z, T *dz, int64_t n) {
   constexpr int V = 16 / sizeof(T);
   using Vec = Packed16<T>;
   const int64_t step = (int64_t)gridDim.x * kThreads * V;
@@ -707,10 +843,10 @@ template <typename T> __global__ __launch_bounds__(kThreads) void act_backward_k
       *reinterpret_cast<u32x4 *>(a) = *reinterpret_cast<const Vec *>(dy + i);
       *reinterpret_cast<u32x4 *>(b) = *reinterpret_cast<const Vec *>(z + i);
 #pragma unroll
-      for (int v = 0; v < V; ++v) a[v] = (T)(as_float(a[v]) * activation_slope(as_float(b[v]), act));
+      for (int v = 0; v < V; ++v) a[v] = (T)(as_float(a[v]) * activation_slope<T, ACT>(as_float(b[v])));
       *reinterpret_cast<Vec *>(dz + i) = *reinterpret_cast<const u32x4 *>(a);
     } else {
-      for (int64_t j = i; j < n; ++j) dz[j] = (T)(as_float(dy[j]) * activation_slope(as_float(z[j]), act));
+      for (int64_t j = i; j < n; ++j) dz[j] = (T)(as_float(dy[j]) * activation_slope<T, ACT>(as_float(z[j])));
     }
   }
 }
@@ -725,16 +861,30 @@ int launched(const char *name) {
 
 constexpr int64_t kMaxBlocks = ((int64_t)1 << 31) - 1;
 
-template <typename T, int BM, int BN, bool BR> int run_rows(RowsArgs &g, hipStream_t st) {
+template <typename T, int BM, int BN, int WM, int WN, bool BR> int run_rows(RowsArgs &g, hipStream_t st) {
   constexpr int NBUF = Elem<T>::PARTS == 1 ? 2 : 1;
   g.tiles_n = (g.n + BN - 1) / BN;
-  const int64_t slots = slots_of(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, BM);
-  if (slots > kMaxBlocks / g.tiles_n) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
-  hipLaunchKernelGGL((mm_rows_kernel<T, BM, BN, BR, NBUF>), dim3((unsigned)(slots * g.tiles_n)), dim3(kThreads), 0, st, g);
+  g.slots = slots_of(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, BM);
+  if (g.slots > kMaxBlocks / g.tiles_n) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
+  hipLaunchKernelGGL((mm_rows_kernel<T, BM, BN, WM, WN, BR, NBUF>), dim3((unsigned)(g.slots * g.tiles_n)), dim3(64 * WM * WN), 0, st, g);
   return launched("mm_rows_kernel");
 }
+template <typename T, int FM> int run_few(RowsArgs &g, hipStream_t st) {
+  g.tiles_n = (g.n + 31) / 32;
+  const int64_t tiles_m = (g.groups.rows + 32 * FM - 1) / (32 * FM);
+  hipLaunchKernelGGL((mm_few_rows_kernel<T, FM>), dim3((unsigned)(tiles_m * g.tiles_n)), dim3(512), 0, st, g);
+  return launched("mm_few_rows_kernel");
+}
 template <typename T, bool BR> int rows_typed(RowsArgs &g, hipStream_t st) {
-  return g.n <= 64 ? run_rows<T, 128, 64, BR>(g, st) : run_rows<T, 128, 128, BR>(g, st);
+  const int64_t tiles = ((g.groups.rows + 127) / 128) * ((g.n + 127) / 128);
+  if constexpr (!BR) {
+    if (!g.groups.ptr && tiles < 128 && g.k >= 128) return g.groups.rows <= 32 ? run_few<T, 1>(g, st) : run_few<T, 2>(g, st);
+  }
+  if (g.n <= 64) return run_rows<T, 128, 64, 2, 2, BR>(g, st);
+  if constexpr (Elem<T>::PARTS == 1) {
+    if (g.n > 128 && g.k >= 512 && tiles >= 1024) return run_rows<T, 256, 256, 2, 4, BR>(g, st);
+  }
+  return run_rows<T, 128, 128, 2, 2, BR>(g, st);
 }
 int rows_product(RowsArgs &g, bool br, int dtype, hipStream_t st) {
   if (g.groups.rows == 0 || g.n == 0) return GEOT_OK;
@@ -764,11 +914,11 @@ WeightPlan weight_plan(int64_t rows, int64_t groups, bool with_ptr, int64_t np, 
   if (w.slots < 1) w.slots = 1;
   return w;
 }
-template <typename T, int BM, int BN> int run_weight(WeightArgs &g, int64_t slots, hipStream_t st) {
+template <typename T, int BM, int BN, int WM, int WN> int run_weight(WeightArgs &g, int64_t slots, hipStream_t st) {
   constexpr int NBUF = Elem<T>::PARTS == 1 ? 2 : 1;
   const int64_t tiles = g.tiles_p * g.tiles_q;
   if (slots > kMaxBlocks / tiles) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
-  hipLaunchKernelGGL((mm_weight_kernel<T, BM, BN, NBUF>), dim3((unsigned)(slots * tiles)), dim3(kThreads), 0, st, g);
+  hipLaunchKernelGGL((mm_weight_kernel<T, BM, BN, WM, WN, NBUF>), dim3((unsigned)(slots * tiles)), dim3(64 * WM * WN), 0, st, g);
   if (const int rc = launched("mm_weight_kernel")) return rc;
   if (g.groups.rows > g.unit) { // some group may have several chunks
     const int64_t per = (g.np * g.nq + (g.colsum ? g.ns : 0) + 15) / 16;
@@ -778,8 +928,8 @@ template <typename T, int BM, int BN> int run_weight(WeightArgs &g, int64_t slot
   return GEOT_OK;
 }
 template <typename T> int weight_typed(WeightArgs &g, int64_t slots, hipStream_t st) {
-  if (g.np <= 64) return g.nq <= 64 ? run_weight<T, 64, 64>(g, slots, st) : run_weight<T, 64, 128>(g, slots, st);
-  return g.nq <= 64 ? run_weight<T, 128, 64>(g, slots, st) : run_weight<T, 128, 128>(g, slots, st);
+  if (g.np <= 64) return g.nq <= 64 ? run_weight<T, 64, 64, 2, 2>(g, slots, st) : run_weight<T, 64, 128, 2, 2>(g, slots, st);
+  return g.nq <= 64 ? run_weight<T, 128, 64, 2, 2>(g, slots, st) : run_weight<T, 128, 128, 2, 2>(g, slots, st);
 }
 int weight_product(WeightArgs &g, int dtype, void *workspace, size_t workspace_bytes, hipStream_t st) {
   if (g.groups.groups == 0 || (g.np * g.nq == 0 && !(g.colsum && g.ns > 0))) return GEOT_OK;
@@ -852,12 +1002,17 @@ int geot_activation_backward(const void *dy, const void *z, void *dz, int64_t n,
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t vec = dtype == GEOT_F32 ? 4 : 8, want = (n + vec * kThreads - 1) / (vec * kThreads);
   const unsigned blocks = (unsigned)(want < 8192 ? want : 8192);
-  switch (dtype) {
-  case GEOT_F32: hipLaunchKernelGGL(act_backward_kernel<float>, dim3(blocks), dim3(kThreads), 0, st, (const float *)dy, (const float *)z, (float *)dz, n, activation); break;
-  case GEOT_F16: hipLaunchKernelGGL(act_backward_kernel<f16>, dim3(blocks), dim3(kThreads), 0, st, (const f16 *)dy, (const f16 *)z, (f16 *)dz, n, activation); break;
-  case GEOT_BF16: hipLaunchKernelGGL(act_backward_kernel<bf16>, dim3(blocks), dim3(kThreads), 0, st, (const bf16 *)dy, (const bf16 *)z, (bf16 *)dz, n, activation); break;
-  default: return geot_internal_fail(GEOT_EUNSUPPORTED, "geot_activation_backward: float32, float16 and bfloat16");
-  }
+  auto run = [&](auto *t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    by_activation(activation, [&](auto act) {
+      hipLaunchKernelGGL((act_backward_kernel<T, decltype(act)::value>), dim3(blocks), dim3(kThreads), 0, st, static_cast<const T *>(dy), static_cast<const T *>(z),
+                         static_cast<T *>(dz), n);
+    });
+  };
+  if (dtype == GEOT_F32) run((float *)nullptr);
+  else if (dtype == GEOT_F16) run((f16 *)nullptr);
+  else if (dtype == GEOT_BF16) run((bf16 *)nullptr);
+  else return geot_internal_fail(GEOT_EUNSUPPORTED, "geot_activation_backward: float32, float16 and bfloat16");
   return launched("act_backward_kernel");
 }
 
