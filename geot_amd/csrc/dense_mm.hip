@@ -199,13 +199,20 @@ template <typename T, int R, int NT, bool SUM> struct StageR {
 #pragma unroll
         for (int j = 0; j < 8; ++j) reg[i][j] = *reinterpret_cast<const Packed8<T> *>(p + j * ld);
       } else {
+        const bool wide = row + VR <= rows;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          alignas(8) T tmp[VR];
-          const bool in_k = k0 + chunk * 8 + j < k_end;
+          const int64_t k = k0 + chunk * 8 + j;
+          u32x2 v = {0, 0};
+          if (k < k_end && wide) {
+            v = *reinterpret_cast<const Packed8<T> *>(p + j * ld);
+          } else if (k < k_end && row < rows) {
+            alignas(8) T tmp[VR];
 #pragma unroll
-          for (int r = 0; r < VR; ++r) tmp[r] = in_k && row + r < rows ? p[j * ld + r] : (T)0.0f;
-          reg[i][j] = *reinterpret_cast<const u32x2 *>(tmp);
+            for (int r = 0; r < VR; ++r) tmp[r] = row + r < rows ? p[j * ld + r] : (T)0.0f;
+            v = *reinterpret_cast<const u32x2 *>(tmp);
+          }
+          reg[i][j] = v;
         }
       }
     }
@@ -324,10 +331,11 @@ __device__ inline bool finite(float v) { return (__float_as_uint(v) & 0x7f800000
 // float32 rounding).  The same exponential serves the density in the slope.  erfcf + expf instead bound the kernels by their vector
 // instructions: a gelu layer of 2.4 M x 128 -> 256 bf16 took 1527 us forward and 1064 us for its dz, 640 and 760 us of memory time.
 struct Normal {
-  float cdf, bell; // Phi(z), exp(-z^2 / 2)
+  float tail, bell; // Phi(-|z|), exp(-z^2 / 2)
 };
 template <bool EXACT> __device__ inline Normal normal_of(float z) {
-  const float a = fminf(fabsf(z), 20.0f); // (exp(-200) is 0 in float32: nothing changes behind; a NaN goes on in z)
+  // (EXACT: exp(-200) is 0 in float32, nothing changes behind 20 but inf - inf below; a NaN goes on in z)
+  const float a = EXACT ? fminf(fabsf(z), 20.0f) : fabsf(z);
   const float t = __builtin_amdgcn_rcpf(fmaf(0.26f, a, 1.0f));
   constexpr float half_log2e = 0.72134752044448170f;
   const float sq = a * a, arg = sq * half_log2e;
@@ -345,8 +353,7 @@ template <bool EXACT> __device__ inline Normal normal_of(float z) {
   r = fmaf(r, t, 0.10293274372816086f);
   r = fmaf(r, t, 0.10303061455488205f);
   r = fmaf(r, t, 0.10375823080539703f);
-  const float tail = r * t * bell;
-  return {z < 0.0f ? tail : 1.0f - tail, bell};
+  return {r * t * bell, bell};
 }
 template <bool EXACT> __device__ inline float logistic(float z) {
   constexpr float log2e = 1.44269504088896341f;
@@ -361,7 +368,10 @@ template <bool EXACT> __device__ inline float logistic(float z) {
 // ACT is a compile-time choice inside the loops over elements.  T: float operands take the exact forms.
 template <typename T, int ACT> __device__ inline float activate(float z) {
   if constexpr (ACT == GEOT_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
-  else if constexpr (ACT == GEOT_ACT_GELU) return z * normal_of<sizeof(T) == 4>(z).cdf;
+  else if constexpr (ACT == GEOT_ACT_GELU) { // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+    const float y = fmaf(-fabsf(z), normal_of<sizeof(T) == 4>(z).tail, fmaxf(z, 0.0f));
+    return sizeof(T) == 4 && z != z ? z : y; // (16 bits: the tail of a NaN is one)
+  }
   else if constexpr (ACT == GEOT_ACT_SILU) return z * logistic<sizeof(T) == 4>(z);
   else return z;
 }
@@ -369,7 +379,7 @@ template <typename T, int ACT> __device__ inline float activation_slope(float z)
   if constexpr (ACT == GEOT_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
   else if constexpr (ACT == GEOT_ACT_GELU) {
     const Normal n = normal_of<sizeof(T) == 4>(z);
-    return fmaf(z * 0.39894228040143268f, n.bell, n.cdf);
+    return fmaf(z * 0.39894228040143268f, n.bell, z < 0.0f ? n.tail : 1.0f - n.tail);
   } else if constexpr (ACT == GEOT_ACT_SILU) {
     const float s = logistic<sizeof(T) == 4>(z);
     return s * fmaf(z, 1.0f - s, 1.0f);
@@ -388,7 +398,7 @@ template <typename F> __device__ __host__ inline void by_activation(int act, F f
 // ---- groups of rows --------------------------------------------------------------------------------------------------------------
 // Rows are cut at the boundaries q_0 = 0, q_1 = ptr[0], ..., q_{G+1} = ptr[G], q_{G+2} = rows (each clamped into [0, rows]): G groups,
 // and the rows in front of and behind them, whose results are zero.  Piece j starts at slot floor(q_j / unit) + j of the launch: that
-// leaves it at least ceil(len / unit) slots and makes the slot of a workgroup a binary search in ptr - no scan, no table, no second
+// leaves it at least ceil(len / unit) slots and makes the slot of a workgroup a search in ptr - no scan, no table, no second
 // launch; at most G + 2 slots stay empty.  Without a pointer array there is one group, all rows.
 struct Groups {
   const int64_t *ptr;
@@ -406,15 +416,23 @@ struct Piece {
   int64_t index;      // which unit of the piece this slot is (may lie behind its end)
   int64_t start;      // the piece's first slot
 };
+// The last piece whose first slot is <= slot, found 64 candidates a step (one a lane): a binary search's chain of dependent loads was
+// several microseconds of every workgroup.  Every lane of the wave takes part.
 __device__ inline Piece piece_of(const Groups &g, int64_t unit, int64_t slot) {
   if (!g.ptr) return {0, 0, g.rows, slot, 0};
-  int64_t lo = 0, hi = g.groups + 1; // the last piece whose first slot is <= slot
-  while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) / 2;
-    if (g.bound(mid) / unit + mid <= slot) lo = mid;
-    else hi = mid - 1;
+  const int lane = threadIdx.x % 64;
+  int64_t lo = 0, len = g.groups + 2;
+  while (len > 1) {
+    const int64_t step = (len + 63) / 64, at = lane * step;
+    const bool ok = at < len && g.bound(lo + at) / unit + lo + at <= slot;
+    int count = __popcll(__ballot(ok));
+    count = count > 0 ? count : 1;
+    lo += (count - 1) * step;
+    len -= (count - 1) * step;
+    len = len < step ? len : step;
   }
   const int64_t q0 = g.bound(lo), q1 = g.bound(lo + 1), start = q0 / unit + lo;
+  if (slot < start) return {-1, 0, 0, 0, 0}; // (only where ptr does not ascend: no rows)
   return {lo >= 1 && lo <= g.groups ? lo - 1 : -1, q0, q1, slot - start, start};
 }
 int64_t slots_of(int64_t rows, int64_t groups, bool with_ptr, int64_t unit) {
@@ -479,7 +497,7 @@ struct RowsArgs {
   int64_t lda, ldb, ldr, ldy, b_group, bias_group; // strides in elements
   Groups groups;
   int64_t n, k;
-  int64_t slots, tiles_n;
+  int64_t slots, tiles_n, band; // band: row tiles of a group of tiles (tile_of)
   int act;
 };
 
@@ -521,10 +539,11 @@ __device__ inline void finish_row(const RowsArgs &g, int64_t row, int64_t col, i
 
 // A workgroup's tile: groups of 8 row tiles, inside a group the column tiles one after the other with the 8 row tiles fastest - what runs
 // at one time on an XCD shares both operands (8 + 8 panels for 64 tiles instead of 2 + 32 in plain order at 32 column tiles).
-constexpr int64_t kGroupRows = 8;
-__device__ inline void tile_of(int64_t id, int64_t slots, int64_t tiles_n, int64_t &slot, int64_t &tile) {
-  const int64_t per = kGroupRows * tiles_n, group = id / per, in = id % per, first = group * kGroupRows;
-  const int64_t height = slots - first < kGroupRows ? slots - first : kGroupRows;
+// Groups of rows (ptr) keep the plain order: row tiles side by side rarely share a matrix (64 groups of 512 rows, 1024 -> 2048 f16: 280 us
+// in plain order, 342 in bands of 8; without groups, 8192 x 4096 x 4096: 372 and 306).
+__device__ inline void tile_of(int64_t id, int64_t slots, int64_t tiles_n, int64_t band, int64_t &slot, int64_t &tile) {
+  const int64_t per = band * tiles_n, group = id / per, in = id % per, first = group * band;
+  const int64_t height = slots - first < band ? slots - first : band;
   slot = first + in % height;
   tile = in / height;
 }
@@ -539,7 +558,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mm_rows_kernel(const RowsArgs
   __shared__ __attribute__((aligned(16))) char lds[NBUF * STAGE > EPI ? NBUF * STAGE : EPI];
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, wm = wave / WN, wn = wave % WN;
   int64_t slot, tile;
-  tile_of(xcd_contiguous(blockIdx.x, gridDim.x), g.slots, g.tiles_n, slot, tile);
+  tile_of(xcd_contiguous(blockIdx.x, gridDim.x), g.slots, g.tiles_n, g.band, slot, tile);
   const int64_t n0 = tile * BN;
   const Piece piece = piece_of(g.groups, BM, slot);
   const int64_t r0 = piece.begin + piece.index * BM;
@@ -753,18 +772,41 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mm_weight_kernel(const Weight
       const int64_t row = i0 + acc.tile_row(lr, i);
       if (row >= g.np) continue;
       const f32x4 q = *reinterpret_cast<const f32x4 *>(out + lr * (BN + 4) + col);
+      const int64_t cc = j0 + col;
+      if (cc >= g.nq) continue;
+      const int cols = g.nq - cc < 4 ? (int)(g.nq - cc) : 4;
+      alignas(16) float v[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int64_t cc = j0 + col + c;
-        if (cc >= g.nq) break;
-        float v = q[c];
+        v[c] = q[c];
         if constexpr (E::PARTS == 3) {
-          if (!finite(v))
-            v = element_again(reinterpret_cast<const float *>(P) + r0 * g.ldp + row, g.ldp, reinterpret_cast<const float *>(Q) + r0 * g.ldq + cc, g.ldq,
-                              k_len);
+          if (!finite(v[c]) && c < cols)
+            v[c] = element_again(reinterpret_cast<const float *>(P) + r0 * g.ldp + row, g.ldp, reinterpret_cast<const float *>(Q) + r0 * g.ldq + cc + c, g.ldq,
+                                 k_len);
         }
-        if (whole) static_cast<T *>(g.out)[(piece.group * g.np + row) * g.nq + cc] = (T)v;
-        else g.part[slot * per_slot + row * g.nq + cc] = v;
+      }
+      if (whole) {
+        T *o = static_cast<T *>(g.out) + (piece.group * g.np + row) * g.nq + cc;
+        alignas(16) T tmp[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmp[c] = (T)v[c];
+        if (cols == 4) {
+          if constexpr (sizeof(T) == 4) *reinterpret_cast<Packed16<T> *>(o) = *reinterpret_cast<const u32x4 *>(tmp);
+          else *reinterpret_cast<Packed8<T> *>(o) = *reinterpret_cast<const u32x2 *>(tmp);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (c < cols) o[c] = tmp[c];
+        }
+      } else {
+        float *o = g.part + slot * per_slot + row * g.nq + cc;
+        if (cols == 4) {
+          *reinterpret_cast<Packed16<float> *>(o) = *reinterpret_cast<const u32x4 *>(v);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (c < cols) o[c] = v[c];
+        }
       }
     }
   }
@@ -861,11 +903,11 @@ int launched(const char *name) {
 
 constexpr int64_t kMaxBlocks = ((int64_t)1 << 31) - 1;
 
-template <typename T, int BM, int BN, int WM, int WN, bool BR> int run_rows(RowsArgs &g, hipStream_t st) {
-  constexpr int NBUF = Elem<T>::PARTS == 1 ? 2 : 1;
+template <typename T, int BM, int BN, int WM, int WN, bool BR, int NBUF> int run_rows(RowsArgs &g, hipStream_t st) {
   g.tiles_n = (g.n + BN - 1) / BN;
   g.slots = slots_of(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, BM);
   if (g.slots > kMaxBlocks / g.tiles_n) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
+  g.band = g.groups.ptr ? 1 : 8;
   hipLaunchKernelGGL((mm_rows_kernel<T, BM, BN, WM, WN, BR, NBUF>), dim3((unsigned)(g.slots * g.tiles_n)), dim3(64 * WM * WN), 0, st, g);
   return launched("mm_rows_kernel");
 }
@@ -880,11 +922,14 @@ template <typename T, bool BR> int rows_typed(RowsArgs &g, hipStream_t st) {
   if constexpr (!BR) {
     if (!g.groups.ptr && tiles < 128 && g.k >= 128) return g.groups.rows <= 32 ? run_few<T, 1>(g, st) : run_few<T, 2>(g, st);
   }
-  if (g.n <= 64) return run_rows<T, 128, 64, 2, 2, BR>(g, st);
+  constexpr int LONG = Elem<T>::PARTS == 1 ? 2 : 1;
+  const bool shallow = g.k <= 4 * Elem<T>::BK;
+  if (g.n <= 64) return shallow ? run_rows<T, 128, 64, 2, 2, BR, 1>(g, st) : run_rows<T, 128, 64, 2, 2, BR, LONG>(g, st);
   if constexpr (Elem<T>::PARTS == 1) {
-    if (g.n > 128 && g.k >= 512 && tiles >= 1024) return run_rows<T, 256, 256, 2, 4, BR>(g, st);
+    const int64_t per_group = g.groups.ptr ? g.groups.rows / (g.groups.groups > 0 ? g.groups.groups : 1) : g.groups.rows;
+    if (g.n > 128 && g.k >= 512 && tiles >= 1024 && per_group >= 2048) return run_rows<T, 256, 256, 2, 4, BR, 2>(g, st);
   }
-  return run_rows<T, 128, 128, 2, 2, BR>(g, st);
+  return shallow ? run_rows<T, 128, 128, 2, 2, BR, 1>(g, st) : run_rows<T, 128, 128, 2, 2, BR, LONG>(g, st);
 }
 int rows_product(RowsArgs &g, bool br, int dtype, hipStream_t st) {
   if (g.groups.rows == 0 || g.n == 0) return GEOT_OK;
@@ -922,7 +967,11 @@ template <typename T, int BM, int BN, int WM, int WN> int run_weight(WeightArgs 
   if (const int rc = launched("mm_weight_kernel")) return rc;
   if (g.groups.rows > g.unit) { // some group may have several chunks
     const int64_t per = (g.np * g.nq + (g.colsum ? g.ns : 0) + 15) / 16;
-    hipLaunchKernelGGL((mm_join_kernel<T>), dim3((unsigned)(per < 2048 ? per : 2048), (unsigned)g.groups.groups), dim3(kThreads), 0, st, g);
+    // (which groups have several chunks only the device knows: few workgroups a group when there are many - 2048 each cost 50 us at 64
+    // groups of one chunk)
+    int64_t wide = 8192 / g.groups.groups;
+    wide = wide < 32 ? 32 : wide > 2048 ? 2048 : wide;
+    hipLaunchKernelGGL((mm_join_kernel<T>), dim3((unsigned)(per < wide ? per : wide), (unsigned)g.groups.groups), dim3(kThreads), 0, st, g);
     return launched(nullptr);
   }
   return GEOT_OK;
