@@ -115,17 +115,24 @@ template <typename T, int R, int NT> struct StageK {
     base = b + first * ld_ + k_begin;
     k_end = k_end_ - k_begin;
   }
-  __device__ void load(int64_t k0, int tid) {
-    const bool inside = k0 + E::BK <= k_end;
+  __device__ bool fast() const { return true; }
+  // a whole step (k0 + BK <= k_end)
+  __device__ void load_fast(int64_t k0, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = tid + i * NT;
-      const int chunk = idx % L::CK;
-      int row = idx / L::CK;
-      row = row < rows ? row : rows - 1;
-      const int64_t k = k0 + chunk * 8;
-      const T *p = base + row * ld + k;
-      if (inside || k + 8 <= k_end) {
+      const int idx = tid + i * NT, row = idx / L::CK;
+      const T *p = base + (row < rows ? row : rows - 1) * ld + k0 + idx % L::CK * 8;
+#pragma unroll
+      for (int w = 0; w < W; ++w) reg[i][w] = reinterpret_cast<const Packed16<T> *>(p)[w];
+    }
+  }
+  __device__ void load_any(int64_t k0, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = tid + i * NT, row = idx / L::CK;
+      const int64_t k = k0 + idx % L::CK * 8;
+      const T *p = base + (row < rows ? row : rows - 1) * ld + k;
+      if (k + 8 <= k_end) {
 #pragma unroll
         for (int w = 0; w < W; ++w) reg[i][w] = reinterpret_cast<const Packed16<T> *>(p)[w];
       } else {
@@ -185,35 +192,37 @@ template <typename T, int R, int NT, bool SUM> struct StageR {
         for (int j = 0; j < VR; ++j) sum[i][j] = 0.0f;
     }
   }
-  __device__ void load(int64_t k0, int tid) {
-    const bool inside = k0 + E::BK <= k_end && rows == R;
+  // columns behind the last one are never stored: a block that lies behind reads the last whole one instead, which needs the width
+  // (of an edge tile) to be whole blocks
+  __device__ bool fast() const { return rows == R || (rows % VR == 0 && rows > 0); }
+  __device__ void load_fast(int64_t k0, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = tid + i * NT;
-      const int row = (idx % (R / VR)) * VR, chunk = idx / (R / VR);
+      const int idx = tid + i * NT, row = (idx % (R / VR)) * VR, chunk = WHOLE || idx < BLOCKS ? idx / (R / VR) : 0;
+      const T *p = base + (k0 + chunk * 8) * ld + (row + VR <= rows ? row : rows - VR);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) reg[i][j] = *reinterpret_cast<const Packed8<T> *>(p + j * ld);
+    }
+  }
+  __device__ void load_any(int64_t k0, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = tid + i * NT, row = (idx % (R / VR)) * VR, chunk = WHOLE || idx < BLOCKS ? idx / (R / VR) : 0;
       const T *p = base + (k0 + chunk * 8) * ld + row;
-      if (!WHOLE && idx >= BLOCKS) {
+      const bool wide = row + VR <= rows;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) reg[i][j] = u32x2{0, 0};
-      } else if (inside) {
+      for (int j = 0; j < 8; ++j) {
+        const int64_t k = k0 + chunk * 8 + j;
+        u32x2 v = {0, 0};
+        if (k < k_end && wide) {
+          v = *reinterpret_cast<const Packed8<T> *>(p + j * ld);
+        } else if (k < k_end && row < rows) {
+          alignas(8) T tmp[VR];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) reg[i][j] = *reinterpret_cast<const Packed8<T> *>(p + j * ld);
-      } else {
-        const bool wide = row + VR <= rows;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int64_t k = k0 + chunk * 8 + j;
-          u32x2 v = {0, 0};
-          if (k < k_end && wide) {
-            v = *reinterpret_cast<const Packed8<T> *>(p + j * ld);
-          } else if (k < k_end && row < rows) {
-            alignas(8) T tmp[VR];
-#pragma unroll
-            for (int r = 0; r < VR; ++r) tmp[r] = row + r < rows ? p[j * ld + r] : (T)0.0f;
-            v = *reinterpret_cast<const u32x2 *>(tmp);
-          }
-          reg[i][j] = v;
+          for (int r = 0; r < VR; ++r) tmp[r] = row + r < rows ? p[j * ld + r] : (T)0.0f;
+          v = *reinterpret_cast<const u32x2 *>(tmp);
         }
+        reg[i][j] = v;
       }
     }
   }
@@ -397,7 +406,7 @@ template <typename F> __device__ __host__ inline void by_activation(int act, F f
 
 // ---- groups of rows --------------------------------------------------------------------------------------------------------------
 // Rows are cut at the boundaries q_0 = 0, q_1 = ptr[0], ..., q_{G+1} = ptr[G], q_{G+2} = rows (each clamped into [0, rows]): G groups,
-// and the rows in front of and behind them, whose results are zero.  Piece j starts at slot floor(q_j / unit) + j of the launch: that
+// and the rows in front of and behind them, whose results are zero.  Piece j starts at slot floor(q_j / unit) + j of the launch (unit a power of two): that
 // leaves it at least ceil(len / unit) slots and makes the slot of a workgroup a search in ptr - no scan, no table, no second
 // launch; at most G + 2 slots stay empty.  Without a pointer array there is one group, all rows.
 struct Groups {
@@ -416,22 +425,26 @@ struct Piece {
   int64_t index;      // which unit of the piece this slot is (may lie behind its end)
   int64_t start;      // the piece's first slot
 };
+// one value of the wave in scalar registers (the compiler cannot see that what depends on it is uniform)
+__device__ inline int64_t uniform(int64_t v) {
+  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)((uint64_t)v >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
 // The last piece whose first slot is <= slot, found 64 candidates a step (one a lane): a binary search's chain of dependent loads was
 // several microseconds of every workgroup.  Every lane of the wave takes part.
-__device__ inline Piece piece_of(const Groups &g, int64_t unit, int64_t slot) {
+__device__ inline Piece piece_of(const Groups &g, int unit_log2, int64_t slot) {
   if (!g.ptr) return {0, 0, g.rows, slot, 0};
   const int lane = threadIdx.x % 64;
   int64_t lo = 0, len = g.groups + 2;
   while (len > 1) {
-    const int64_t step = (len + 63) / 64, at = lane * step;
-    const bool ok = at < len && g.bound(lo + at) / unit + lo + at <= slot;
+    const int64_t step = (len + 63) >> 6, at = lane * step;
+    const bool ok = at < len && (g.bound(lo + at) >> unit_log2) + lo + at <= slot;
     int count = __popcll(__ballot(ok));
     count = count > 0 ? count : 1;
-    lo += (count - 1) * step;
-    len -= (count - 1) * step;
+    lo = uniform(lo + (count - 1) * step);
+    len = uniform(len - (count - 1) * step);
     len = len < step ? len : step;
   }
-  const int64_t q0 = g.bound(lo), q1 = g.bound(lo + 1), start = q0 / unit + lo;
+  const int64_t q0 = uniform(g.bound(lo)), q1 = uniform(g.bound(lo + 1)), start = (q0 >> unit_log2) + lo;
   if (slot < start) return {-1, 0, 0, 0, 0}; // (only where ptr does not ascend: no rows)
   return {lo >= 1 && lo <= g.groups ? lo - 1 : -1, q0, q1, slot - start, start};
 }
@@ -441,48 +454,82 @@ int64_t slots_of(int64_t rows, int64_t groups, bool with_ptr, int64_t unit) {
 }
 
 // Workgroups go to the 8 XCDs round robin; tiles that share an operand should share an L2: XCD x takes the x-th eighth of the tiles.
-__device__ inline int64_t xcd_contiguous(int64_t block, int64_t blocks) {
-  const int64_t x = block % 8, q = blocks / 8, r = blocks % 8;
+// (32 bits from here to the tile: a launch has fewer than 2^31 workgroups, and a 64-bit division is some 140 instructions.)
+__device__ inline uint32_t xcd_contiguous(uint32_t block, uint32_t blocks) {
+  const uint32_t x = block % 8, q = blocks / 8, r = blocks % 8;
   return x * q + (x < r ? x : r) + block / 8;
 }
 
 // The reduction: the next step's operands are on their way from memory while this one's are multiplied.  NBUF 2: a barrier a step.
+// Whole steps run in a loop of their own: with both forms of a load behind one branch the compiler waits for the first operand's loads
+// before it issues the second's (64 experts' weight gradient: 480 us, see the kernel).
 template <typename T, int BM, int BN, int WM, int WN, int NBUF, typename SA, typename SB>
 __device__ inline void staged_products(SA &sa, SB &sb, Accum<T, BM, BN, WM, WN> &acc, char *lds, int64_t k_len, int tid, int wm, int wn, int lane) {
   constexpr int A_BYTES = Tile<T, BM>::BYTES, STAGE = A_BYTES + Tile<T, BN>::BYTES, BK = Elem<T>::BK;
   if (k_len <= 0) return;
-  sa.load(0, tid);
-  sb.load(0, tid);
+  const int64_t k_fast = sa.fast() && sb.fast() ? k_len : 0; // steps that end at or in front of it take load_fast
+  if (BK <= k_fast) {
+    sa.load_fast(0, tid);
+    sb.load_fast(0, tid);
+  } else {
+    sa.load_any(0, tid);
+    sb.load_any(0, tid);
+  }
+  int64_t k0 = 0;
   if constexpr (NBUF == 2) {
     sa.store(lds, tid);
     sb.store(lds + A_BYTES, tid);
-    if (BK < k_len) {
-      sa.load(BK, tid);
-      sb.load(BK, tid);
+    if (2 * BK <= k_fast) {
+      sa.load_fast(BK, tid);
+      sb.load_fast(BK, tid);
+    } else if (BK < k_len) {
+      sa.load_any(BK, tid);
+      sb.load_any(BK, tid);
     }
     __syncthreads();
-    int cur = 0;
-    for (int64_t k0 = 0; k0 < k_len; k0 += BK) {
-      char *now = lds + cur * STAGE, *next = lds + (cur ^ 1) * STAGE;
+    char *now = lds, *next = lds + STAGE;
+    auto turn = [&] {
+      __syncthreads();
+      char *t = now;
+      now = next;
+      next = t;
+    };
+    for (; k0 + 3 * BK <= k_fast; k0 += BK) {
+      acc.step(now, now + A_BYTES, wm, wn, lane);
+      sa.store(next, tid);
+      sb.store(next + A_BYTES, tid);
+      sa.load_fast(k0 + 2 * BK, tid);
+      sb.load_fast(k0 + 2 * BK, tid);
+      turn();
+    }
+    for (; k0 < k_len; k0 += BK) {
       acc.step(now, now + A_BYTES, wm, wn, lane);
       if (k0 + BK < k_len) {
         sa.store(next, tid);
         sb.store(next + A_BYTES, tid);
         if (k0 + 2 * BK < k_len) {
-          sa.load(k0 + 2 * BK, tid);
-          sb.load(k0 + 2 * BK, tid);
+          sa.load_any(k0 + 2 * BK, tid);
+          sb.load_any(k0 + 2 * BK, tid);
         }
       }
-      __syncthreads();
-      cur ^= 1;
+      turn();
     }
   } else {
-    for (int64_t k0 = 0; k0 < k_len; k0 += BK) {
+    for (; k0 + 2 * BK <= k_fast; k0 += BK) {
+      sa.store(lds, tid);
+      sb.store(lds + A_BYTES, tid);
+      sa.load_fast(k0 + BK, tid);
+      sb.load_fast(k0 + BK, tid);
+      __syncthreads();
+      acc.step(lds, lds + A_BYTES, wm, wn, lane);
+      __syncthreads();
+    }
+    for (; k0 < k_len; k0 += BK) {
       sa.store(lds, tid);
       sb.store(lds + A_BYTES, tid);
       if (k0 + BK < k_len) {
-        sa.load(k0 + BK, tid);
-        sb.load(k0 + BK, tid);
+        sa.load_any(k0 + BK, tid);
+        sb.load_any(k0 + BK, tid);
       }
       __syncthreads();
       acc.step(lds, lds + A_BYTES, wm, wn, lane);
@@ -497,7 +544,7 @@ struct RowsArgs {
   int64_t lda, ldb, ldr, ldy, b_group, bias_group; // strides in elements
   Groups groups;
   int64_t n, k;
-  int64_t slots, tiles_n, band; // band: row tiles of a group of tiles (tile_of)
+  uint32_t slots, tiles_n, band; // band: row tiles of a group of tiles (tile_of)
   int act;
 };
 
@@ -541,9 +588,9 @@ __device__ inline void finish_row(const RowsArgs &g, int64_t row, int64_t col, i
 // at one time on an XCD shares both operands (8 + 8 panels for 64 tiles instead of 2 + 32 in plain order at 32 column tiles).
 // Groups of rows (ptr) keep the plain order: row tiles side by side rarely share a matrix (64 groups of 512 rows, 1024 -> 2048 f16: 280 us
 // in plain order, 342 in bands of 8; without groups, 8192 x 4096 x 4096: 372 and 306).
-__device__ inline void tile_of(int64_t id, int64_t slots, int64_t tiles_n, int64_t band, int64_t &slot, int64_t &tile) {
-  const int64_t per = band * tiles_n, group = id / per, in = id % per, first = group * band;
-  const int64_t height = slots - first < band ? slots - first : band;
+__device__ inline void tile_of(uint32_t id, uint32_t slots, uint32_t tiles_n, uint32_t band, uint32_t &slot, uint32_t &tile) {
+  const uint32_t per = band * tiles_n, group = id / per, in = id % per, first = group * band;
+  const uint32_t height = slots - first < band ? slots - first : band;
   slot = first + in % height;
   tile = in / height;
 }
@@ -557,10 +604,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mm_rows_kernel(const RowsArgs
   constexpr int NT = 64 * WM * WN, STAGE = LA::BYTES + LB::BYTES, EPI = 32 * WM * (BN + 4) * 4;
   __shared__ __attribute__((aligned(16))) char lds[NBUF * STAGE > EPI ? NBUF * STAGE : EPI];
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, wm = wave / WN, wn = wave % WN;
-  int64_t slot, tile;
+  uint32_t slot, tile;
   tile_of(xcd_contiguous(blockIdx.x, gridDim.x), g.slots, g.tiles_n, g.band, slot, tile);
-  const int64_t n0 = tile * BN;
-  const Piece piece = piece_of(g.groups, BM, slot);
+  const int64_t n0 = (int64_t)tile * BN;
+  const Piece piece = piece_of(g.groups, __builtin_ctz(BM), slot);
   const int64_t r0 = piece.begin + piece.index * BM;
   if (r0 >= piece.end) return;
   const int64_t rows = piece.end - r0 < BM ? piece.end - r0 : BM;
@@ -630,7 +677,7 @@ template <typename T, int FM> __global__ __launch_bounds__(512, 2) void mm_few_r
   constexpr int W = 8, U = 4 / FM < 1 ? 1 : 4 / FM, P16 = 8 * sizeof(T) / 16;
   __shared__ __attribute__((aligned(16))) float part[W][32 * FM][36];
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
-  const int64_t tile = blockIdx.x % g.tiles_n, r0 = (int64_t)(blockIdx.x / g.tiles_n) * 32 * FM, n0 = tile * 32;
+  const int64_t r0 = (int64_t)(blockIdx.x / g.tiles_n) * 32 * FM, n0 = (int64_t)(blockIdx.x % g.tiles_n) * 32;
   const T *rows[FM + 1]; // of A, then of B: rows that do not exist read the last one
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
@@ -725,8 +772,9 @@ struct WeightArgs {
   float *part;         // partial products of the chunks of groups that have several: [slots][np * nq + (colsum ? ns : 0)]
   int64_t ldp, ldq, np, nq, ns;
   Groups groups;
-  int64_t unit;        // rows of a chunk
-  int64_t tiles_p, tiles_q;
+  int64_t unit;        // rows of a chunk: 1 << unit_log2
+  int unit_log2;
+  uint32_t tiles_p, tiles_q;
   int sum_p;
 };
 
@@ -738,9 +786,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mm_weight_kernel(const Weight
   constexpr int NT = 64 * WM * WN, STAGE = LA::BYTES + LB::BYTES, EPI = 32 * WM * (BN + 4) * 4;
   __shared__ __attribute__((aligned(16))) char lds[NBUF * STAGE > EPI ? NBUF * STAGE : EPI];
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, wm = wave / WN, wn = wave % WN;
-  const int64_t tile = xcd_contiguous(blockIdx.x, gridDim.x), tiles = g.tiles_p * g.tiles_q;
-  const int64_t slot = tile / tiles, t = tile % tiles, i0 = (t / g.tiles_q) * BM, j0 = (t % g.tiles_q) * BN;
-  const Piece piece = piece_of(g.groups, g.unit, slot);
+  const uint32_t tile = xcd_contiguous(blockIdx.x, gridDim.x), tiles = g.tiles_p * g.tiles_q, t = tile % tiles;
+  const int64_t slot = tile / tiles, i0 = (int64_t)(t / g.tiles_q) * BM, j0 = (int64_t)(t % g.tiles_q) * BN;
+  const Piece piece = piece_of(g.groups, g.unit_log2, slot);
   if (piece.group < 0) return;
   const int64_t len = piece.end - piece.begin, r0 = piece.begin + piece.index * g.unit;
   if (len > 0 ? r0 >= piece.end : piece.index > 0) return;   // (a group without rows still writes its zeros, once)
@@ -845,7 +893,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void mm_join_kernel
   if (!g.groups.ptr) piece = {0, 0, g.groups.rows, 0, 0};
   else {
     const int64_t q0 = g.groups.bound(group + 1), q1 = g.groups.bound(group + 2);
-    piece = {group, q0, q1, 0, q0 / g.unit + group + 1};
+    piece = {group, q0, q1, 0, (q0 >> g.unit_log2) + group + 1};
   }
   const int64_t len = piece.end - piece.begin;
   if (len <= g.unit) return;
@@ -904,15 +952,16 @@ int launched(const char *name) {
 constexpr int64_t kMaxBlocks = ((int64_t)1 << 31) - 1;
 
 template <typename T, int BM, int BN, int WM, int WN, bool BR, int NBUF> int run_rows(RowsArgs &g, hipStream_t st) {
-  g.tiles_n = (g.n + BN - 1) / BN;
-  g.slots = slots_of(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, BM);
-  if (g.slots > kMaxBlocks / g.tiles_n) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
+  const int64_t tiles_n = (g.n + BN - 1) / BN, slots = slots_of(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, BM);
+  if (tiles_n > kMaxBlocks / 8 || slots > kMaxBlocks / tiles_n) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
+  g.tiles_n = (uint32_t)tiles_n;
+  g.slots = (uint32_t)slots;
   g.band = g.groups.ptr ? 1 : 8;
   hipLaunchKernelGGL((mm_rows_kernel<T, BM, BN, WM, WN, BR, NBUF>), dim3((unsigned)(g.slots * g.tiles_n)), dim3(64 * WM * WN), 0, st, g);
   return launched("mm_rows_kernel");
 }
 template <typename T, int FM> int run_few(RowsArgs &g, hipStream_t st) {
-  g.tiles_n = (g.n + 31) / 32;
+  g.tiles_n = (uint32_t)((g.n + 31) / 32);
   const int64_t tiles_m = (g.groups.rows + 32 * FM - 1) / (32 * FM);
   hipLaunchKernelGGL((mm_few_rows_kernel<T, FM>), dim3((unsigned)(tiles_m * g.tiles_n)), dim3(512), 0, st, g);
   return launched("mm_few_rows_kernel");
@@ -945,6 +994,7 @@ int rows_product(RowsArgs &g, bool br, int dtype, hipStream_t st) {
 constexpr int64_t kWeightBlocks = 1024;
 struct WeightPlan {
   int64_t tiles_p, tiles_q, unit, slots;
+  int unit_log2;
 };
 WeightPlan weight_plan(int64_t rows, int64_t groups, bool with_ptr, int64_t np, int64_t nq) {
   WeightPlan w;
@@ -953,16 +1003,16 @@ WeightPlan weight_plan(int64_t rows, int64_t groups, bool with_ptr, int64_t np, 
   w.tiles_q = nq > 0 ? (nq + bn - 1) / bn : 1;
   const int64_t tiles = w.tiles_p * w.tiles_q;
   const int64_t want = kWeightBlocks / tiles > 1 ? kWeightBlocks / tiles : 1;
-  w.unit = (rows + want - 1) / want;
-  w.unit = w.unit < 256 ? 256 : (w.unit + 63) / 64 * 64;
-  w.slots = with_ptr ? rows / w.unit + groups + 2 : (rows + w.unit - 1) / w.unit;
+  w.unit_log2 = 8;
+  while (((int64_t)2 << w.unit_log2) * want <= rows) ++w.unit_log2; // the power of two at or below rows / want
+  w.unit = (int64_t)1 << w.unit_log2;
+  w.slots = slots_of(rows, groups, with_ptr, w.unit);
   if (w.slots < 1) w.slots = 1;
   return w;
 }
 template <typename T, int BM, int BN, int WM, int WN> int run_weight(WeightArgs &g, int64_t slots, hipStream_t st) {
   constexpr int NBUF = Elem<T>::PARTS == 1 ? 2 : 1;
-  const int64_t tiles = g.tiles_p * g.tiles_q;
-  if (slots > kMaxBlocks / tiles) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
+  const int64_t tiles = (int64_t)g.tiles_p * g.tiles_q;
   hipLaunchKernelGGL((mm_weight_kernel<T, BM, BN, WM, WN, NBUF>), dim3((unsigned)(slots * tiles)), dim3(64 * WM * WN), 0, st, g);
   if (const int rc = launched("mm_weight_kernel")) return rc;
   if (g.groups.rows > g.unit) { // some group may have several chunks
@@ -983,9 +1033,11 @@ template <typename T> int weight_typed(WeightArgs &g, int64_t slots, hipStream_t
 int weight_product(WeightArgs &g, int dtype, void *workspace, size_t workspace_bytes, hipStream_t st) {
   if (g.groups.groups == 0 || (g.np * g.nq == 0 && !(g.colsum && g.ns > 0))) return GEOT_OK;
   const WeightPlan w = weight_plan(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, g.np, g.nq);
+  if (w.tiles_p * w.tiles_q > kMaxBlocks / w.slots) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
   g.unit = w.unit;
-  g.tiles_p = w.tiles_p;
-  g.tiles_q = w.tiles_q;
+  g.unit_log2 = w.unit_log2;
+  g.tiles_p = (uint32_t)w.tiles_p;
+  g.tiles_q = (uint32_t)w.tiles_q;
   g.part = static_cast<float *>(workspace);
   if (g.groups.rows > w.unit) {
     const size_t need = (size_t)w.slots * (size_t)(g.np * g.nq + (g.colsum ? g.ns : 0)) * sizeof(float);
