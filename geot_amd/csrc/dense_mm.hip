@@ -597,7 +597,7 @@ __device__ inline void tile_of(uint32_t id, uint32_t slots, uint32_t tiles_n, ui
 
 // y rows.  BR: B's output index is contiguous (element (n, k) at b[k * ldb + n]), otherwise its reduction index (b[n * ldb + k]).
 template <typename T, int BM, int BN, int WM, int WN, bool BR, int NBUF>
-__global__ __launch_bounds__(64 * WM * WN, 2) void mm_rows_kernel(const RowsArgs g) {
+__global__ __launch_bounds__(64 * WM * WN, NBUF == 1 ? 3 : 2) void mm_rows_kernel(const RowsArgs g) {
   using E = Elem<T>;
   using LA = Tile<T, BM>;
   using LB = Tile<T, BN>;
@@ -772,14 +772,14 @@ struct WeightArgs {
   float *part;         // partial products of the chunks of groups that have several: [slots][np * nq + (colsum ? ns : 0)]
   int64_t ldp, ldq, np, nq, ns;
   Groups groups;
-  int64_t unit;        // rows of a chunk: 1 << unit_log2
+  int64_t unit;        // rows of a chunk; with groups 1 << unit_log2
   int unit_log2;
   uint32_t tiles_p, tiles_q;
   int sum_p;
 };
 
 template <typename T, int BM, int BN, int WM, int WN, int NBUF>
-__global__ __launch_bounds__(64 * WM * WN, 2) void mm_weight_kernel(const WeightArgs g) {
+__global__ __launch_bounds__(64 * WM * WN, 3) void mm_weight_kernel(const WeightArgs g) {
   using E = Elem<T>;
   using LA = Tile<T, BM>;
   using LB = Tile<T, BN>;
@@ -971,14 +971,12 @@ template <typename T, bool BR> int rows_typed(RowsArgs &g, hipStream_t st) {
   if constexpr (!BR) {
     if (!g.groups.ptr && tiles < 128 && g.k >= 128) return g.groups.rows <= 32 ? run_few<T, 1>(g, st) : run_few<T, 2>(g, st);
   }
-  constexpr int LONG = Elem<T>::PARTS == 1 ? 2 : 1;
-  const bool shallow = g.k <= 4 * Elem<T>::BK;
-  if (g.n <= 64) return shallow ? run_rows<T, 128, 64, 2, 2, BR, 1>(g, st) : run_rows<T, 128, 64, 2, 2, BR, LONG>(g, st);
+  if (g.n <= 64) return run_rows<T, 128, 64, 2, 2, BR, 1>(g, st);
   if constexpr (Elem<T>::PARTS == 1) {
     const int64_t per_group = g.groups.ptr ? g.groups.rows / (g.groups.groups > 0 ? g.groups.groups : 1) : g.groups.rows;
     if (g.n > 128 && g.k >= 512 && tiles >= 1024 && per_group >= 2048) return run_rows<T, 256, 256, 2, 4, BR, 2>(g, st);
   }
-  return shallow ? run_rows<T, 128, 128, 2, 2, BR, 1>(g, st) : run_rows<T, 128, 128, 2, 2, BR, LONG>(g, st);
+  return run_rows<T, 128, 128, 2, 2, BR, 1>(g, st);
 }
 int rows_product(RowsArgs &g, bool br, int dtype, hipStream_t st) {
   if (g.groups.rows == 0 || g.n == 0) return GEOT_OK;
@@ -990,8 +988,8 @@ int rows_product(RowsArgs &g, bool br, int dtype, hipStream_t st) {
   return geot_internal_fail(GEOT_EUNSUPPORTED, "matrix products take float32, float16 and bfloat16");
 }
 
-// Chunks of rows.  Enough workgroups to fill the chip (kWeightBlocks), and no chunk below 256 rows.
-constexpr int64_t kWeightBlocks = 1024;
+// Chunks of rows: one full round of workgroups (3 a CU, 4 of the 64 x 64 tiles), and no chunk below 256 rows.  Groups of rows take chunks
+// of a power of two (piece_of).
 struct WeightPlan {
   int64_t tiles_p, tiles_q, unit, slots;
   int unit_log2;
@@ -1002,16 +1000,21 @@ WeightPlan weight_plan(int64_t rows, int64_t groups, bool with_ptr, int64_t np, 
   w.tiles_p = np > 0 ? (np + bm - 1) / bm : 1; // (a side of width 0 still has its column sums)
   w.tiles_q = nq > 0 ? (nq + bn - 1) / bn : 1;
   const int64_t tiles = w.tiles_p * w.tiles_q;
-  const int64_t want = kWeightBlocks / tiles > 1 ? kWeightBlocks / tiles : 1;
+  const int64_t round = np <= 64 && nq <= 64 ? 1024 : 768, want = round / tiles > 1 ? round / tiles : 1;
   w.unit_log2 = 8;
-  while (((int64_t)2 << w.unit_log2) * want <= rows) ++w.unit_log2; // the power of two at or below rows / want
-  w.unit = (int64_t)1 << w.unit_log2;
+  if (with_ptr) {
+    while (((int64_t)2 << w.unit_log2) * want <= rows) ++w.unit_log2; // the power of two at or below rows / want
+    w.unit = (int64_t)1 << w.unit_log2;
+  } else {
+    w.unit = ((rows + want - 1) / want + 63) / 64 * 64;
+    w.unit = w.unit < 256 ? 256 : w.unit;
+  }
   w.slots = slots_of(rows, groups, with_ptr, w.unit);
   if (w.slots < 1) w.slots = 1;
   return w;
 }
 template <typename T, int BM, int BN, int WM, int WN> int run_weight(WeightArgs &g, int64_t slots, hipStream_t st) {
-  constexpr int NBUF = Elem<T>::PARTS == 1 ? 2 : 1;
+  constexpr int NBUF = 1;
   const int64_t tiles = (int64_t)g.tiles_p * g.tiles_q;
   hipLaunchKernelGGL((mm_weight_kernel<T, BM, BN, WM, WN, NBUF>), dim3((unsigned)(slots * tiles)), dim3(64 * WM * WN), 0, st, g);
   if (const int rc = launched("mm_weight_kernel")) return rc;
