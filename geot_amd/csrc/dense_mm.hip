@@ -173,7 +173,7 @@ template <typename T, int R, int NT, bool SUM> struct StageR {
   static constexpr int BLOCKS = (R / VR) * L::CK;
   static constexpr int N = (BLOCKS + NT - 1) / NT;
   static constexpr bool WHOLE = BLOCKS % NT == 0;
-  u32x2 reg[N][8];
+  u32x2 reg[N][8] = {};
   float sum[SUM ? N : 1][VR];
   const T *base;
   int64_t ld, k_end;
@@ -198,7 +198,8 @@ template <typename T, int R, int NT, bool SUM> struct StageR {
   __device__ void load_fast(int64_t k0, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = tid + i * NT, row = (idx % (R / VR)) * VR, chunk = WHOLE || idx < BLOCKS ? idx / (R / VR) : 0;
+      const int idx = tid + i * NT, row = (idx % (R / VR)) * VR, chunk = idx / (R / VR);
+      if (!WHOLE && idx >= BLOCKS) continue; // (whole waves)
       const T *p = base + (k0 + chunk * 8) * ld + (row + VR <= rows ? row : rows - VR);
 #pragma unroll
       for (int j = 0; j < 8; ++j) reg[i][j] = *reinterpret_cast<const Packed8<T> *>(p + j * ld);
@@ -207,7 +208,8 @@ template <typename T, int R, int NT, bool SUM> struct StageR {
   __device__ void load_any(int64_t k0, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int idx = tid + i * NT, row = (idx % (R / VR)) * VR, chunk = WHOLE || idx < BLOCKS ? idx / (R / VR) : 0;
+      const int idx = tid + i * NT, row = (idx % (R / VR)) * VR, chunk = idx / (R / VR);
+      if (!WHOLE && idx >= BLOCKS) continue;
       const T *p = base + (k0 + chunk * 8) * ld + row;
       const bool wide = row + VR <= rows;
 #pragma unroll
@@ -342,17 +344,16 @@ __device__ inline bool finite(float v) { return (__float_as_uint(v) & 0x7f800000
 struct Normal {
   float tail, bell; // Phi(-|z|), exp(-z^2 / 2)
 };
-template <bool EXACT> __device__ inline Normal normal_of(float z) {
-  // (EXACT: exp(-200) is 0 in float32, nothing changes behind 20 but inf - inf below; a NaN goes on in z)
-  const float a = EXACT ? fminf(fabsf(z), 20.0f) : fabsf(z);
+__device__ inline Normal normal_of(float z) {
+  // (exp(-200) is 0 in float32, nothing changes behind 20 but inf - inf below; a NaN goes on in z)
+  const float a = fminf(fabsf(z), 20.0f);
   const float t = __builtin_amdgcn_rcpf(fmaf(0.26f, a, 1.0f));
   constexpr float half_log2e = 0.72134752044448170f;
   const float sq = a * a, arg = sq * half_log2e;
   float bell = __builtin_amdgcn_exp2f(-arg);
-  if constexpr (EXACT) { // what the two products above rounded away (up to 24 x 2^-24 in the argument)
-    const float rest = fmaf(sq, half_log2e, -arg) + fmaf(a, a, -sq) * half_log2e;
-    bell = fmaf(bell * rest, -0.69314718055994531f, bell);
-  }
+  // what the two products above rounded away (up to 24 x 2^-24 in the argument)
+  const float rest = fmaf(sq, half_log2e, -arg) + fmaf(a, a, -sq) * half_log2e;
+  bell = fmaf(bell * rest, -0.69314718055994531f, bell);
   float r = 0.030395518988370895f;
   r = fmaf(r, t, -0.15229645371437073f);
   r = fmaf(r, t, 0.25038889050483704f);
@@ -363,6 +364,35 @@ template <bool EXACT> __device__ inline Normal normal_of(float z) {
   r = fmaf(r, t, 0.10303061455488205f);
   r = fmaf(r, t, 0.10375823080539703f);
   return {r * t * bell, bell};
+}
+// 16-bit results: fewer instructions (the exact form's 25 an element were 610 us of vector time in the layer above).  log2 Phi(-a) is close
+// to a parabola: a polynomial of degree 7 in the exponent, 2.7e-5 (2^-15.2) of the value up to a = 6 and falling on behind.
+__device__ inline float gelu16(float z) {
+  const float a = fminf(fabsf(z), 16.0f);
+  float p = 1.122847152146278e-06f;
+  p = fmaf(p, a, -4.626810914487578e-05f);
+  p = fmaf(p, a, 0.0008012278121896088f);
+  p = fmaf(p, a, -0.007969655096530914f);
+  p = fmaf(p, a, 0.05281980335712433f);
+  p = fmaf(p, a, 0.45959118008613586f);
+  p = fmaf(p, a, 1.1508647203445435f);
+  p = fmaf(p, a, 1.0f);
+  // max(z, 0) - a Phi(-a), the maximum as a half sum: NaN stays
+  return fmaf(-a, __builtin_amdgcn_exp2f(-p), fmaf(0.5f, fabsf(z), 0.5f * z));
+}
+// gelu'(-a) = exp(-a^2 / 2) (R(a) - a / sqrt(2 pi)), gelu'(z) + gelu'(-z) = 1: degree 7 in a, 2.4e-5 (2^-15.3) absolute
+__device__ inline float gelu_slope16(float z) {
+  const float a = fminf(fabsf(z), 16.0f);
+  float q = -4.211963459965773e-05f;
+  q = fmaf(q, a, 0.0009205337846651673f);
+  q = fmaf(q, a, -0.0081043541431427f);
+  q = fmaf(q, a, 0.03846684470772743f);
+  q = fmaf(q, a, -0.1147356703877449f);
+  q = fmaf(q, a, 0.24307765066623688f);
+  q = fmaf(q, a, -0.79688920f);
+  q = fmaf(q, a, 0.4999766945838928f);
+  q *= __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+  return z < 0.0f ? q : 1.0f - q;
 }
 template <bool EXACT> __device__ inline float logistic(float z) {
   constexpr float log2e = 1.44269504088896341f;
@@ -377,17 +407,19 @@ template <bool EXACT> __device__ inline float logistic(float z) {
 // ACT is a compile-time choice inside the loops over elements.  T: float operands take the exact forms.
 template <typename T, int ACT> __device__ inline float activate(float z) {
   if constexpr (ACT == GEOT_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
+  else if constexpr (ACT == GEOT_ACT_GELU && sizeof(T) == 2) return gelu16(z);
   else if constexpr (ACT == GEOT_ACT_GELU) { // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
-    const float y = fmaf(-fabsf(z), normal_of<sizeof(T) == 4>(z).tail, fmaxf(z, 0.0f));
-    return sizeof(T) == 4 && z != z ? z : y; // (16 bits: the tail of a NaN is one)
+    const float y = fmaf(-fabsf(z), normal_of(z).tail, fmaxf(z, 0.0f));
+    return z != z ? z : y;
   }
   else if constexpr (ACT == GEOT_ACT_SILU) return z * logistic<sizeof(T) == 4>(z);
   else return z;
 }
 template <typename T, int ACT> __device__ inline float activation_slope(float z) {
   if constexpr (ACT == GEOT_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
+  else if constexpr (ACT == GEOT_ACT_GELU && sizeof(T) == 2) return gelu_slope16(z);
   else if constexpr (ACT == GEOT_ACT_GELU) {
-    const Normal n = normal_of<sizeof(T) == 4>(z);
+    const Normal n = normal_of(z);
     return fmaf(z * 0.39894228040143268f, n.bell, z < 0.0f ? n.tail : 1.0f - n.tail);
   } else if constexpr (ACT == GEOT_ACT_SILU) {
     const float s = logistic<sizeof(T) == 4>(z);
@@ -467,24 +499,25 @@ template <typename T, int BM, int BN, int WM, int WN, int NBUF, typename SA, typ
 __device__ inline void staged_products(SA &sa, SB &sb, Accum<T, BM, BN, WM, WN> &acc, char *lds, int64_t k_len, int tid, int wm, int wn, int lane) {
   constexpr int A_BYTES = Tile<T, BM>::BYTES, STAGE = A_BYTES + Tile<T, BN>::BYTES, BK = Elem<T>::BK;
   if (k_len <= 0) return;
+  const int tb = (tid + 32 * WM * WN) % (64 * WM * WN); // (where a tile is fewer blocks than threads, the other half of them stages B)
   const int64_t k_fast = sa.fast() && sb.fast() ? k_len : 0; // steps that end at or in front of it take load_fast
   if (BK <= k_fast) {
     sa.load_fast(0, tid);
-    sb.load_fast(0, tid);
+    sb.load_fast(0, tb);
   } else {
     sa.load_any(0, tid);
-    sb.load_any(0, tid);
+    sb.load_any(0, tb);
   }
   int64_t k0 = 0;
   if constexpr (NBUF == 2) {
     sa.store(lds, tid);
-    sb.store(lds + A_BYTES, tid);
+    sb.store(lds + A_BYTES, tb);
     if (2 * BK <= k_fast) {
       sa.load_fast(BK, tid);
-      sb.load_fast(BK, tid);
+      sb.load_fast(BK, tb);
     } else if (BK < k_len) {
       sa.load_any(BK, tid);
-      sb.load_any(BK, tid);
+      sb.load_any(BK, tb);
     }
     __syncthreads();
     char *now = lds, *next = lds + STAGE;
@@ -497,19 +530,19 @@ __device__ inline void staged_products(SA &sa, SB &sb, Accum<T, BM, BN, WM, WN> 
     for (; k0 + 3 * BK <= k_fast; k0 += BK) {
       acc.step(now, now + A_BYTES, wm, wn, lane);
       sa.store(next, tid);
-      sb.store(next + A_BYTES, tid);
+      sb.store(next + A_BYTES, tb);
       sa.load_fast(k0 + 2 * BK, tid);
-      sb.load_fast(k0 + 2 * BK, tid);
+      sb.load_fast(k0 + 2 * BK, tb);
       turn();
     }
     for (; k0 < k_len; k0 += BK) {
       acc.step(now, now + A_BYTES, wm, wn, lane);
       if (k0 + BK < k_len) {
         sa.store(next, tid);
-        sb.store(next + A_BYTES, tid);
+        sb.store(next + A_BYTES, tb);
         if (k0 + 2 * BK < k_len) {
           sa.load_any(k0 + 2 * BK, tid);
-          sb.load_any(k0 + 2 * BK, tid);
+          sb.load_any(k0 + 2 * BK, tb);
         }
       }
       turn();
@@ -517,19 +550,19 @@ __device__ inline void staged_products(SA &sa, SB &sb, Accum<T, BM, BN, WM, WN> 
   } else {
     for (; k0 + 2 * BK <= k_fast; k0 += BK) {
       sa.store(lds, tid);
-      sb.store(lds + A_BYTES, tid);
+      sb.store(lds + A_BYTES, tb);
       sa.load_fast(k0 + BK, tid);
-      sb.load_fast(k0 + BK, tid);
+      sb.load_fast(k0 + BK, tb);
       __syncthreads();
       acc.step(lds, lds + A_BYTES, wm, wn, lane);
       __syncthreads();
     }
     for (; k0 < k_len; k0 += BK) {
       sa.store(lds, tid);
-      sb.store(lds + A_BYTES, tid);
+      sb.store(lds + A_BYTES, tb);
       if (k0 + BK < k_len) {
         sa.load_any(k0 + BK, tid);
-        sb.load_any(k0 + BK, tid);
+        sb.load_any(k0 + BK, tb);
       }
       __syncthreads();
       acc.step(lds, lds + A_BYTES, wm, wn, lane);
@@ -548,40 +581,94 @@ struct RowsArgs {
   int act;
 };
 
-// V consecutive columns of one row: bias, z, activation, residual, y.  cols of them exist.
-template <typename T, int V, int ACT>
-__device__ inline void finish_row(const RowsArgs &g, int64_t row, int64_t col, int cols, float (&v)[V], const float (&bias)[V]) {
-  using Vec = Packed16<T>;
+// V consecutive columns of a row, `cols` of which exist
+template <typename T, int V> __device__ inline u32x4 load_cols(const T *p, int cols) {
+  if (cols == V) return *reinterpret_cast<const Packed16<T> *>(p);
   alignas(16) T tmp[V];
 #pragma unroll
-  for (int c = 0; c < V; ++c) v[c] += bias[c];
-  if (g.z) {
-    T *zp = static_cast<T *>(g.z) + row * g.n + col;
-#pragma unroll
-    for (int c = 0; c < V; ++c) tmp[c] = (T)v[c];
-    if (cols == V) *reinterpret_cast<Vec *>(zp) = *reinterpret_cast<const u32x4 *>(tmp);
-    else
-      for (int c = 0; c < V; ++c)
-        if (c < cols) zp[c] = tmp[c];
-  }
-#pragma unroll
-  for (int c = 0; c < V; ++c) v[c] = activate<T, ACT>(v[c]);
-  if (g.residual) {
-    const T *rp = static_cast<const T *>(g.residual) + row * g.ldr + col;
-    if (cols == V) *reinterpret_cast<u32x4 *>(tmp) = *reinterpret_cast<const Vec *>(rp);
-    else
-#pragma unroll
-      for (int c = 0; c < V; ++c) tmp[c] = c < cols ? rp[c] : (T)0.0f;
-#pragma unroll
-    for (int c = 0; c < V; ++c) v[c] += as_float(tmp[c]);
-  }
-  T *yp = static_cast<T *>(g.y) + row * g.ldy + col;
+  for (int c = 0; c < V; ++c) tmp[c] = c < cols ? p[c] : (T)0.0f;
+  return *reinterpret_cast<const u32x4 *>(tmp);
+}
+template <typename T, int V> __device__ inline void store_cols(T *p, int cols, const float (&v)[V]) {
+  alignas(16) T tmp[V];
 #pragma unroll
   for (int c = 0; c < V; ++c) tmp[c] = (T)v[c];
-  if (cols == V) *reinterpret_cast<Vec *>(yp) = *reinterpret_cast<const u32x4 *>(tmp);
+  if (cols == V) *reinterpret_cast<Packed16<T> *>(p) = *reinterpret_cast<const u32x4 *>(tmp);
   else
+#pragma unroll
     for (int c = 0; c < V; ++c)
-      if (c < cols) yp[c] = tmp[c];
+      if (c < cols) p[c] = tmp[c];
+}
+// What becomes of a row's sums.  DZ false: y = act(z) + residual, z stored if asked for; `ext` is the residual's row.  DZ true:
+// dz = dy act'(z), added up per column; `ext` is dy's.
+template <typename T, int V, int ACT, bool DZ>
+__device__ inline void finish_row(const RowsArgs &g, int64_t row, int64_t col, int cols, float (&v)[V], const float (&bias)[V], bool has_ext, u32x4 ext, float (&sum)[V]) {
+  alignas(16) T tmp[V];
+  *reinterpret_cast<u32x4 *>(tmp) = ext;
+#pragma unroll
+  for (int c = 0; c < V; ++c) v[c] += bias[c];
+  if constexpr (DZ) {
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      v[c] = as_float(tmp[c]) * activation_slope<T, ACT>(v[c]);
+      sum[c] += v[c];
+    }
+  } else {
+    if (g.z) store_cols<T, V>(static_cast<T *>(g.z) + row * g.n + col, cols, v);
+#pragma unroll
+    for (int c = 0; c < V; ++c) v[c] = activate<T, ACT>(v[c]);
+    if (has_ext) {
+#pragma unroll
+      for (int c = 0; c < V; ++c) v[c] += as_float(tmp[c]);
+    }
+  }
+  store_cols<T, V>(static_cast<T *>(g.y) + row * g.ldy + col, cols, v);
+}
+
+// A finished tile: 32 * WM rows at a time through LDS, so that every access to memory is whole rows, V consecutive columns a thread.  What
+// is read beside the sums (the residual, dy) is on its way before the barriers.  a_row(r) / b_col(c): the operands of element_again.
+template <typename T, int BM, int BN, int WM, int WN, int ACT, bool DZ, bool BR>
+__device__ inline void tile_epilogue(const RowsArgs &g, const Accum<T, BM, BN, WM, WN> &acc, float *out, const T *ext, int64_t ld_ext, const T *B, int64_t r0, int64_t rows,
+                                     int64_t nc, int cols, int64_t k_len, const float (&bias)[16 / sizeof(T)], float (&sum)[16 / sizeof(T)], int tid, int wm, int wn, int lane) {
+  constexpr int NT = 64 * WM * WN, V = 16 / sizeof(T), TPR = BN / V, RPP = NT / TPR, PASSES = 32 * WM / RPP;
+  const int col = (tid % TPR) * V;
+#pragma unroll
+  for (int i = 0; i < acc.FM; ++i) {
+    u32x4 pre[PASSES];
+    if (ext && cols > 0) {
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const int64_t tr = acc.tile_row(tid / TPR + p * RPP, i), row = r0 + (tr < rows ? tr : rows - 1);
+        pre[p] = load_cols<T, V>(ext + row * ld_ext + nc, cols);
+      }
+    }
+    if (i) __syncthreads();
+    acc.put(out, i, wm, wn, lane);
+    __syncthreads();
+    if (cols > 0) {
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const int lr = tid / TPR + p * RPP;
+        const int64_t tr = acc.tile_row(lr, i), row = r0 + tr;
+        if (tr >= rows) continue;
+        float v[V];
+#pragma unroll
+        for (int c = 0; c < V; c += 4) {
+          const f32x4 q = *reinterpret_cast<const f32x4 *>(out + lr * (BN + 4) + col + c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[c + e] = q[e];
+        }
+        if constexpr (Elem<T>::PARTS == 3) {
+#pragma unroll
+          for (int c = 0; c < V; ++c)
+            if (!finite(v[c]) && c < cols)
+              v[c] = element_again(static_cast<const float *>(g.a) + row * g.lda, 1, reinterpret_cast<const float *>(B) + (BR ? nc + c : (nc + c) * g.ldb),
+                                   BR ? g.ldb : 1, k_len);
+        }
+        finish_row<T, V, ACT, DZ>(g, row, nc, cols, v, bias, ext != nullptr, pre[p], sum);
+      }
+    }
+  }
 }
 
 // A workgroup's tile: groups of 8 row tiles, inside a group the column tiles one after the other with the 8 row tiles fastest - what runs
@@ -624,47 +711,65 @@ __global__ __launch_bounds__(64 * WM * WN, NBUF == 1 ? 3 : 2) void mm_rows_kerne
   sb.open(B, g.ldb, n0, g.n - n0, 0, k_len);
   staged_products<T, BM, BN, WM, WN, NBUF>(sa, sb, acc, lds, k_len, tid, wm, wn, lane);
 
-  // epilogue: 32 * WM rows at a time through LDS, so that every access to memory is whole rows; V consecutive columns a thread
+  constexpr int V = 16 / sizeof(T), TPR = BN / V;
+  const int64_t nc = n0 + (tid % TPR) * V;
+  const int cols = nc + V <= g.n ? V : (nc < g.n ? (int)(g.n - nc) : 0);
+  float bias[V], none[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    bias[v] = g.bias && real && v < cols ? as_float(static_cast<const T *>(g.bias)[piece.group * g.bias_group + nc + v]) : 0.0f;
+  by_activation(g.act, [&](auto act) {
+    tile_epilogue<T, BM, BN, WM, WN, decltype(act)::value, false, BR>(g, acc, reinterpret_cast<float *>(lds), static_cast<const T *>(g.residual), g.ldr, B, r0, rows, nc, cols,
+                                                                     k_len, bias, none, tid, wm, wn, lane);
+  });
+}
+
+// dz = dy act'(z) with z = x W^T + b computed again instead of read: narrow layers are bound by memory, and z costs a write in the forward
+// pass and a read here where x, which the weight's gradient reads anyway, is all this needs (2.4 M x 128 -> 256 bf16: 3.8 GB and 850 us
+// for dz from a saved z, 3.1 GB so, and the forward pass writes 1.3 GB less).  z is not rounded on its way.  Column sums of dz - the bias's
+// gradient - are taken before its rounding, one row of partial sums a row tile.  (One workgroup over several row tiles spilled 70 registers: 2057 us.)
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 3) void mm_preactivation_kernel(const RowsArgs g, const T *dy, float *part) {
+  constexpr int NT = 64 * WM * WN, STAGE = Tile<T, BM>::BYTES + Tile<T, BN>::BYTES, EPI = 32 * WM * (BN + 4) * 4;
+  __shared__ __attribute__((aligned(16))) char lds[STAGE > EPI ? STAGE : EPI];
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, wm = wave / WN, wn = wave % WN;
+  uint32_t slot, tile;
+  tile_of(xcd_contiguous(blockIdx.x, gridDim.x), g.slots, g.tiles_n, g.band, slot, tile);
+  const int64_t n0 = (int64_t)tile * BN, r0 = (int64_t)slot * BM, rows = g.groups.rows - r0 < BM ? g.groups.rows - r0 : BM;
+  Accum<T, BM, BN, WM, WN> acc;
+  acc.clear();
+  {
+    StageK<T, BM, NT> sa;
+    StageK<T, BN, NT> sb;
+    sa.open(static_cast<const T *>(g.a), g.lda, r0, rows, 0, g.k);
+    sb.open(static_cast<const T *>(g.b), g.ldb, n0, g.n - n0, 0, g.k);
+    staged_products<T, BM, BN, WM, WN, 1>(sa, sb, acc, lds, g.k, tid, wm, wn, lane);
+  }
   constexpr int V = 16 / sizeof(T), TPR = BN / V, RPP = NT / TPR;
   const int col = (tid % TPR) * V;
   const int64_t nc = n0 + col;
   const int cols = nc + V <= g.n ? V : (nc < g.n ? (int)(g.n - nc) : 0);
-  float bias[V];
+  float bias[V], sum[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v)
-    bias[v] = g.bias && real && v < cols ? as_float(static_cast<const T *>(g.bias)[piece.group * g.bias_group + nc + v]) : 0.0f;
+  for (int v = 0; v < V; ++v) {
+    bias[v] = g.bias && v < cols ? as_float(static_cast<const T *>(g.bias)[nc + v]) : 0.0f;
+    sum[v] = 0.0f;
+  }
   float *out = reinterpret_cast<float *>(lds);
   by_activation(g.act, [&](auto act) {
-#pragma unroll
-    for (int i = 0; i < acc.FM; ++i) {
-      if (i) __syncthreads();
-      acc.put(out, i, wm, wn, lane);
-      __syncthreads();
-      if (cols > 0) {
-#pragma unroll 2
-        for (int lr = tid / TPR; lr < 32 * WM; lr += RPP) {
-          const int64_t tr = acc.tile_row(lr, i);
-          if (tr >= rows) continue;
-          const int64_t row = r0 + tr;
-          float v[V];
-#pragma unroll
-          for (int c = 0; c < V; c += 4) {
-            const f32x4 q = *reinterpret_cast<const f32x4 *>(out + lr * (BN + 4) + col + c);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[c + e] = q[e];
-          }
-          if constexpr (E::PARTS == 3) {
-#pragma unroll
-            for (int c = 0; c < V; ++c)
-              if (!finite(v[c]) && c < cols)
-                v[c] = element_again(reinterpret_cast<const float *>(A) + row * g.lda, 1,
-                                     reinterpret_cast<const float *>(B) + (BR ? nc + c : (nc + c) * g.ldb), BR ? g.ldb : 1, k_len);
-          }
-          finish_row<T, V, decltype(act)::value>(g, row, nc, cols, v, bias);
-        }
-      }
-    }
+    tile_epilogue<T, BM, BN, WM, WN, decltype(act)::value, true, false>(g, acc, out, dy, g.n, static_cast<const T *>(g.b), r0, rows, nc, cols, g.k, bias, sum, tid, wm, wn,
+                                                                       lane);
   });
+  if (!part) return;
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < V; ++v) out[(tid / TPR) * BN + col + v] = sum[v];
+  __syncthreads();
+  for (int c = tid; c < BN && n0 + c < g.n; c += NT) {
+    float s = 0.0f;
+    for (int r = 0; r < RPP; ++r) s += out[r * BN + c];
+    part[(int64_t)slot * g.n + n0 + c] = s;
+  }
 }
 
 // Few rows (or few columns): too few tiles to fill the chip, and the time of a call is that of reading one operand - for a single row of
@@ -740,7 +845,7 @@ template <typename T, int FM> __global__ __launch_bounds__(512, 2) void mm_few_r
   const int64_t nc = n0 + col;
   const int cols = nc + V <= g.n ? V : (nc < g.n ? (int)(g.n - nc) : 0);
   if (cols == 0) return;
-  float bias[V];
+  float bias[V], none[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) bias[v] = g.bias && v < cols ? as_float(static_cast<const T *>(g.bias)[nc + v]) : 0.0f;
   for (int lr = tid / TPR; lr < 32 * FM && r0 + lr < g.groups.rows; lr += 512 / TPR) {
@@ -761,7 +866,9 @@ template <typename T, int FM> __global__ __launch_bounds__(512, 2) void mm_few_r
         if (!finite(v[c]) && c < cols)
           v[c] = element_again(static_cast<const float *>(g.a) + (r0 + lr) * g.lda, 1, static_cast<const float *>(g.b) + (nc + c) * g.ldb, 1, g.k);
     }
-    by_activation(g.act, [&](auto act) { finish_row<T, V, decltype(act)::value>(g, r0 + lr, nc, cols, v, bias); });
+    u32x4 ext = {0, 0, 0, 0};
+    if (g.residual) ext = load_cols<T, V>(static_cast<const T *>(g.residual) + (r0 + lr) * g.ldr + nc, cols);
+    by_activation(g.act, [&](auto act) { finish_row<T, V, decltype(act)::value, false>(g, r0 + lr, nc, cols, v, bias, g.residual != nullptr, ext, none); });
   }
 }
 
@@ -778,13 +885,18 @@ struct WeightArgs {
   int sum_p;
 };
 
-template <typename T, int BM, int BN, int WM, int WN, int NBUF>
+template <int WHICH, typename A, typename B> __device__ inline auto &pick(A &a, B &b) {
+  if constexpr (WHICH == 1) return a;
+  else return b;
+}
+// SUMS: column sums of nothing (0), p (1) or q (2) beside the product
+template <typename T, int BM, int BN, int WM, int WN, int SUMS>
 __global__ __launch_bounds__(64 * WM * WN, 3) void mm_weight_kernel(const WeightArgs g) {
   using E = Elem<T>;
   using LA = Tile<T, BM>;
   using LB = Tile<T, BN>;
   constexpr int NT = 64 * WM * WN, STAGE = LA::BYTES + LB::BYTES, EPI = 32 * WM * (BN + 4) * 4;
-  __shared__ __attribute__((aligned(16))) char lds[NBUF * STAGE > EPI ? NBUF * STAGE : EPI];
+  __shared__ __attribute__((aligned(16))) char lds[STAGE > EPI ? STAGE : EPI];
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, wm = wave / WN, wn = wave % WN;
   const uint32_t tile = xcd_contiguous(blockIdx.x, gridDim.x), tiles = g.tiles_p * g.tiles_q, t = tile % tiles;
   const int64_t slot = tile / tiles, i0 = (int64_t)(t / g.tiles_q) * BM, j0 = (int64_t)(t % g.tiles_q) * BN;
@@ -795,18 +907,17 @@ __global__ __launch_bounds__(64 * WM * WN, 3) void mm_weight_kernel(const Weight
   const int64_t r1 = len <= 0 ? r0 : (r0 + g.unit < piece.end ? r0 + g.unit : piece.end);
   const bool whole = len <= g.unit;                          // this chunk is all of its group
   const T *P = static_cast<const T *>(g.p), *Q = static_cast<const T *>(g.q);
-  const bool sums = g.colsum && (g.sum_p ? j0 == 0 : i0 == 0);
+  const bool sums = SUMS == 1 ? j0 == 0 : SUMS == 2 && i0 == 0;
 
   Accum<T, BM, BN, WM, WN> acc;
   acc.clear();
-  StageR<T, BM, NT, true> sa;
-  StageR<T, BN, NT, true> sb;
+  StageR<T, BM, NT, SUMS == 1> sa;
+  StageR<T, BN, NT, SUMS == 2> sb;
   sa.open(P, g.ldp, i0, g.np - i0, r0, r1);
   sb.open(Q, g.ldq, j0, g.nq - j0, r0, r1);
-  sa.add = sums && g.sum_p;
-  sb.add = sums && !g.sum_p;
+  sa.add = sb.add = sums;
   const int64_t k_len = r1 - r0;
-  staged_products<T, BM, BN, WM, WN, NBUF>(sa, sb, acc, lds, k_len, tid, wm, wn, lane);
+  staged_products<T, BM, BN, WM, WN, 1>(sa, sb, acc, lds, k_len, tid, wm, wn, lane);
 
   const int64_t per_slot = g.np * g.nq + (g.colsum ? g.ns : 0);
   float *out = reinterpret_cast<float *>(lds);
@@ -859,29 +970,30 @@ __global__ __launch_bounds__(64 * WM * WN, 3) void mm_weight_kernel(const Weight
     }
   }
 
+  if constexpr (SUMS == 0) return;
   if (sums) { // (uniform over the workgroup) column sums: CK threads hold each column's share
     __syncthreads();
-    auto fold = [&](auto &st, int R, int64_t first, int64_t n) {
-      using S = typename std::remove_reference<decltype(st)>::type;
+    const int part_id = SUMS == 1 ? tid : (tid + NT / 2) % NT; // (as staged_products numbers the threads of each operand)
+    constexpr int R = SUMS == 1 ? BM : BN;
+    const int64_t first = SUMS == 1 ? i0 : j0, n = SUMS == 1 ? g.np : g.nq;
+    auto &st = pick<SUMS>(sa, sb);
+    using S = typename std::remove_reference<decltype(st)>::type;
 #pragma unroll
-      for (int i = 0; i < S::N; ++i) {
-        const int idx = tid + i * NT;
-        if (idx < S::BLOCKS) {
-          const int row = (idx % (R / S::VR)) * S::VR, chunk = idx / (R / S::VR);
+    for (int i = 0; i < S::N; ++i) {
+      const int idx = part_id + i * NT;
+      if (idx < S::BLOCKS) {
+        const int row = (idx % (R / S::VR)) * S::VR, chunk = idx / (R / S::VR);
 #pragma unroll
-          for (int r = 0; r < S::VR; ++r) out[chunk * R + row + r] = st.sum[i][r];
-        }
+        for (int r = 0; r < S::VR; ++r) out[chunk * R + row + r] = st.sum[i][r];
       }
-      __syncthreads();
-      for (int c = tid; c < R && first + c < n; c += NT) {
-        float s = 0.0f;
-        for (int k = 0; k < E::BK / 8; ++k) s += out[k * R + c];
-        if (whole) static_cast<T *>(g.colsum)[piece.group * g.ns + first + c] = (T)s;
-        else g.part[slot * per_slot + g.np * g.nq + first + c] = s;
-      }
-    };
-    if (g.sum_p) fold(sa, BM, i0, g.np);
-    else fold(sb, BN, j0, g.nq);
+    }
+    __syncthreads();
+    for (int c = tid; c < R && first + c < n; c += NT) {
+      float s = 0.0f;
+      for (int k = 0; k < E::BK / 8; ++k) s += out[k * R + c];
+      if (whole) static_cast<T *>(g.colsum)[piece.group * g.ns + first + c] = (T)s;
+      else g.part[slot * per_slot + g.np * g.nq + first + c] = s;
+    }
   }
 }
 
@@ -922,23 +1034,78 @@ template <typename T> __global__ __launch_bounds__(kThreads) void mm_join_kernel
   }
 }
 
-// ---- the activation's gradient: dz = dy * act'(z) -----------------------------------------------------------------------------------
-template <typename T, int ACT> __global__ __launch_bounds__(kThreads) void act_backward_kernel(const T *dy, const T *z, T *dz, int64_t n) {
+// ---- the activation's gradient from a saved z: dz = dy * act'(z), and the column sums of dz before its rounding ------------------------
+// A workgroup takes tx vectors of columns (blockDim = tx x 256 / tx) and every gridDim.y-th set of rows.
+template <typename T, int ACT>
+__global__ __launch_bounds__(kThreads) void act_backward_kernel(const T *dy, const T *z, T *dz, float *part, int64_t rows, int64_t n) {
   constexpr int V = 16 / sizeof(T);
-  using Vec = Packed16<T>;
-  const int64_t step = (int64_t)gridDim.x * kThreads * V;
-  for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * V; i < n; i += step) {
-    if (i + V <= n) {
-      alignas(16) T a[V], b[V];
-      *reinterpret_cast<u32x4 *>(a) = *reinterpret_cast<const Vec *>(dy + i);
-      *reinterpret_cast<u32x4 *>(b) = *reinterpret_cast<const Vec *>(z + i);
+  __shared__ float fold[kThreads][V + 1];
+  const int64_t col = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * V;
+  const int cols = col + V <= n ? V : (col < n ? (int)(n - col) : 0);
+  float sum[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) a[v] = (T)(as_float(a[v]) * activation_slope<T, ACT>(as_float(b[v])));
-      *reinterpret_cast<Vec *>(dz + i) = *reinterpret_cast<const u32x4 *>(a);
-    } else {
-      for (int64_t j = i; j < n; ++j) dz[j] = (T)(as_float(dy[j]) * activation_slope<T, ACT>(as_float(z[j])));
+  for (int v = 0; v < V; ++v) sum[v] = 0.0f;
+  if (cols > 0) {
+#pragma unroll 2
+    for (int64_t row = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; row < rows; row += (int64_t)gridDim.y * blockDim.y) {
+      const int64_t at = row * n + col;
+      alignas(16) T a[V], b[V];
+      if (cols == V) {
+        *reinterpret_cast<u32x4 *>(a) = *reinterpret_cast<const Packed16<T> *>(dy + at);
+        *reinterpret_cast<u32x4 *>(b) = *reinterpret_cast<const Packed16<T> *>(z + at);
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          a[v] = v < cols ? dy[at + v] : (T)0.0f;
+          b[v] = v < cols ? z[at + v] : (T)0.0f;
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float d = as_float(a[v]) * activation_slope<T, ACT>(as_float(b[v]));
+        sum[v] += d;
+        a[v] = (T)d;
+      }
+      if (cols == V) *reinterpret_cast<Packed16<T> *>(dz + at) = *reinterpret_cast<const u32x4 *>(a);
+      else
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (v < cols) dz[at + v] = a[v];
     }
   }
+  if (!part) return;
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x;
+#pragma unroll
+  for (int v = 0; v < V; ++v) fold[tid][v] = sum[v];
+  __syncthreads();
+  if (threadIdx.y != 0) return;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float s = 0.0f;
+    for (unsigned y = 0; y < blockDim.y; ++y) s += fold[y * blockDim.x + threadIdx.x][v];
+    if (v < cols) part[(int64_t)blockIdx.y * n + col + v] = s;
+  }
+}
+
+// part [rows, n] -> out[n] (or, of gridDim.y > 1, a row of it per block row): 16 threads a column, each every 16th row of the block
+// row's share, then the 16 by halves
+template <typename T> __global__ __launch_bounds__(kThreads) void column_join_kernel(const float *part, int64_t rows, int64_t n, T *out) {
+  __shared__ float fold[kThreads];
+  const int lane = threadIdx.x % 16, way = threadIdx.x / 16;
+  const int64_t i = (int64_t)blockIdx.x * 16 + lane, share = (rows + gridDim.y - 1) / gridDim.y, first = blockIdx.y * share;
+  const int64_t last = first + share < rows ? first + share : rows;
+  float s = 0.0f;
+  if (i < n)
+#pragma unroll 8
+    for (int64_t r = first + way; r < last; r += 16) s += part[r * n + i];
+  fold[threadIdx.x] = s;
+  __syncthreads();
+#pragma unroll
+  for (int h = 128; h >= 16; h /= 2) {
+    if ((int)threadIdx.x < h) fold[threadIdx.x] += fold[threadIdx.x + h];
+    __syncthreads();
+  }
+  if (way == 0 && i < n) out[blockIdx.y * n + i] = (T)fold[lane];
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------------------
@@ -988,6 +1155,55 @@ int rows_product(RowsArgs &g, bool br, int dtype, hipStream_t st) {
   return geot_internal_fail(GEOT_EUNSUPPORTED, "matrix products take float32, float16 and bfloat16");
 }
 
+// Column sums of dz: a row of partial sums per row tile (dz from x) or per block row of the grid (dz from z), joined in two steps where
+// there are many.
+constexpr int64_t kColumnParts = 1024, kColumnJoin = 64;
+int64_t column_parts(int64_t rows) { // of either form
+  const int64_t tiles = (rows + 127) / 128;
+  return (tiles > kColumnParts ? tiles : kColumnParts) + kColumnJoin;
+}
+template <typename T, int BN> int run_preactivation(RowsArgs &g, const void *dy, float *part, hipStream_t st, int64_t &parts) {
+  const int64_t tiles_n = (g.n + BN - 1) / BN;
+  parts = (g.groups.rows + 127) / 128;
+  if (tiles_n > kMaxBlocks / 8 || parts > kMaxBlocks / tiles_n) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
+  g.tiles_n = (uint32_t)tiles_n;
+  g.slots = (uint32_t)parts;
+  g.band = 8;
+  hipLaunchKernelGGL((mm_preactivation_kernel<T, 128, BN, 2, 2>), dim3((unsigned)(parts * tiles_n)), dim3(256), 0, st, g, static_cast<const T *>(dy), part);
+  return launched("mm_preactivation_kernel");
+}
+template <typename T> int preactivation_typed(RowsArgs &g, const void *dy, const void *z, float *part, void *dbias, hipStream_t st) {
+  int64_t parts = 0;
+  if (!z) {
+    if (const int rc = g.n <= 64 ? run_preactivation<T, 64>(g, dy, part, st, parts) : run_preactivation<T, 128>(g, dy, part, st, parts)) return rc;
+  } else {
+    const int64_t vectors = (g.n * (int64_t)sizeof(T) + 15) / 16;
+    unsigned tx = 1;
+    while (tx < 256 && tx < vectors) tx *= 2;
+    const unsigned ty = 256 / tx;
+    const int64_t gx = (vectors + tx - 1) / tx, need = (g.groups.rows + ty - 1) / ty;
+    if (gx > kMaxBlocks) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
+    parts = part ? kColumnParts : 8192;
+    parts = need < parts ? need : parts;
+    by_activation(g.act, [&](auto act) {
+      hipLaunchKernelGGL((act_backward_kernel<T, decltype(act)::value>), dim3((unsigned)gx, (unsigned)parts), dim3(tx, ty), 0, st, static_cast<const T *>(dy),
+                         static_cast<const T *>(z), static_cast<T *>(g.y), part, g.groups.rows, g.n);
+    });
+    if (const int rc = launched("act_backward_kernel")) return rc;
+  }
+  if (!part) return GEOT_OK;
+  const unsigned wide = (unsigned)((g.n + 15) / 16);
+  if (parts > 8 * kColumnJoin) {
+    float *joined = part + parts * g.n;
+    hipLaunchKernelGGL((column_join_kernel<float>), dim3(wide, (unsigned)kColumnJoin), dim3(kThreads), 0, st, part, parts, g.n, joined);
+    if (const int rc = launched(nullptr)) return rc;
+    part = joined;
+    parts = kColumnJoin;
+  }
+  hipLaunchKernelGGL((column_join_kernel<T>), dim3(wide), dim3(kThreads), 0, st, part, parts, g.n, static_cast<T *>(dbias));
+  return launched(nullptr);
+}
+
 // Chunks of rows: one full round of workgroups (3 a CU, 4 of the 64 x 64 tiles), and no chunk below 256 rows.  Groups of rows take chunks
 // of a power of two (piece_of).
 struct WeightPlan {
@@ -1014,9 +1230,11 @@ WeightPlan weight_plan(int64_t rows, int64_t groups, bool with_ptr, int64_t np, 
   return w;
 }
 template <typename T, int BM, int BN, int WM, int WN> int run_weight(WeightArgs &g, int64_t slots, hipStream_t st) {
-  constexpr int NBUF = 1;
   const int64_t tiles = (int64_t)g.tiles_p * g.tiles_q;
-  hipLaunchKernelGGL((mm_weight_kernel<T, BM, BN, WM, WN, NBUF>), dim3((unsigned)(slots * tiles)), dim3(64 * WM * WN), 0, st, g);
+  const dim3 grid((unsigned)(slots * tiles)), block(64 * WM * WN);
+  if (!g.colsum) hipLaunchKernelGGL((mm_weight_kernel<T, BM, BN, WM, WN, 0>), grid, block, 0, st, g);
+  else if (g.sum_p) hipLaunchKernelGGL((mm_weight_kernel<T, BM, BN, WM, WN, 1>), grid, block, 0, st, g);
+  else hipLaunchKernelGGL((mm_weight_kernel<T, BM, BN, WM, WN, 2>), grid, block, 0, st, g);
   if (const int rc = launched("mm_weight_kernel")) return rc;
   if (g.groups.rows > g.unit) { // some group may have several chunks
     const int64_t per = (g.np * g.nq + (g.colsum ? g.ns : 0) + 15) / 16;
@@ -1099,25 +1317,34 @@ int geot_linear_grad_weight(const void *dz, const void *x, int64_t ldx, void *dw
   return weight_product(g, dtype, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
-int geot_activation_backward(const void *dy, const void *z, void *dz, int64_t n, int activation, int dtype, void *stream) {
-  if (n < 0 || (n > 0 && (!dy || !z || !dz))) return geot_internal_fail(GEOT_EINVAL, "geot_activation_backward: bad argument");
-  if (activation < GEOT_ACT_NONE || activation > GEOT_ACT_SILU) return geot_internal_fail(GEOT_EINVAL, "geot_activation_backward: unknown activation");
-  if (n == 0) return GEOT_OK;
+int geot_linear_keeps_preactivation(int64_t in, int activation, int residual, int dtype) {
+  if (activation == GEOT_ACT_NONE || (activation == GEOT_ACT_RELU && !residual)) return 0;
+  return in > (dtype == GEOT_F32 ? 128 : 256);
+}
+
+size_t geot_linear_grad_preactivation_workspace_bytes(int64_t rows, int64_t out) {
+  return bad_size(rows, out, 0) ? 0 : (size_t)column_parts(rows) * (size_t)out * sizeof(float);
+}
+
+int geot_linear_grad_preactivation(const void *dy, const void *z, const void *x, int64_t ldx, const void *weight, const void *bias, void *dz, void *dbias,
+                                   int64_t rows, int64_t in, int64_t out, int activation, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+  if (bad_size(rows, in, out) || ldx < 0) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_preactivation: negative size");
+  if (activation < GEOT_ACT_NONE || activation > GEOT_ACT_SILU) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_preactivation: unknown activation");
+  if (rows == 0 || out == 0) return GEOT_OK;
+  if (!dy || !dz || (!z && in > 0 && (!x || !weight))) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_preactivation: null pointer");
+  if (dbias && (!workspace || workspace_bytes < geot_linear_grad_preactivation_workspace_bytes(rows, out) || ((uintptr_t)workspace & 15)))
+    return geot_internal_fail(GEOT_EWORKSPACE, "geot_linear_grad_preactivation: workspace too small or misaligned");
+  RowsArgs g{};
+  g.a = x; g.lda = ldx; g.b = weight; g.ldb = in; g.bias = bias; g.y = dz; g.ldy = out;
+  g.groups = {nullptr, 1, rows}; g.n = out; g.k = in; g.act = activation;
+  float *part = dbias ? static_cast<float *>(workspace) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t vec = dtype == GEOT_F32 ? 4 : 8, want = (n + vec * kThreads - 1) / (vec * kThreads);
-  const unsigned blocks = (unsigned)(want < 8192 ? want : 8192);
-  auto run = [&](auto *t) {
-    using T = std::remove_pointer_t<decltype(t)>;
-    by_activation(activation, [&](auto act) {
-      hipLaunchKernelGGL((act_backward_kernel<T, decltype(act)::value>), dim3(blocks), dim3(kThreads), 0, st, static_cast<const T *>(dy), static_cast<const T *>(z),
-                         static_cast<T *>(dz), n);
-    });
-  };
-  if (dtype == GEOT_F32) run((float *)nullptr);
-  else if (dtype == GEOT_F16) run((f16 *)nullptr);
-  else if (dtype == GEOT_BF16) run((bf16 *)nullptr);
-  else return geot_internal_fail(GEOT_EUNSUPPORTED, "geot_activation_backward: float32, float16 and bfloat16");
-  return launched("act_backward_kernel");
+  switch (dtype) {
+  case GEOT_F32: return preactivation_typed<float>(g, dy, z, part, dbias, st);
+  case GEOT_F16: return preactivation_typed<f16>(g, dy, z, part, dbias, st);
+  case GEOT_BF16: return preactivation_typed<bf16>(g, dy, z, part, dbias, st);
+  }
+  return geot_internal_fail(GEOT_EUNSUPPORTED, "matrix products take float32, float16 and bfloat16");
 }
 
 int geot_segment_matmul(const void *x, int64_t ldx, const int64_t *ptr, const void *weight, const void *bias, void *y, int64_t rows, int64_t groups,

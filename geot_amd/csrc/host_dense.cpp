@@ -87,8 +87,8 @@ std::tuple<at::Tensor, at::Tensor> linear_forward_op(const at::Tensor &x_in, con
   const auto bias = dense(bias_in);
   const int64_t in = w.size(1), out = w.size(0);
   at::Tensor y = at::empty(with_width(x_in, out), x_in.options());
-  // what the activation's gradient needs: z, except that relu without a residual has its answer in y
-  const bool keep = save && act != GEOT_ACT_NONE && !(act == GEOT_ACT_RELU && !given(residual_in));
+  // what the activation's gradient needs: z, except that relu without a residual has its answer in y, and that narrow layers compute it again
+  const bool keep = save && geot_linear_keeps_preactivation(in, act, given(residual_in), dt);
   at::Tensor z = keep ? at::empty_like(y) : at::empty({0}, x_in.options());
   Rows r{at::Tensor(), 0, 0};
   if (given(residual_in)) r = as_rows(*residual_in);
@@ -101,36 +101,42 @@ std::tuple<at::Tensor, at::Tensor> linear_train_op(const at::Tensor &x, const at
   return linear_forward_op(x, w, bias, residual, activation, true);
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward_op(const at::Tensor &grad_in, const at::Tensor &x_in, const at::Tensor &w_in, const at::Tensor &z_in,
-                                                                  c10::string_view activation, bool need_x, bool need_w, bool need_b) {
-  check_linear(x_in, w_in, c10::nullopt, grad_in);
+// z: what the forward kept ([0]: nothing - no activation, or one whose z is computed again)
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward_op(const at::Tensor &grad_in, const at::Tensor &x_in, const at::Tensor &w_in,
+                                                                  const c10::optional<at::Tensor> &bias_in, const at::Tensor &z_in, c10::string_view activation,
+                                                                  bool need_x, bool need_w, bool need_b) {
+  check_linear(x_in, w_in, bias_in, grad_in);
   const int act = activation_code(activation);
-  TORCH_CHECK(act == GEOT_ACT_NONE || (z_in.sizes() == grad_in.sizes() && z_in.scalar_type() == grad_in.scalar_type()),
-              "linear: the backward pass of '", activation, "' needs what the differentiable forward (geot_dense::linear_train) saved");
-  require_gpu("linear", {&grad_in, &x_in, &w_in, &z_in});
+  const bool has_z = z_in.sizes() == grad_in.sizes() && z_in.numel() > 0;
+  TORCH_CHECK(!has_z || z_in.scalar_type() == grad_in.scalar_type(), "linear: the backward pass needs what the differentiable forward (geot_dense::linear_train) saved");
+  require_gpu("linear", {&grad_in, &x_in, &w_in, ptr_of(bias_in), &z_in});
   const int dt = dense_dtype(x_in, "linear");
   GEOT_DEVICE_GUARD(x_in);
   void *st = stream_of(x_in);
   const Rows x = as_rows(x_in);
   const at::Tensor w = w_in.contiguous();
   const int64_t in = w.size(1), out = w.size(0);
-  at::Tensor dz = grad_in.contiguous();
+  at::Tensor dz = grad_in.contiguous(), dx, dw, db;
   if (act != GEOT_ACT_NONE) {
-    const at::Tensor z = z_in.contiguous(), dy = dz;
+    const at::Tensor dy = dz, z = has_z ? z_in.contiguous() : at::Tensor();
+    const auto bias = dense(bias_in);
     dz = at::empty_like(dy);
-    GEOT_CALL(geot_activation_backward(dy.data_ptr(), z.data_ptr(), dz.data_ptr(), dz.numel(), act, dt, st));
+    if (need_b) db = x.rows > 0 ? at::empty({out}, w.options()) : at::zeros({out}, w.options());
+    const at::Tensor ws = scratch(x_in, need_b ? geot_linear_grad_preactivation_workspace_bytes(x.rows, out) : 0);
+    GEOT_CALL(geot_linear_grad_preactivation(dy.data_ptr(), has_z ? z.data_ptr() : nullptr, x.t.data_ptr(), x.ld, w.data_ptr(), data_of(bias), dz.data_ptr(),
+                                             need_b ? db.data_ptr() : nullptr, x.rows, in, out, act, dt, ws.data_ptr(), ws.numel(), st));
   }
-  at::Tensor dx, dw, db;
   if (need_x) {
     dx = at::empty(x_in.sizes(), x_in.options());
     GEOT_CALL(geot_linear_grad_input(dz.data_ptr(), w.data_ptr(), dx.data_ptr(), x.rows, in, out, dt, st));
   }
-  if (need_w || need_b) {
+  const bool sums = need_b && act == GEOT_ACT_NONE;
+  if (need_w || sums) {
     const int64_t cols = need_w ? in : 0; // (the bias's gradient alone: column sums beside a product of width 0)
-    dw = need_w ? at::empty_like(w) : at::Tensor();
-    db = need_b ? at::empty({out}, w.options()) : at::Tensor();
+    if (need_w) dw = at::empty_like(w);
+    if (sums) db = at::empty({out}, w.options());
     const at::Tensor ws = scratch(x_in, geot_linear_grad_weight_workspace_bytes(x.rows, cols, out));
-    GEOT_CALL(geot_linear_grad_weight(dz.data_ptr(), x.t.data_ptr(), x.ld, need_w ? dw.data_ptr() : nullptr, need_b ? db.data_ptr() : nullptr, x.rows, cols, out, dt,
+    GEOT_CALL(geot_linear_grad_weight(dz.data_ptr(), x.t.data_ptr(), x.ld, need_w ? dw.data_ptr() : nullptr, sums ? db.data_ptr() : nullptr, x.rows, cols, out, dt,
                                       ws.data_ptr(), ws.numel(), st));
   }
   const at::Tensor none = at::empty({0}, x_in.options());
@@ -279,7 +285,7 @@ TORCH_LIBRARY_FRAGMENT(geot_dense, m) {
   m.def("linear(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, str activation) -> Tensor", linear_op);
   m.def("linear_forward(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, str activation, bool save) -> (Tensor, Tensor)");
   m.def("linear_train(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, str activation) -> (Tensor, Tensor)");
-  m.def("linear_backward(Tensor grad, Tensor x, Tensor weight, Tensor z, str activation, bool need_x, bool need_weight, bool need_bias) -> (Tensor, Tensor, Tensor)");
+  m.def("linear_backward(Tensor grad, Tensor x, Tensor weight, Tensor? bias, Tensor z, str activation, bool need_x, bool need_weight, bool need_bias) -> (Tensor, Tensor, Tensor)");
   m.def("segment_matmul(Tensor x, Tensor ptr, Tensor weight, Tensor? bias) -> Tensor", segment_matmul_op);
   m.def("segment_matmul_forward(Tensor x, Tensor ptr, Tensor weight, Tensor? bias) -> Tensor");
   m.def("segment_matmul_train(Tensor x, Tensor ptr, Tensor weight, Tensor? bias) -> Tensor");

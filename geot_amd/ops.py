@@ -441,9 +441,14 @@ torch.library.register_autograd("geot::index_scatter", _is_backward, setup_conte
 # --------------------------------------------------------------------------------------------------
 # dense rows (csrc/host_dense.cpp): fake-tensor rules and autograd formulas of the differentiable forms
 # --------------------------------------------------------------------------------------------------
+_ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+_FLOATS = {torch.float32: _lib.GEOT_F32, torch.float16: _lib.GEOT_F16, torch.bfloat16: _lib.GEOT_BF16}
+
+
 def _fake_linear(x, weight, bias, residual, activation, save=True):
     y = x.new_empty([*x.shape[:-1], weight.shape[0]])
-    keep = save and activation != "none" and not (activation == "relu" and residual is None)
+    keep = save and _lib.load().geot_linear_keeps_preactivation(int(weight.shape[1]), _ACTIVATIONS.get(activation, 0), int(residual is not None),
+                                                                _FLOATS.get(x.dtype, 0))
     return y, (torch.empty_like(y) if keep else x.new_empty([0]))
 
 
@@ -456,7 +461,7 @@ def _(x, weight, bias, residual, activation):
 
 
 @torch.library.register_fake("geot_dense::linear_backward")
-def _(grad, x, weight, z, activation, need_x, need_weight, need_bias):
+def _(grad, x, weight, bias, z, activation, need_x, need_weight, need_bias):
     return (x.new_empty(x.shape if need_x else [0]), weight.new_empty(weight.shape if need_weight else [0]),
             weight.new_empty([weight.shape[0] if need_bias else 0]))
 
@@ -510,7 +515,7 @@ def _linear_setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
     ctx.mark_non_differentiable(z)
     # relu without a residual: y has z's sign, nothing else is kept
-    ctx.save_for_backward(x, weight, y if activation == "relu" and residual is None else z)
+    ctx.save_for_backward(x, weight, bias, y if activation == "relu" and residual is None else z)
 
 
 def _linear_backward(ctx, grad, _grad_z):
@@ -518,11 +523,11 @@ def _linear_backward(ctx, grad, _grad_z):
     if grad is None:
         return None, None, None, None, None
     _once("linear")
-    x, weight, z = ctx.saved_tensors
+    x, weight, bias, z = ctx.saved_tensors
     need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
     dx = dw = db = None
     if need_x or need_w or need_b:
-        dx, dw, db = torch.ops.geot_dense.linear_backward(grad, x, weight, z, ctx.activation, need_x, need_w, need_b)
+        dx, dw, db = torch.ops.geot_dense.linear_backward(grad, x, weight, bias, z, ctx.activation, need_x, need_w, need_b)
     return dx if need_x else None, dw if need_w else None, db if need_b else None, grad if need_r else None, None
 
 
@@ -674,8 +679,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     residual [..., out]; ``activation``: 'none', 'relu', 'gelu' (the error-function form) or 'silu'.
 
     float32, float16 or bfloat16, one dtype for all operands; sums in float32, one rounding.  Differentiable in every tensor (the
-    backward pass itself is not).  A training call keeps the pre-activation in the operands' dtype ('none', and 'relu' without a
-    residual, keep nothing)."""
+    backward pass itself is not).  A training call of a wide layer keeps the pre-activation in the operands' dtype; a narrow one (in <= 256,
+    float32 128) computes it again in the backward pass, and 'none', and 'relu' without a residual, do not need it."""
     return torch.ops.geot_dense.linear(x, weight, bias, residual, activation)
 
 

@@ -392,8 +392,15 @@ int geot_slab_mh_sddmm(const geot_slab_plan *plan, const void *mat_1, const void
 enum { GEOT_ACT_NONE = 0, GEOT_ACT_RELU = 1, GEOT_ACT_GELU = 2 /* z * Phi(z), the error-function form */, GEOT_ACT_SILU = 3 };
 int geot_linear(const void *x, int64_t ldx, const void *weight, const void *bias, const void *residual, int64_t ld_residual, void *z,
                 void *y, int64_t rows, int64_t in, int64_t out, int activation, int dtype, void *stream);
-/* dz[i] = dy[i] * act'(z[i]); dz may be dy.  For relu z may be y (they have one sign). */
-int geot_activation_backward(const void *dy, const void *z, void *dz, int64_t n, int activation, int dtype, void *stream);
+/* dz = dy act'(z) [rows, out], and the bias's gradient dbias = column sums of dz (before its rounding) [out] or NULL.  z: what geot_linear
+ * wrote, or y for relu without a residual (they have one sign), or NULL: computed again from x, weight and bias - what
+ * geot_linear_keeps_preactivation says (0: do not keep z) for layers where that moves fewer bytes.  dz may be dy when z is given.
+ * workspace (with dbias): 16-byte aligned, no content expected, free after the call. */
+int geot_linear_keeps_preactivation(int64_t in, int activation, int residual, int dtype);
+size_t geot_linear_grad_preactivation_workspace_bytes(int64_t rows, int64_t out);
+int geot_linear_grad_preactivation(const void *dy, const void *z, const void *x, int64_t ldx, const void *weight, const void *bias, void *dz,
+                                   void *dbias, int64_t rows, int64_t in, int64_t out, int activation, int dtype, void *workspace,
+                                   size_t workspace_bytes, void *stream);
 /* dx = dz weight   [rows, in] */
 int geot_linear_grad_input(const void *dz, const void *weight, void *dx, int64_t rows, int64_t in, int64_t out, int dtype, void *stream);
 /* dweight = dz^T x [out, in]; dbias = column sums of dz [out] or NULL.  The rows are split over workgroups and the parts joined in a

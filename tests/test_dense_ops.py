@@ -4,7 +4,8 @@ Tolerances are bounds, element by element, with u = half a step of the dtype (re
 sum of n products is off by at most n steps of 2^-23 of the sum of their absolute values (a matrix instruction may truncate where it
 adds: a whole step); a float32 product of split operands is six such products plus at most 2^-23 of |ab| left out.  The gradient of an
 activation is taken at z rounded to the dtype: |act''| <= 0.8 (gelu) or 0.5 (silu) times that rounding; relu's may be 0 or 1 where |z| is
-below the sum's own error.
+below the sum's own error.  gelu and its slope are polynomials: for 16-bit results 2^-15 of the value and 2^-15 absolute (what their fits
+leave), for float32 below 2^-20 like the other activations.
 """
 import math
 
@@ -66,7 +67,8 @@ class LinearReference:
             z, size = z + b.double(), size + b.double().abs()
         e_z = terms(k, dt) * size
         f, slope = act64(z, act)
-        self.y, self.e_y = f, 1.2 * e_z + 2.0 ** -20 * f.abs()
+        fit = 2.0 ** -15 if act == "gelu" and dt != torch.float32 else 0.0
+        self.y, self.e_y = f, 1.2 * e_z + (2.0 ** -20 + fit) * f.abs()
         if r is not None:
             r = r.double().reshape(m, n)
             self.y, self.e_y = f + r, self.e_y + STEP * (f.abs() + r.abs())
@@ -77,7 +79,7 @@ class LinearReference:
         dz = dy * slope
         e_dz = torch.zeros_like(dz)
         if act != "none":
-            e_slope = CURVATURE[act] * (e_z + u * z.abs() + tiny) + 2.0 ** -20 * (slope.abs() + z.abs() / 2)
+            e_slope = CURVATURE[act] * (e_z + u * z.abs() + tiny) + 2.0 ** -20 * (slope.abs() + z.abs() / 2) + fit
             if act == "relu":
                 e_slope = (z.abs() <= e_z + tiny).double()
             e_dz = dy.abs() * e_slope + u * dz.abs() + tiny
@@ -169,8 +171,11 @@ def test_fake_shapes():
         x = torch.empty(3, 4, 8, dtype=torch.bfloat16, device="cuda")
         w = torch.empty(6, 8, dtype=torch.bfloat16, device="cuda")
         assert geot.linear(x, w, activation="gelu").shape == (3, 4, 6)
-        y, z = torch.ops.geot_dense.linear_train(x, w, None, None, "gelu")
-        assert z.shape == y.shape and torch.ops.geot_dense.linear_train(x, w, None, None, "relu")[1].numel() == 0
+        # a narrow layer's pre-activation is computed again, a wide one's is kept (unless y has its sign)
+        assert torch.ops.geot_dense.linear_train(x, w, None, None, "gelu")[1].numel() == 0
+        xw, ww = torch.empty(3, 4, 300, dtype=torch.bfloat16, device="cuda"), torch.empty(6, 300, dtype=torch.bfloat16, device="cuda")
+        y, z = torch.ops.geot_dense.linear_train(xw, ww, None, None, "gelu")
+        assert z.shape == y.shape and torch.ops.geot_dense.linear_train(xw, ww, None, None, "relu")[1].numel() == 0
         assert geot.layer_norm(x, w[0].float()).shape == x.shape
         assert torch.ops.geot_dense.layer_norm_train(x, w[0].float(), None, 1e-5)[1].shape == (3, 12)
         assert geot.segment_matmul(x[0], torch.empty(3, dtype=torch.int64, device="cuda"), torch.empty(2, 8, 5, dtype=torch.bfloat16, device="cuda")).shape == (4, 5)
