@@ -278,12 +278,12 @@ def load() -> ctypes.CDLL:
     L.geot_linear_grad_preactivation.argtypes = [c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_int, c_vp, c_sz, c_vp]
     L.geot_linear_grad_input.argtypes = [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_vp]
     L.geot_linear_grad_weight_workspace_bytes.restype = c_sz
-    L.geot_linear_grad_weight_workspace_bytes.argtypes = [c_i64, c_i64, c_i64]
+    L.geot_linear_grad_weight_workspace_bytes.argtypes = [c_i64, c_i64, c_i64, c_int]
     L.geot_linear_grad_weight.argtypes = [c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_vp, c_sz, c_vp]
     L.geot_segment_matmul.argtypes = [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp]
     L.geot_segment_matmul_grad_input.argtypes = [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp]
     L.geot_segment_matmul_grad_weight_workspace_bytes.restype = c_sz
-    L.geot_segment_matmul_grad_weight_workspace_bytes.argtypes = [c_i64, c_i64, c_i64, c_i64]
+    L.geot_segment_matmul_grad_weight_workspace_bytes.argtypes = [c_i64, c_i64, c_i64, c_i64, c_int]
     L.geot_segment_matmul_grad_weight.argtypes = [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_sz, c_vp]
     L.geot_layer_norm.argtypes = [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_f, c_int, c_int, c_vp]
     L.geot_layer_norm_backward_workspace_bytes.restype = c_sz

@@ -289,15 +289,25 @@ template <typename T, int BM, int BN, int WM, int WN> struct Accum {
         for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
   }
   __device__ void products(const typename E::Frag (&a)[E::PARTS][FM], const typename E::Frag (&b)[E::PARTS][FN]) {
-    // the smallest partial products first
-    constexpr int NP = E::PARTS == 1 ? 1 : 6;
-    constexpr int PA[6] = {E::PARTS == 1 ? 0 : 2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
 #pragma unroll
-    for (int p = 0; p < NP; ++p)
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+      for (int j = 0; j < FN; ++j) {
+        if constexpr (E::PARTS == 1) {
+          acc[i][j] = E::mfma(a[0][i], b[0][j], acc[i][j]);
+        } else {
+          // the six partial products of 16 reduction values, smallest first, in a sum of their own: the long sum then rounds once for them
+          // (added to it one by one, K = 4048 came out 1.0e-6 off where a float32 product is 0.6e-6)
+          constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
+          f32x16 t;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = E::mfma(a[PA[p]][i], b[PB[p]][j], acc[i][j]);
+          for (int e = 0; e < 16; ++e) t[e] = 0.0f;
+#pragma unroll
+          for (int p = 0; p < 6; ++p) t = E::mfma(a[PA[p]][i], b[PB[p]][j], t);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][j][e] += t[e];
+        }
+      }
   }
   __device__ void step(const char *la, const char *lb, int wm, int wn, int lane) {
     using F = typename E::Frag;
@@ -1138,12 +1148,13 @@ template <typename T, bool BR> int rows_typed(RowsArgs &g, hipStream_t st) {
   if constexpr (!BR) {
     if (!g.groups.ptr && tiles < 128 && g.k >= 128) return g.groups.rows <= 32 ? run_few<T, 1>(g, st) : run_few<T, 2>(g, st);
   }
-  if (g.n <= 64) return run_rows<T, 128, 64, 2, 2, BR, 1>(g, st);
+  // (split operands: two column fragments a wave and their six parts do not fit the registers of three workgroups a CU)
+  if (Elem<T>::PARTS == 3 || g.n <= 64) return run_rows<T, 128, 64, 2, 2, BR, 1>(g, st);
   if constexpr (Elem<T>::PARTS == 1) {
     const int64_t per_group = g.groups.ptr ? g.groups.rows / (g.groups.groups > 0 ? g.groups.groups : 1) : g.groups.rows;
     if (g.n > 128 && g.k >= 512 && tiles >= 1024 && per_group >= 2048) return run_rows<T, 256, 256, 2, 4, BR, 2>(g, st);
+    return run_rows<T, 128, 128, 2, 2, BR, 1>(g, st);
   }
-  return run_rows<T, 128, 128, 2, 2, BR, 1>(g, st);
 }
 int rows_product(RowsArgs &g, bool br, int dtype, hipStream_t st) {
   if (g.groups.rows == 0 || g.n == 0) return GEOT_OK;
@@ -1175,7 +1186,10 @@ template <typename T, int BN> int run_preactivation(RowsArgs &g, const void *dy,
 template <typename T> int preactivation_typed(RowsArgs &g, const void *dy, const void *z, float *part, void *dbias, hipStream_t st) {
   int64_t parts = 0;
   if (!z) {
-    if (const int rc = g.n <= 64 ? run_preactivation<T, 64>(g, dy, part, st, parts) : run_preactivation<T, 128>(g, dy, part, st, parts)) return rc;
+    int rc;
+    if constexpr (Elem<T>::PARTS == 3) rc = run_preactivation<T, 64>(g, dy, part, st, parts);
+    else rc = g.n <= 64 ? run_preactivation<T, 64>(g, dy, part, st, parts) : run_preactivation<T, 128>(g, dy, part, st, parts);
+    if (rc) return rc;
   } else {
     const int64_t vectors = (g.n * (int64_t)sizeof(T) + 15) / 16;
     unsigned tx = 1;
@@ -1210,9 +1224,9 @@ struct WeightPlan {
   int64_t tiles_p, tiles_q, unit, slots;
   int unit_log2;
 };
-WeightPlan weight_plan(int64_t rows, int64_t groups, bool with_ptr, int64_t np, int64_t nq) {
+WeightPlan weight_plan(int64_t rows, int64_t groups, bool with_ptr, int64_t np, int64_t nq, int dtype) {
   WeightPlan w;
-  const int64_t bm = np <= 64 ? 64 : 128, bn = nq <= 64 ? 64 : 128;
+  const int64_t bm = np <= 64 ? 64 : 128, bn = nq <= 64 || dtype == GEOT_F32 ? 64 : 128;
   w.tiles_p = np > 0 ? (np + bm - 1) / bm : 1; // (a side of width 0 still has its column sums)
   w.tiles_q = nq > 0 ? (nq + bn - 1) / bn : 1;
   const int64_t tiles = w.tiles_p * w.tiles_q;
@@ -1248,12 +1262,14 @@ template <typename T, int BM, int BN, int WM, int WN> int run_weight(WeightArgs 
   return GEOT_OK;
 }
 template <typename T> int weight_typed(WeightArgs &g, int64_t slots, hipStream_t st) {
-  if (g.np <= 64) return g.nq <= 64 ? run_weight<T, 64, 64, 2, 2>(g, slots, st) : run_weight<T, 64, 128, 2, 2>(g, slots, st);
-  return g.nq <= 64 ? run_weight<T, 128, 64, 2, 2>(g, slots, st) : run_weight<T, 128, 128, 2, 2>(g, slots, st);
+  if constexpr (Elem<T>::PARTS == 1) {
+    if (g.nq > 64) return g.np <= 64 ? run_weight<T, 64, 128, 2, 2>(g, slots, st) : run_weight<T, 128, 128, 2, 2>(g, slots, st);
+  }
+  return g.np <= 64 ? run_weight<T, 64, 64, 2, 2>(g, slots, st) : run_weight<T, 128, 64, 2, 2>(g, slots, st);
 }
 int weight_product(WeightArgs &g, int dtype, void *workspace, size_t workspace_bytes, hipStream_t st) {
   if (g.groups.groups == 0 || (g.np * g.nq == 0 && !(g.colsum && g.ns > 0))) return GEOT_OK;
-  const WeightPlan w = weight_plan(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, g.np, g.nq);
+  const WeightPlan w = weight_plan(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, g.np, g.nq, dtype);
   if (w.tiles_p * w.tiles_q > kMaxBlocks / w.slots) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
   g.unit = w.unit;
   g.unit_log2 = w.unit_log2;
@@ -1301,9 +1317,9 @@ int geot_linear_grad_input(const void *dz, const void *weight, void *dx, int64_t
   return rows_product(g, true, dtype, static_cast<hipStream_t>(stream));
 }
 
-size_t geot_linear_grad_weight_workspace_bytes(int64_t rows, int64_t in, int64_t out) {
+size_t geot_linear_grad_weight_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype) {
   if (bad_size(rows, in, out)) return 0;
-  const WeightPlan w = weight_plan(rows, 1, false, out, in);
+  const WeightPlan w = weight_plan(rows, 1, false, out, in, dtype);
   return rows > w.unit ? (size_t)w.slots * (size_t)(in * out + out) * sizeof(float) : 0;
 }
 
@@ -1367,9 +1383,9 @@ int geot_segment_matmul_grad_input(const void *dy, const int64_t *ptr, const voi
   return rows_product(g, false, dtype, static_cast<hipStream_t>(stream));
 }
 
-size_t geot_segment_matmul_grad_weight_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out) {
+size_t geot_segment_matmul_grad_weight_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype) {
   if (bad_size(rows, in, out) || groups < 0 || groups > 65535) return 0;
-  const WeightPlan w = weight_plan(rows, groups, true, in, out);
+  const WeightPlan w = weight_plan(rows, groups, true, in, out, dtype);
   return rows > w.unit ? (size_t)w.slots * (size_t)(in * out + out) * sizeof(float) : 0;
 }
 

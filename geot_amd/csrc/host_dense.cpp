@@ -4,13 +4,17 @@
 // dispatcher namespace of their own, so that `geot` holds what the reference's layers define and expect there.  Each comes as
 //   geot_dense::<op>            what a user calls: looks whether a gradient is asked for and goes to one of
 //   geot_dense::<op>_forward    the kernel, nothing kept for a backward pass (inference stays out of Python altogether)
-//   geot_dense::<op>_train      the differentiable form; its fake-tensor rule and autograd formula are in geot_amd/ops.py, over
+//   geot_dense::<op>_train      the differentiable form (autograd formulas below; fake-tensor rules in geot_amd/ops.py), over
 //   geot_dense::<op>_backward   the gradients
+// The formulas are C++ here, unlike the aggregations' in ops.py: a training step of a few rows is host time, and a Python formula was 60 us
+// of its 90.
 // Every call runs on its tensors' device and that device's current stream, allocates what it needs from torch's caching allocator (under
 // capture: from the graph's own pool, so two captured graphs share no scratch) and neither synchronises nor remembers anything.
 #include "host.h"
 
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/GradMode.h>
+#include <torch/csrc/autograd/custom_function.h>
 
 namespace {
 using namespace geot_host;
@@ -135,7 +139,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward_op(const at::Tens
     const int64_t cols = need_w ? in : 0; // (the bias's gradient alone: column sums beside a product of width 0)
     if (need_w) dw = at::empty_like(w);
     if (sums) db = at::empty({out}, w.options());
-    const at::Tensor ws = scratch(x_in, geot_linear_grad_weight_workspace_bytes(x.rows, cols, out));
+    const at::Tensor ws = scratch(x_in, geot_linear_grad_weight_workspace_bytes(x.rows, cols, out, dt));
     GEOT_CALL(geot_linear_grad_weight(dz.data_ptr(), x.t.data_ptr(), x.ld, need_w ? dw.data_ptr() : nullptr, sums ? db.data_ptr() : nullptr, x.rows, cols, out, dt,
                                       ws.data_ptr(), ws.numel(), st));
   }
@@ -203,7 +207,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> segment_matmul_backward_op(const 
     const int64_t rows_p = need_w ? in : 0;
     dw = need_w ? at::empty_like(w) : at::Tensor();
     db = need_b ? at::empty({groups, out}, w.options()) : at::Tensor();
-    const at::Tensor ws = scratch(x_in, geot_segment_matmul_grad_weight_workspace_bytes(x.rows, groups, rows_p, out));
+    const at::Tensor ws = scratch(x_in, geot_segment_matmul_grad_weight_workspace_bytes(x.rows, groups, rows_p, out, dt));
     GEOT_CALL(geot_segment_matmul_grad_weight(x.t.data_ptr(), x.ld, index_ptr(ptr), dy.data_ptr(), need_w ? dw.data_ptr() : nullptr, need_b ? db.data_ptr() : nullptr,
                                               x.rows, groups, rows_p, out, dt, ws.data_ptr(), ws.numel(), st));
   }
@@ -279,6 +283,121 @@ at::Tensor layer_norm_op(const at::Tensor &x, const c10::optional<at::Tensor> &w
   return std::get<0>(fwd.call(x, w, b, eps, false));
 }
 
+// ---- autograd ------------------------------------------------------------------------------------------------------------------------
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+at::Tensor or_undefined(const c10::optional<at::Tensor> &t) { return given(t) ? *t : at::Tensor(); }
+c10::optional<at::Tensor> or_none(const at::Tensor &t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; }
+at::Tensor if_needed(bool need, const at::Tensor &t) { return need ? t : at::Tensor(); }
+// these backward passes have no gradient of their own; a caller that asks for one (create_graph) is told so
+void first_order_only(const char *op) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!c10::GradMode::is_enabled(), op, ": the backward pass is not differentiable (create_graph=True is not supported)");
+}
+
+// y = act(z) + residual, z = x W^T + b:  dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = column sums of dz;  dresidual = dy
+struct LinearFunction : torch::autograd::Function<LinearFunction> {
+  static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &w, const c10::optional<at::Tensor> &bias, const c10::optional<at::Tensor> &residual,
+                               std::string act) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::linear_train", "").typed<decltype(linear_train_op)>();
+    auto [y, z] = op.call(x, w, bias, residual, act);
+    // relu without a residual: y has z's sign, nothing else is kept
+    ctx->save_for_backward({x, w, or_undefined(bias), act == "relu" && !given(residual) ? y : z});
+    ctx->saved_data["bias"] = given(bias);
+    ctx->saved_data["residual"] = given(residual);
+    ctx->saved_data["activation"] = act;
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({z});
+    return {y, z};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    variable_list out(5);
+    const at::Tensor &dy = grads[0];
+    if (!dy.defined()) return out;
+    first_order_only("linear");
+    const auto saved = ctx->get_saved_variables();
+    size_t at = 2; // (inputs that were not given are not counted)
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
+    const bool nb = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(at++), nr = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(at);
+    if (nx || nw || nb) {
+      static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::linear_backward", "").typed<decltype(linear_backward_op)>();
+      const std::string act = ctx->saved_data["activation"].toStringRef();
+      auto [dx, dw, db] = op.call(dy, saved[0], saved[1], or_none(saved[2]), saved[3], act, nx, nw, nb);
+      out[0] = if_needed(nx, dx);
+      out[1] = if_needed(nw, dw);
+      out[2] = if_needed(nb, db);
+    }
+    out[3] = if_needed(nr, dy);
+    return out;
+  }
+};
+std::tuple<at::Tensor, at::Tensor> linear_train_autograd(const at::Tensor &x, const at::Tensor &w, const c10::optional<at::Tensor> &bias,
+                                                         const c10::optional<at::Tensor> &residual, c10::string_view activation) {
+  auto r = LinearFunction::apply(x, w, bias, residual, std::string(activation));
+  return std::make_tuple(r[0], r[1]);
+}
+
+// per group g:  dx = dy W[g]^T;  dW[g] = x_g^T dy_g;  db[g] = column sums of dy_g
+struct SegmentMatmulFunction : torch::autograd::Function<SegmentMatmulFunction> {
+  static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &ptr, const at::Tensor &w, const c10::optional<at::Tensor> &bias) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::segment_matmul_train", "").typed<decltype(segment_matmul_forward_op)>();
+    ctx->save_for_backward({x, ptr, w});
+    ctx->saved_data["bias"] = given(bias);
+    ctx->set_materialize_grads(false);
+    return op.call(x, ptr, w, bias);
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    variable_list out(4);
+    if (!grads[0].defined()) return out;
+    first_order_only("segment_matmul");
+    const auto saved = ctx->get_saved_variables();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(2);
+    const bool nb = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(3);
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::segment_matmul_backward", "").typed<decltype(segment_matmul_backward_op)>();
+    auto [dx, dw, db] = op.call(grads[0], saved[0], saved[1], saved[2], nx, nw, nb);
+    out[0] = if_needed(nx, dx);
+    out[2] = if_needed(nw, dw);
+    out[3] = if_needed(nb, db);
+    return out;
+  }
+};
+at::Tensor segment_matmul_train_autograd(const at::Tensor &x, const at::Tensor &ptr, const at::Tensor &w, const c10::optional<at::Tensor> &bias) {
+  return SegmentMatmulFunction::apply(x, ptr, w, bias);
+}
+
+// h = (x - mean) rstd, g = dy w:  dx = rstd (g - mean g - h mean(g h));  dw = sum over rows of dy h;  db = sum over rows of dy
+struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
+  static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const c10::optional<at::Tensor> &w, const c10::optional<at::Tensor> &b, double eps) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::layer_norm_train", "").typed<decltype(layer_norm_train_op)>();
+    auto [y, stats] = op.call(x, w, b, eps);
+    ctx->save_for_backward({x, or_undefined(w), or_undefined(b), stats});
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({stats});
+    return {y, stats};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    variable_list out(4);
+    if (!grads[0].defined()) return out;
+    first_order_only("layer_norm");
+    const auto saved = ctx->get_saved_variables();
+    size_t at = 1; // (inputs that were not given are not counted)
+    const bool nx = ctx->needs_input_grad(0), nw = saved[1].defined() && ctx->needs_input_grad(at++), nb = saved[2].defined() && ctx->needs_input_grad(at);
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::layer_norm_backward", "").typed<decltype(layer_norm_backward_op)>();
+    auto [dx, dw, db] = op.call(grads[0], saved[0], or_none(saved[1]), or_none(saved[2]), saved[3], nw || nb);
+    out[0] = if_needed(nx, dx);
+    out[1] = if_needed(nw, dw);
+    out[2] = if_needed(nb, db);
+    return out;
+  }
+};
+std::tuple<at::Tensor, at::Tensor> layer_norm_train_autograd(const at::Tensor &x, const c10::optional<at::Tensor> &w, const c10::optional<at::Tensor> &b, double eps) {
+  auto r = LayerNormFunction::apply(x, w, b, eps);
+  return std::make_tuple(r[0], r[1]);
+}
+
 } // namespace
 
 TORCH_LIBRARY_FRAGMENT(geot_dense, m) {
@@ -309,3 +428,8 @@ TORCH_LIBRARY_FRAGMENT(geot_dense, m) {
   m.impl("layer_norm_backward", layer_norm_backward_op)
 TORCH_LIBRARY_IMPL(geot_dense, CUDA, m) { GEOT_DENSE_IMPLS(m); }
 TORCH_LIBRARY_IMPL(geot_dense, CPU, m) { GEOT_DENSE_IMPLS(m); }
+TORCH_LIBRARY_IMPL(geot_dense, Autograd, m) {
+  m.impl("linear_train", linear_train_autograd);
+  m.impl("segment_matmul_train", segment_matmul_train_autograd);
+  m.impl("layer_norm_train", layer_norm_train_autograd);
+}

@@ -153,6 +153,68 @@ def rewrite_graph(gm: fx.GraphModule, sort_edges: bool = False) -> int:
     return fused
 
 
+_ACTIVATIONS = {aten.relu.default: "relu", aten.silu.default: "silu", aten.gelu.default: "gelu"}
+_DENSE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _single_user(node) -> Optional[fx.Node]:
+    users = list(node.users)
+    return users[0] if len(users) == 1 else None
+
+
+def _dense_operands(*nodes) -> bool:
+    """All of one dtype the dense operators take."""
+    vals = [n.meta.get("val") for n in nodes if n is not None]
+    return all(v is not None and v.dtype in _DENSE_DTYPES and v.dtype == vals[0].dtype for v in vals)
+
+
+def rewrite_dense(gm: fx.GraphModule) -> int:
+    """Rewrite ``aten.linear`` - with the relu / silu / gelu (error-function form) and the addition of a tensor of the result's shape that
+    alone consume it - into ``geot_dense::linear``, and ``aten.layer_norm`` over the last dimension into ``geot_dense::layer_norm``, in
+    place; returns the number of rewritten products and normalisations.  Other dtypes, broadcast additions and shared intermediates keep
+    their aten form."""
+    graph = gm.graph
+    done = 0
+    for node in list(graph.nodes):
+        if _is(node, aten.linear.default):
+            x, w = node.args[:2]
+            b = node.args[2] if len(node.args) > 2 else None
+            if not _dense_operands(x, w, b) or len(_shape(w)) != 2:
+                continue
+            last, act, residual = node, "none", None
+            nxt = _single_user(last)
+            if nxt is not None and nxt.op == "call_function" and nxt.target in _ACTIVATIONS and \
+                    nxt.kwargs.get("approximate", "none") == "none" and len(nxt.args) == 1:
+                last, act = nxt, _ACTIVATIONS[nxt.target]
+                nxt = _single_user(last)
+            if nxt is not None and _is(nxt, aten.add.Tensor) and nxt.kwargs.get("alpha", 1) == 1:
+                other = nxt.args[1] if nxt.args[0] is last else nxt.args[0]
+                if isinstance(other, fx.Node) and other is not last and _shape(other) == _shape(last) and _dense_operands(x, other):
+                    last, residual = nxt, other
+            with graph.inserting_before(last):         # (every operand, the residual among them, is defined in front of `last`)
+                new = graph.call_function(torch.ops.geot_dense.linear.default, (x, w, b, residual, act))
+        elif _is(node, aten.layer_norm.default):
+            x, shape = node.args[:2]
+            w = node.args[2] if len(node.args) > 2 else node.kwargs.get("weight")
+            b = node.args[3] if len(node.args) > 3 else node.kwargs.get("bias")
+            eps = node.args[4] if len(node.args) > 4 else node.kwargs.get("eps", 1e-5)
+            if len(shape) != 1 or not _dense_operands(x, w, b):
+                continue
+            last = node
+            with graph.inserting_before(node):
+                new = graph.call_function(torch.ops.geot_dense.layer_norm.default, (x, w, b, eps))
+        else:
+            continue
+        new.meta["val"] = last.meta.get("val")
+        last.replace_all_uses_with(new)
+        done += 1
+    if done:
+        graph.eliminate_dead_code()
+        graph.lint()
+        gm.recompile()
+    return done
+
+
 def _placeholder_values(exported: ExportedProgram, args) -> dict:
     """placeholder name -> concrete tensor, for the exported graph's lifted parameters / buffers / constants and the user's inputs."""
     import torch.utils._pytree as pytree
@@ -238,12 +300,15 @@ def bind_static_graphs(exported: ExportedProgram, args, slab_mode: str = "auto")
 
 
 def pattern_transform(model: torch.nn.Module, args, sort_edges: bool = False, static_graph: bool = False, slab_mode: str = "auto",
-                      **kwargs) -> ExportedProgram:
+                      dense: bool = False, **kwargs) -> ExportedProgram:
     """Export ``model`` on ``args`` and fuse its message-passing patterns (same call shape as the
     reference's ``pattern_transform(model, args, **kwargs)``, geot/match_replace/match_replace.py:8-32; extra keywords ``sort_edges``,
     ``static_graph``).  ``static_graph=True``: the fused nodes are bound to ``geot_amd.Graph`` handles built here, once, from the example
-    inputs' edge list (see :func:`bind_static_graphs` for the promise that goes with it); ``exported.geot_graphs`` lists the handles."""
+    inputs' edge list (see :func:`bind_static_graphs` for the promise that goes with it); ``exported.geot_graphs`` lists the handles.
+    ``dense=True``: the layers' products and normalisations become ``geot_amd.linear`` / ``geot_amd.layer_norm`` nodes too
+    (:func:`rewrite_dense`); ``exported.geot_dense_nodes`` counts them."""
     exported = export(model, args, **kwargs)
     exported.geot_fused_nodes = rewrite_graph(exported.graph_module, sort_edges=sort_edges and not static_graph)
     exported.geot_graphs = bind_static_graphs(exported, args, slab_mode=slab_mode) if static_graph else []
+    exported.geot_dense_nodes = rewrite_dense(exported.graph_module) if dense else 0
     return exported

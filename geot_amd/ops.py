@@ -439,7 +439,7 @@ torch.library.register_autograd("geot::index_scatter", _is_backward, setup_conte
 
 
 # --------------------------------------------------------------------------------------------------
-# dense rows (csrc/host_dense.cpp): fake-tensor rules and autograd formulas of the differentiable forms
+# dense rows (csrc/host_dense.cpp, which holds their autograd formulas too): fake-tensor rules
 # --------------------------------------------------------------------------------------------------
 _ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 _FLOATS = {torch.float32: _lib.GEOT_F32, torch.float16: _lib.GEOT_F16, torch.bfloat16: _lib.GEOT_BF16}
@@ -500,80 +500,6 @@ def _(grad, x, weight, bias, stats, need_params):
     dtype = next((p.dtype for p in (weight, bias) if p is not None), x.dtype)
     n = x.shape[-1] if need_params else 0
     return x.new_empty(x.shape), x.new_empty([n], dtype=dtype), x.new_empty([n], dtype=dtype)
-
-
-def _once(name: str) -> None:
-    """These backward passes have no gradient of their own; a caller that asks for one (create_graph) is told so."""
-    if torch.is_grad_enabled():
-        raise NotImplementedError(f"{name}: the backward pass is not differentiable (create_graph=True is not supported)")
-
-
-def _linear_setup(ctx, inputs, output):
-    x, weight, bias, residual, activation = inputs
-    y, z = output
-    ctx.activation = activation
-    ctx.set_materialize_grads(False)
-    ctx.mark_non_differentiable(z)
-    # relu without a residual: y has z's sign, nothing else is kept
-    ctx.save_for_backward(x, weight, bias, y if activation == "relu" and residual is None else z)
-
-
-def _linear_backward(ctx, grad, _grad_z):
-    """y = act(z) + residual, z = x W^T + b:  dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = column sums of dz;  dresidual = dy."""
-    if grad is None:
-        return None, None, None, None, None
-    _once("linear")
-    x, weight, bias, z = ctx.saved_tensors
-    need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-    dx = dw = db = None
-    if need_x or need_w or need_b:
-        dx, dw, db = torch.ops.geot_dense.linear_backward(grad, x, weight, bias, z, ctx.activation, need_x, need_w, need_b)
-    return dx if need_x else None, dw if need_w else None, db if need_b else None, grad if need_r else None, None
-
-
-torch.library.register_autograd("geot_dense::linear_train", _linear_backward, setup_context=_linear_setup)
-
-
-def _segment_matmul_setup(ctx, inputs, output):
-    x, ptr, weight, _bias = inputs
-    ctx.set_materialize_grads(False)
-    ctx.save_for_backward(x, ptr, weight)
-
-
-def _segment_matmul_backward(ctx, grad):
-    """Per group g:  dx = dy W[g]^T;  dW[g] = x_g^T dy_g;  db[g] = column sums of dy_g."""
-    if grad is None:
-        return None, None, None, None
-    _once("segment_matmul")
-    x, ptr, weight = ctx.saved_tensors
-    need_x, _, need_w, need_b = ctx.needs_input_grad
-    dx, dw, db = torch.ops.geot_dense.segment_matmul_backward(grad, x, ptr, weight, need_x, need_w, need_b)
-    return dx if need_x else None, None, dw if need_w else None, db if need_b else None
-
-
-torch.library.register_autograd("geot_dense::segment_matmul_train", _segment_matmul_backward, setup_context=_segment_matmul_setup)
-
-
-def _layer_norm_setup(ctx, inputs, output):
-    x, weight, bias, _eps = inputs
-    _y, stats = output
-    ctx.set_materialize_grads(False)
-    ctx.mark_non_differentiable(stats)
-    ctx.save_for_backward(x, weight, bias, stats)
-
-
-def _layer_norm_backward(ctx, grad, _grad_stats):
-    """h = (x - mean) rstd, g = dy w:  dx = rstd (g - mean g - h mean(g h));  dw = sum over rows of dy h;  db = sum over rows of dy."""
-    if grad is None:
-        return None, None, None, None
-    _once("layer_norm")
-    x, weight, bias, stats = ctx.saved_tensors
-    need_x, need_w, need_b, _ = ctx.needs_input_grad
-    dx, dw, db = torch.ops.geot_dense.layer_norm_backward(grad, x, weight, bias, stats, need_w or need_b)
-    return dx if need_x else None, dw if need_w else None, db if need_b else None, None
-
-
-torch.library.register_autograd("geot_dense::layer_norm_train", _layer_norm_backward, setup_context=_layer_norm_setup)
 
 
 # --------------------------------------------------------------------------------------------------

@@ -405,7 +405,7 @@ int geot_linear_grad_preactivation(const void *dy, const void *z, const void *x,
 int geot_linear_grad_input(const void *dz, const void *weight, void *dx, int64_t rows, int64_t in, int64_t out, int dtype, void *stream);
 /* dweight = dz^T x [out, in]; dbias = column sums of dz [out] or NULL.  The rows are split over workgroups and the parts joined in a
  * fixed order; `workspace`: geot_linear_grad_weight_workspace_bytes, 16-byte aligned, no content expected, free after the call. */
-size_t geot_linear_grad_weight_workspace_bytes(int64_t rows, int64_t in, int64_t out);
+size_t geot_linear_grad_weight_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype);
 int geot_linear_grad_weight(const void *dz, const void *x, int64_t ldx, void *dweight, void *dbias, int64_t rows, int64_t in, int64_t out,
                             int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
@@ -419,7 +419,7 @@ int geot_segment_matmul(const void *x, int64_t ldx, const int64_t *ptr, const vo
 int geot_segment_matmul_grad_input(const void *dy, const int64_t *ptr, const void *weight, void *dx, int64_t rows, int64_t groups, int64_t in,
                                    int64_t out, int dtype, void *stream);
 /* dweight[g] = x_g^T dy_g [groups, in, out]; dbias[g] = column sums of dy_g [groups, out] or NULL */
-size_t geot_segment_matmul_grad_weight_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out);
+size_t geot_segment_matmul_grad_weight_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype);
 int geot_segment_matmul_grad_weight(const void *x, int64_t ldx, const int64_t *ptr, const void *dy, void *dweight, void *dbias, int64_t rows,
                                     int64_t groups, int64_t in, int64_t out, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 

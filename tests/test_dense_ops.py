@@ -157,8 +157,8 @@ def test_refused_abi_calls():
     assert L.geot_linear(None, 4, None, None, None, 0, None, None, 0, 4, 4, 9, 0, None) == einval
     assert L.geot_linear(16, 4, 16, None, None, 0, None, 16, 2, 4, 4, 0, 1, None) == eunsupported       # (float64: refused before any launch)
     assert L.geot_segment_matmul(16, 4, 16, 16, None, 16, 2, 65536, 4, 4, 0, None) == einval
-    need = L.geot_linear_grad_weight_workspace_bytes(1_000_000, 64, 64)
-    assert need > 0 and L.geot_linear_grad_weight_workspace_bytes(100, 64, 64) == 0
+    need = L.geot_linear_grad_weight_workspace_bytes(1_000_000, 64, 64, 0)
+    assert need > 0 and L.geot_linear_grad_weight_workspace_bytes(100, 64, 64, 0) == 0
     assert L.geot_linear_grad_weight(16, 16, 64, 16, 16, 1_000_000, 64, 64, 0, 16, need - 4, None) == eworkspace
     assert L.geot_layer_norm(16, 4, None, None, 16, None, 2, 4, 1e-5, 1, 1, None) == eunsupported
     assert L.geot_layer_norm_backward(16, 4, None, 16, 16, 16, 16, 16, 2, 4, 0, 0, 16, 4, None) == eworkspace
@@ -737,3 +737,60 @@ def test_compile():
         assert torch.allclose(a, c, rtol=1e-5, atol=1e-5)
     with torch.no_grad():
         assert torch.allclose(torch.compile(f)(*leaves), want, rtol=1e-5, atol=1e-5)
+
+
+# ---- in rewritten models ----------------------------------------------------------------------------------------------------------------
+class _Block(torch.nn.Module):
+    """A layer in plain torch: aggregation, feed-forward with a skip connection, normalisation, and a product that must keep its form."""
+
+    def __init__(self, f):
+        super().__init__()
+        self.a, self.b, self.c = torch.nn.Linear(f, 2 * f), torch.nn.Linear(2 * f, f), torch.nn.Linear(f, f, bias=False)
+        self.norm = torch.nn.LayerNorm(f)
+
+    def forward(self, x, edge_index):
+        row, col = edge_index[0], edge_index[1]
+        agg = x.new_zeros(x.shape).index_add(0, row, x.index_select(0, col))
+        h = self.b(torch.nn.functional.gelu(self.a(agg))) + x
+        z = self.c(h)
+        return self.norm(torch.nn.functional.silu(z)) * z       # z is used twice: its activation stays outside
+
+
+def _block_problem(device):
+    torch.manual_seed(0)
+    g = torch.Generator().manual_seed(1)
+    row = torch.sort(torch.randint(0, 300, (2000,), generator=g)).values
+    return _Block(24).to(device), (torch.randn(300, 24, generator=g).to(device), torch.stack([row, torch.randint(0, 300, (2000,), generator=g)]).to(device))
+
+
+def test_rewritten_model_nodes():
+    from geot_amd.match_replace import pattern_transform
+    model, args = _block_problem("cpu")
+    plain = pattern_transform(model, args)
+    assert plain.geot_dense_nodes == 0 and plain.geot_fused_nodes == 1
+    ep = pattern_transform(model, args, dense=True)
+    nodes = [n for n in ep.graph_module.graph.nodes if n.op == "call_function"]
+    linears = [n for n in nodes if n.target == torch.ops.geot_dense.linear.default]
+    assert ep.geot_dense_nodes == 4 and ep.geot_fused_nodes == 1
+    assert [(n.args[4], n.args[3] is not None, n.args[2] is not None) for n in linears] == [("gelu", False, True), ("none", True, True), ("none", False, False)]
+    assert sum(n.target == torch.ops.geot_dense.layer_norm.default for n in nodes) == 1
+    assert sum(n.target == torch.ops.aten.silu.default for n in nodes) == 1
+
+
+@gpu
+def test_rewritten_model_computes_and_trains():
+    from geot_amd.match_replace import pattern_transform
+    model, args = _block_problem("cuda")
+    want = model(*args)
+    params = list(model.parameters())
+    dy = torch.randn(want.shape, generator=torch.Generator().manual_seed(2)).cuda()
+    grads = torch.autograd.grad(want, params, dy)
+    ep = pattern_transform(model, args, dense=True)
+    mod = ep.module()
+    got = mod(*args)
+    new = dict(mod.named_parameters())
+    got_grads = torch.autograd.grad(got, [new[k] for k, _ in model.named_parameters()], dy)
+    for a, b in zip((want, *grads), (got, *got_grads)):
+        assert float((a - b).abs().max()) <= 1e-4 * max(1.0, float(a.abs().max()))
+    with torch.no_grad():
+        assert float((mod(*args) - want).abs().max()) <= 1e-4 * max(1.0, float(want.abs().max()))
