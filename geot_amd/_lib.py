@@ -49,7 +49,8 @@ SYMBOLS = [
     "geot_slab_units", "geot_slab_full_chip", "geot_slab_rows_per_group", "geot_slab_rows_per_group_dtype", "geot_slab_units_for", "geot_slab_rows_per_group_shape", "geot_slab_workspace_bytes", "geot_slab_workspace_bytes_staged", "geot_slab_spmm", "geot_slab_sddmm", "geot_slab_sddmm_staged", "geot_slab_mh_sddmm", "geot_slab_to_plan_order",
     "geot_slab_plan_scratch_bytes", "geot_slab_plan_rows", "geot_slab_plan_groups", "geot_slab_plan_edges",
     "geot_linear", "geot_linear_keeps_preactivation", "geot_linear_grad_preactivation_workspace_bytes", "geot_linear_grad_preactivation",
-    "geot_linear_grad_input", "geot_linear_grad_weight_workspace_bytes", "geot_linear_grad_weight",
+    "geot_linear_grad_input", "geot_linear_grad_input_workspace_bytes", "geot_segment_matmul_workspace_bytes", "geot_segment_matmul_grad_input_workspace_bytes",
+    "geot_linear_grad_weight_workspace_bytes", "geot_linear_grad_weight",
     "geot_segment_matmul", "geot_segment_matmul_grad_input", "geot_segment_matmul_grad_weight_workspace_bytes", "geot_segment_matmul_grad_weight",
     "geot_layer_norm", "geot_layer_norm_backward_workspace_bytes", "geot_layer_norm_backward",
     "geot_profile_enable", "geot_profile_reset", "geot_profile_read", "geot_profile_box", "geot_profile_box_rows", "geot_tune", "geot_set_option", "geot_last_kernel",
@@ -276,12 +277,17 @@ def load() -> ctypes.CDLL:
     L.geot_linear_grad_preactivation_workspace_bytes.restype = c_sz
     L.geot_linear_grad_preactivation_workspace_bytes.argtypes = [c_i64, c_i64]
     L.geot_linear_grad_preactivation.argtypes = [c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_int, c_vp, c_sz, c_vp]
-    L.geot_linear_grad_input.argtypes = [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_vp]
+    L.geot_linear_grad_input.argtypes = [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_vp, c_sz, c_vp]
+    L.geot_linear_grad_input_workspace_bytes.restype = c_sz
+    L.geot_linear_grad_input_workspace_bytes.argtypes = [c_i64, c_i64, c_i64, c_int]
+    for f in (L.geot_segment_matmul_workspace_bytes, L.geot_segment_matmul_grad_input_workspace_bytes):
+        f.restype = c_sz
+        f.argtypes = [c_i64, c_i64, c_i64, c_i64, c_int]
     L.geot_linear_grad_weight_workspace_bytes.restype = c_sz
     L.geot_linear_grad_weight_workspace_bytes.argtypes = [c_i64, c_i64, c_i64, c_int]
     L.geot_linear_grad_weight.argtypes = [c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_vp, c_sz, c_vp]
-    L.geot_segment_matmul.argtypes = [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp]
-    L.geot_segment_matmul_grad_input.argtypes = [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp]
+    L.geot_segment_matmul.argtypes = [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_sz, c_vp]
+    L.geot_segment_matmul_grad_input.argtypes = [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_sz, c_vp]
     L.geot_segment_matmul_grad_weight_workspace_bytes.restype = c_sz
     L.geot_segment_matmul_grad_weight_workspace_bytes.argtypes = [c_i64, c_i64, c_i64, c_i64, c_int]
     L.geot_segment_matmul_grad_weight.argtypes = [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_sz, c_vp]

@@ -589,6 +589,8 @@ struct RowsArgs {
   int64_t n, k;
   uint32_t slots, tiles_n, band; // band: row tiles of a group of tiles (tile_of)
   int act;
+  float *part;     // partial sums of gridDim.y shares of the reduction, k_share values each: [shares][rows][n]
+  int64_t k_share;
 };
 
 // V consecutive columns of a row, `cols` of which exist
@@ -693,7 +695,8 @@ __device__ inline void tile_of(uint32_t id, uint32_t slots, uint32_t tiles_n, ui
 }
 
 // y rows.  BR: B's output index is contiguous (element (n, k) at b[k * ldb + n]), otherwise its reduction index (b[n * ldb + k]).
-template <typename T, int BM, int BN, int WM, int WN, bool BR, int NBUF>
+// SPLIT: a workgroup takes its share of the reduction and leaves float32 sums to mm_rows_join_kernel.
+template <typename T, int BM, int BN, int WM, int WN, bool BR, int NBUF, bool SPLIT>
 __global__ __launch_bounds__(64 * WM * WN, NBUF == 1 ? 3 : 2) void mm_rows_kernel(const RowsArgs g) {
   using E = Elem<T>;
   using LA = Tile<T, BM>;
@@ -709,7 +712,9 @@ __global__ __launch_bounds__(64 * WM * WN, NBUF == 1 ? 3 : 2) void mm_rows_kerne
   if (r0 >= piece.end) return;
   const int64_t rows = piece.end - r0 < BM ? piece.end - r0 : BM;
   const bool real = piece.group >= 0;
-  const int64_t k_len = real ? g.k : 0;
+  if (SPLIT && !real) return; // (the join writes its zeros)
+  const int64_t k_begin = SPLIT ? blockIdx.y * g.k_share : 0;
+  const int64_t k_end = SPLIT && k_begin + g.k_share < g.k ? k_begin + g.k_share : g.k, k_len = real ? k_end - k_begin : 0;
   const T *A = static_cast<const T *>(g.a);
   const T *B = static_cast<const T *>(g.b) + (real ? piece.group * g.b_group : 0);
 
@@ -717,13 +722,37 @@ __global__ __launch_bounds__(64 * WM * WN, NBUF == 1 ? 3 : 2) void mm_rows_kerne
   acc.clear();
   StageK<T, BM, NT> sa;
   typename std::conditional<BR, StageR<T, BN, NT, false>, StageK<T, BN, NT>>::type sb;
-  sa.open(A, g.lda, r0, rows, 0, k_len);
-  sb.open(B, g.ldb, n0, g.n - n0, 0, k_len);
+  sa.open(A, g.lda, r0, rows, k_begin, k_begin + k_len);
+  sb.open(B, g.ldb, n0, g.n - n0, k_begin, k_begin + k_len);
   staged_products<T, BM, BN, WM, WN, NBUF>(sa, sb, acc, lds, k_len, tid, wm, wn, lane);
 
   constexpr int V = 16 / sizeof(T), TPR = BN / V;
   const int64_t nc = n0 + (tid % TPR) * V;
   const int cols = nc + V <= g.n ? V : (nc < g.n ? (int)(g.n - nc) : 0);
+  if constexpr (SPLIT) {
+    float *out = reinterpret_cast<float *>(lds);
+#pragma unroll
+    for (int i = 0; i < acc.FM; ++i) {
+      if (i) __syncthreads();
+      acc.put(out, i, wm, wn, lane);
+      __syncthreads();
+      for (int lr = tid / TPR; lr < 32 * WM; lr += NT / TPR) {
+        const int64_t tr = acc.tile_row(lr, i);
+        if (tr >= rows || cols == 0) continue;
+        float *to = g.part + ((int64_t)blockIdx.y * g.groups.rows + r0 + tr) * g.n + nc;
+        const float *from = out + lr * (BN + 4) + (tid % TPR) * V;
+#pragma unroll
+        for (int c = 0; c < V; c += 4) {
+          if (c + 4 <= cols) *reinterpret_cast<Packed16<float> *>(to + c) = *reinterpret_cast<const u32x4 *>(from + c);
+          else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (c + e < cols) to[c + e] = from[c + e];
+        }
+      }
+    }
+    return;
+  }
   float bias[V], none[V];
 #pragma unroll
   for (int v = 0; v < V; ++v)
@@ -732,6 +761,50 @@ __global__ __launch_bounds__(64 * WM * WN, NBUF == 1 ? 3 : 2) void mm_rows_kerne
     tile_epilogue<T, BM, BN, WM, WN, decltype(act)::value, false, BR>(g, acc, reinterpret_cast<float *>(lds), static_cast<const T *>(g.residual), g.ldr, B, r0, rows, nc, cols,
                                                                      k_len, bias, none, tid, wm, wn, lane);
   });
+}
+
+// The shares of the reduction, added in their order, and what becomes of a row's sums (no activation or residual: linear splits inside a
+// workgroup, mm_few_rows_kernel).  One wave a row of a tile of 128 rows.
+template <typename T, int BN, bool BR> __global__ __launch_bounds__(kThreads) void mm_rows_join_kernel(const RowsArgs g, uint32_t shares) {
+  constexpr int V = 16 / sizeof(T), TPR = BN / V, RPP = kThreads / TPR;
+  const uint32_t slot = blockIdx.x / g.tiles_n, tile = blockIdx.x % g.tiles_n;
+  const Piece piece = piece_of(g.groups, 7, slot);
+  const int64_t r0 = piece.begin + piece.index * 128;
+  if (r0 >= piece.end) return;
+  const int64_t end = piece.end - r0 < 128 ? piece.end : r0 + 128;
+  const bool real = piece.group >= 0;
+  const int64_t nc = (int64_t)tile * BN + (threadIdx.x % TPR) * V;
+  const int cols = nc + V <= g.n ? V : (nc < g.n ? (int)(g.n - nc) : 0);
+  if (cols == 0) return;
+  float bias[V], none[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    bias[v] = g.bias && real && v < cols ? as_float(static_cast<const T *>(g.bias)[piece.group * g.bias_group + nc + v]) : 0.0f;
+  for (int64_t row = r0 + threadIdx.x / TPR + (int64_t)blockIdx.y * RPP; row < end; row += (int64_t)gridDim.y * RPP) {
+    float v[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) v[c] = 0.0f;
+    if (real) {
+#pragma unroll 4
+      for (uint32_t s = 0; s < shares; ++s) {
+        const float *p = g.part + ((int64_t)s * g.groups.rows + row) * g.n + nc;
+#pragma unroll
+        for (int c = 0; c < V; c += 4) {
+          const u32x4 q = load_cols<float, 4>(p + c, cols - c < 4 ? (cols > c ? cols - c : 0) : 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[c + e] += __uint_as_float(q[e]);
+        }
+      }
+      if constexpr (Elem<T>::PARTS == 3) {
+        const float *B = static_cast<const float *>(g.b) + piece.group * g.b_group;
+#pragma unroll
+        for (int c = 0; c < V; ++c)
+          if (!finite(v[c]) && c < cols)
+            v[c] = element_again(static_cast<const float *>(g.a) + row * g.lda, 1, B + (BR ? nc + c : (nc + c) * g.ldb), BR ? g.ldb : 1, g.k);
+      }
+    }
+    finish_row<T, V, GEOT_ACT_NONE, false>(g, row, nc, cols, v, bias, false, u32x4{0, 0, 0, 0}, none);
+  }
 }
 
 // dz = dy act'(z) with z = x W^T + b computed again instead of read: narrow layers are bound by memory, and z costs a write in the forward
@@ -1128,13 +1201,40 @@ int launched(const char *name) {
 
 constexpr int64_t kMaxBlocks = ((int64_t)1 << 31) - 1;
 
+// Reduction values of a workgroup: all of them (k) where the tiles fill the chip, or the reduction is short; else a share such that about
+// two workgroups a CU run, at least four steps each.  (17 rows x 4048 -> 144 f32 in 2 groups: 5 tiles of 127 steps were 192 us.)
+int64_t rows_share(int64_t rows, int64_t groups, bool with_ptr, int64_t n, int64_t k, bool f32) {
+  const int64_t bn = f32 || n <= 64 ? 64 : 128, bk = f32 ? 32 : 64;
+  const int64_t tiles = ((rows + 127) / 128 + (with_ptr ? (groups < rows ? groups : rows) : 0)) * ((n + bn - 1) / bn);
+  if (tiles <= 0 || tiles >= 256 || k < 8 * bk) return k;
+  int64_t shares = (512 + tiles - 1) / tiles;
+  const int64_t most = k / (4 * bk);
+  shares = shares < most ? shares : most;
+  return ((k + shares - 1) / shares + bk - 1) / bk * bk;
+}
+size_t rows_workspace(int64_t rows, int64_t groups, bool with_ptr, int64_t n, int64_t k, int dtype) {
+  const int64_t share = rows_share(rows, groups, with_ptr, n, k, dtype == GEOT_F32);
+  return share < k ? (size_t)((k + share - 1) / share) * (size_t)rows * (size_t)n * sizeof(float) : 0;
+}
 template <typename T, int BM, int BN, int WM, int WN, bool BR, int NBUF> int run_rows(RowsArgs &g, hipStream_t st) {
   const int64_t tiles_n = (g.n + BN - 1) / BN, slots = slots_of(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, BM);
   if (tiles_n > kMaxBlocks / 8 || slots > kMaxBlocks / tiles_n) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
   g.tiles_n = (uint32_t)tiles_n;
   g.slots = (uint32_t)slots;
   g.band = g.groups.ptr ? 1 : 8;
-  hipLaunchKernelGGL((mm_rows_kernel<T, BM, BN, WM, WN, BR, NBUF>), dim3((unsigned)(g.slots * g.tiles_n)), dim3(64 * WM * WN), 0, st, g);
+  const unsigned blocks = g.slots * g.tiles_n;
+  if constexpr (BM == 128) {
+    const int64_t share = rows_share(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, g.n, g.k, Elem<T>::PARTS == 3);
+    if (g.part && share < g.k) {
+      const unsigned shares = (unsigned)((g.k + share - 1) / share);
+      g.k_share = share;
+      hipLaunchKernelGGL((mm_rows_kernel<T, BM, BN, WM, WN, BR, NBUF, true>), dim3(blocks, shares), dim3(64 * WM * WN), 0, st, g);
+      if (const int rc = launched("mm_rows_kernel")) return rc;
+      hipLaunchKernelGGL((mm_rows_join_kernel<T, BN, BR>), dim3(blocks, 4), dim3(kThreads), 0, st, g, shares);
+      return launched(nullptr);
+    }
+  }
+  hipLaunchKernelGGL((mm_rows_kernel<T, BM, BN, WM, WN, BR, NBUF, false>), dim3(blocks), dim3(64 * WM * WN), 0, st, g);
   return launched("mm_rows_kernel");
 }
 template <typename T, int FM> int run_few(RowsArgs &g, hipStream_t st) {
@@ -1156,8 +1256,14 @@ template <typename T, bool BR> int rows_typed(RowsArgs &g, hipStream_t st) {
     return run_rows<T, 128, 128, 2, 2, BR, 1>(g, st);
   }
 }
-int rows_product(RowsArgs &g, bool br, int dtype, hipStream_t st) {
+// (workspace: of the products that may split their reduction over workgroups)
+int rows_product(RowsArgs &g, bool br, int dtype, hipStream_t st, bool may_split = false, void *workspace = nullptr, size_t workspace_bytes = 0) {
   if (g.groups.rows == 0 || g.n == 0) return GEOT_OK;
+  if (may_split) {
+    const size_t need = rows_workspace(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, g.n, g.k, dtype);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return geot_internal_fail(GEOT_EWORKSPACE, "rows product: workspace too small or misaligned");
+    g.part = need ? static_cast<float *>(workspace) : nullptr;
+  }
   switch (dtype) {
   case GEOT_F32: return br ? rows_typed<float, true>(g, st) : rows_typed<float, false>(g, st);
   case GEOT_F16: return br ? rows_typed<f16, true>(g, st) : rows_typed<f16, false>(g, st);
@@ -1308,13 +1414,18 @@ int geot_linear(const void *x, int64_t ldx, const void *weight, const void *bias
   return rows_product(g, false, dtype, static_cast<hipStream_t>(stream));
 }
 
-int geot_linear_grad_input(const void *dz, const void *weight, void *dx, int64_t rows, int64_t in, int64_t out, int dtype, void *stream) {
+size_t geot_linear_grad_input_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype) {
+  return bad_size(rows, in, out) ? 0 : rows_workspace(rows, 1, false, in, out, dtype);
+}
+
+int geot_linear_grad_input(const void *dz, const void *weight, void *dx, int64_t rows, int64_t in, int64_t out, int dtype, void *workspace, size_t workspace_bytes,
+                           void *stream) {
   if (bad_size(rows, in, out)) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_input: negative size");
   if (rows > 0 && in > 0 && (!dx || (out > 0 && (!dz || !weight)))) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_input: null pointer");
   RowsArgs g{};
   g.a = dz; g.lda = out; g.b = weight; g.ldb = in; g.y = dx; g.ldy = in;
   g.groups = {nullptr, 1, rows}; g.n = in; g.k = out; g.act = GEOT_ACT_NONE;
-  return rows_product(g, true, dtype, static_cast<hipStream_t>(stream));
+  return rows_product(g, true, dtype, static_cast<hipStream_t>(stream), true, workspace, workspace_bytes);
 }
 
 size_t geot_linear_grad_weight_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype) {
@@ -1363,24 +1474,32 @@ int geot_linear_grad_preactivation(const void *dy, const void *z, const void *x,
   return geot_internal_fail(GEOT_EUNSUPPORTED, "matrix products take float32, float16 and bfloat16");
 }
 
+size_t geot_segment_matmul_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype) {
+  return bad_size(rows, in, out) || groups < 0 || groups > 65535 ? 0 : rows_workspace(rows, groups, true, out, in, dtype);
+}
+
 int geot_segment_matmul(const void *x, int64_t ldx, const int64_t *ptr, const void *weight, const void *bias, void *y, int64_t rows, int64_t groups,
-                        int64_t in, int64_t out, int dtype, void *stream) {
+                        int64_t in, int64_t out, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
   if (bad_size(rows, in, out) || groups < 0 || groups > 65535 || ldx < 0) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul: negative size, or more than 65535 groups");
   if (rows > 0 && out > 0 && (!y || !ptr || (in > 0 && groups > 0 && (!x || !weight)))) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul: null pointer");
   RowsArgs g{};
   g.a = x; g.lda = ldx; g.b = weight; g.ldb = out; g.b_group = in * out; g.bias = bias; g.bias_group = out; g.y = y; g.ldy = out;
   g.groups = {ptr, groups, rows}; g.n = out; g.k = in; g.act = GEOT_ACT_NONE;
-  return rows_product(g, true, dtype, static_cast<hipStream_t>(stream));
+  return rows_product(g, true, dtype, static_cast<hipStream_t>(stream), true, workspace, workspace_bytes);
+}
+
+size_t geot_segment_matmul_grad_input_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype) {
+  return bad_size(rows, in, out) || groups < 0 || groups > 65535 ? 0 : rows_workspace(rows, groups, true, in, out, dtype);
 }
 
 int geot_segment_matmul_grad_input(const void *dy, const int64_t *ptr, const void *weight, void *dx, int64_t rows, int64_t groups, int64_t in, int64_t out,
-                                   int dtype, void *stream) {
+                                   int dtype, void *workspace, size_t workspace_bytes, void *stream) {
   if (bad_size(rows, in, out) || groups < 0 || groups > 65535) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul_grad_input: negative size, or more than 65535 groups");
   if (rows > 0 && in > 0 && (!dx || !ptr || (out > 0 && groups > 0 && (!dy || !weight)))) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul_grad_input: null pointer");
   RowsArgs g{};
   g.a = dy; g.lda = out; g.b = weight; g.ldb = out; g.b_group = in * out; g.y = dx; g.ldy = in;
   g.groups = {ptr, groups, rows}; g.n = in; g.k = out; g.act = GEOT_ACT_NONE;
-  return rows_product(g, false, dtype, static_cast<hipStream_t>(stream));
+  return rows_product(g, false, dtype, static_cast<hipStream_t>(stream), true, workspace, workspace_bytes);
 }
 
 size_t geot_segment_matmul_grad_weight_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype) {

@@ -132,7 +132,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward_op(const at::Tens
   }
   if (need_x) {
     dx = at::empty(x_in.sizes(), x_in.options());
-    GEOT_CALL(geot_linear_grad_input(dz.data_ptr(), w.data_ptr(), dx.data_ptr(), x.rows, in, out, dt, st));
+    const at::Tensor ws = scratch(x_in, geot_linear_grad_input_workspace_bytes(x.rows, in, out, dt));
+    GEOT_CALL(geot_linear_grad_input(dz.data_ptr(), w.data_ptr(), dx.data_ptr(), x.rows, in, out, dt, ws.data_ptr(), ws.numel(), st));
   }
   const bool sums = need_b && act == GEOT_ACT_NONE;
   if (need_w || sums) {
@@ -181,8 +182,9 @@ at::Tensor segment_matmul_forward_op(const at::Tensor &x_in, const at::Tensor &p
   const at::Tensor ptr = ptr_in.contiguous(), w = w_in.contiguous();
   const auto bias = dense(bias_in);
   at::Tensor y = at::empty({x.rows, w.size(2)}, x_in.options());
+  const at::Tensor ws = scratch(x_in, geot_segment_matmul_workspace_bytes(x.rows, w.size(0), w.size(1), w.size(2), dt));
   GEOT_CALL(geot_segment_matmul(x.t.data_ptr(), x.ld, index_ptr(ptr), w.data_ptr(), data_of(bias), y.data_ptr(), x.rows, w.size(0), w.size(1), w.size(2), dt,
-                                stream_of(x_in)));
+                                ws.data_ptr(), ws.numel(), stream_of(x_in)));
   return y;
 }
 
@@ -201,7 +203,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> segment_matmul_backward_op(const 
   at::Tensor dx, dw, db;
   if (need_x) {
     dx = at::empty(x_in.sizes(), x_in.options());
-    GEOT_CALL(geot_segment_matmul_grad_input(dy.data_ptr(), index_ptr(ptr), w.data_ptr(), dx.data_ptr(), x.rows, groups, in, out, dt, st));
+    const at::Tensor ws = scratch(x_in, geot_segment_matmul_grad_input_workspace_bytes(x.rows, groups, in, out, dt));
+    GEOT_CALL(geot_segment_matmul_grad_input(dy.data_ptr(), index_ptr(ptr), w.data_ptr(), dx.data_ptr(), x.rows, groups, in, out, dt, ws.data_ptr(), ws.numel(), st));
   }
   if (need_w || need_b) {
     const int64_t rows_p = need_w ? in : 0;

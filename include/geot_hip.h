@@ -401,8 +401,11 @@ size_t geot_linear_grad_preactivation_workspace_bytes(int64_t rows, int64_t out)
 int geot_linear_grad_preactivation(const void *dy, const void *z, const void *x, int64_t ldx, const void *weight, const void *bias, void *dz,
                                    void *dbias, int64_t rows, int64_t in, int64_t out, int activation, int dtype, void *workspace,
                                    size_t workspace_bytes, void *stream);
-/* dx = dz weight   [rows, in] */
-int geot_linear_grad_input(const void *dz, const void *weight, void *dx, int64_t rows, int64_t in, int64_t out, int dtype, void *stream);
+/* dx = dz weight   [rows, in].  Products of few tiles split their reduction over workgroups; workspaces of these calls: ..._workspace_bytes
+ * (0 where none is needed), 16-byte aligned, no content expected, free after the call. */
+size_t geot_linear_grad_input_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype);
+int geot_linear_grad_input(const void *dz, const void *weight, void *dx, int64_t rows, int64_t in, int64_t out, int dtype, void *workspace,
+                           size_t workspace_bytes, void *stream);
 /* dweight = dz^T x [out, in]; dbias = column sums of dz [out] or NULL.  The rows are split over workgroups and the parts joined in a
  * fixed order; `workspace`: geot_linear_grad_weight_workspace_bytes, 16-byte aligned, no content expected, free after the call. */
 size_t geot_linear_grad_weight_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype);
@@ -413,11 +416,13 @@ int geot_linear_grad_weight(const void *dz, const void *x, int64_t ldx, void *dw
  * [groups, in, out], bias [groups, out] or NULL (groups <= 65535).  Rows in front of ptr[0] and behind ptr[groups] come out 0, as do
  * their gradients; a group without rows has gradient 0.  Entries of ptr are clamped into [0, rows]; with entries that do not ascend the
  * result is unspecified, but nothing outside the operands is touched. */
+size_t geot_segment_matmul_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype);
 int geot_segment_matmul(const void *x, int64_t ldx, const int64_t *ptr, const void *weight, const void *bias, void *y, int64_t rows,
-                        int64_t groups, int64_t in, int64_t out, int dtype, void *stream);
+                        int64_t groups, int64_t in, int64_t out, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 /* dx[i] = dy[i] weight[g]^T   [rows, in] */
+size_t geot_segment_matmul_grad_input_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype);
 int geot_segment_matmul_grad_input(const void *dy, const int64_t *ptr, const void *weight, void *dx, int64_t rows, int64_t groups, int64_t in,
-                                   int64_t out, int dtype, void *stream);
+                                   int64_t out, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 /* dweight[g] = x_g^T dy_g [groups, in, out]; dbias[g] = column sums of dy_g [groups, out] or NULL */
 size_t geot_segment_matmul_grad_weight_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype);
 int geot_segment_matmul_grad_weight(const void *x, int64_t ldx, const int64_t *ptr, const void *dy, void *dweight, void *dbias, int64_t rows,

@@ -98,7 +98,7 @@ class LinearReference:
 
 
 LINEAR_SHAPES = [(1, 1, 1), (5, 16, 32), (1, 520, 96), (3, 64, 1000), (128, 128, 128), (129, 65, 33), (300, 602, 256), (257, 64, 130), (64, 200, 72),
-                 (200, 7, 128), (1000, 33, 64), (31, 1024, 40)]
+                 (200, 7, 128), (1000, 33, 64), (31, 1024, 40), (2, 120, 1990)]
 
 
 # ---- refusals: no GPU needed ------------------------------------------------------------------------------------------------------
@@ -156,7 +156,10 @@ def test_refused_abi_calls():
     assert L.geot_linear(None, 4, None, None, None, 0, None, None, 2, 4, 4, 0, 0, None) == einval
     assert L.geot_linear(None, 4, None, None, None, 0, None, None, 0, 4, 4, 9, 0, None) == einval
     assert L.geot_linear(16, 4, 16, None, None, 0, None, 16, 2, 4, 4, 0, 1, None) == eunsupported       # (float64: refused before any launch)
-    assert L.geot_segment_matmul(16, 4, 16, 16, None, 16, 2, 65536, 4, 4, 0, None) == einval
+    assert L.geot_segment_matmul(16, 4, 16, 16, None, 16, 2, 65536, 4, 4, 0, None, 0, None) == einval
+    need = L.geot_segment_matmul_workspace_bytes(17, 2, 4096, 128, 0)
+    assert need > 0 and L.geot_segment_matmul_workspace_bytes(1_000_000, 2, 4096, 128, 0) == 0
+    assert L.geot_segment_matmul(16, 4096, 16, 16, None, 16, 17, 2, 4096, 128, 0, 16, need - 4, None) == eworkspace
     need = L.geot_linear_grad_weight_workspace_bytes(1_000_000, 64, 64, 0)
     assert need > 0 and L.geot_linear_grad_weight_workspace_bytes(100, 64, 64, 0) == 0
     assert L.geot_linear_grad_weight(16, 16, 64, 16, 16, 1_000_000, 64, 64, 0, 16, need - 4, None) == eworkspace
@@ -381,6 +384,7 @@ SEGMENTS = [
     (list(range(0, 301, 3)), 24, 40),                       # 100 groups of 3 rows
     ([0, 1, 2, 3, 4], 512, 96),                             # one row a group
     ([0, 3000, 3001, 9000], 72, 48),                        # groups of several chunks beside tiny ones
+    ([2, 19, 19, 20], 1500, 700),                           # few rows, long reductions both ways: split over workgroups (25 rows)
 ]
 
 
@@ -389,7 +393,7 @@ SEGMENTS = [
 @pytest.mark.parametrize("case", range(len(SEGMENTS)))
 def test_segment_matmul(case, dtype):
     rows, k, n = SEGMENTS[case]
-    groups, m = len(rows) - 1, {4: 150, 5: 40}.get(case, rows[-1])
+    groups, m = len(rows) - 1, {4: 150, 5: 40, 9: 25}.get(case, rows[-1])
     x, w, b, dy = (rand(*s, dtype=dtype, seed=100 * case + i, scale=sc) for i, (s, sc) in enumerate(
         [((m, k), 1), ((groups, k, n), k ** -0.5), ((groups, n), 1), ((m, n), 1)]))
     ptr = torch.tensor(rows, device="cuda")
