@@ -54,17 +54,17 @@ template <typename T> using Packed8 = typename Packed<sizeof(T)>::x8;
 
 template <typename T> struct Elem;
 template <> struct Elem<bf16> {
-  static constexpr int PARTS = 1, BK = 64, VR = 4;
+  static constexpr int PARTS = 1, BK = 64;
   typedef bf16x8 Frag;
   static __device__ f32x16 mfma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct Elem<f16> {
-  static constexpr int PARTS = 1, BK = 64, VR = 4;
+  static constexpr int PARTS = 1, BK = 64;
   typedef f16x8 Frag;
   static __device__ f32x16 mfma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct Elem<float> {
-  static constexpr int PARTS = 3, BK = 32, VR = 2;
+  static constexpr int PARTS = 3, BK = 32;
   typedef bf16x8 Frag;
   static __device__ f32x16 mfma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
@@ -165,15 +165,17 @@ template <typename T, int R, int NT> struct StageK {
   }
 };
 
-// Staging, output index contiguous: element (row, k) at base[k * ld + row].  SUM: also adds up what it stages, per row.
-template <typename T, int R, int NT, bool SUM> struct StageR {
+// Staging, output index contiguous: element (row, k) at base[k * ld + row], transposed in registers.  SUM: also adds up what it stages, per row.
+template <typename T, int R, int NT, bool SUM, int LOAD = 8> struct StageR {
   using E = Elem<T>;
   using L = Tile<T, R>;
-  static constexpr int VR = E::VR; // rows of a thread's block: 8 bytes
+  static constexpr int VR = LOAD / sizeof(T), PW = LOAD / 4; // rows of a thread's block: LOAD bytes
+  using Piece = typename std::conditional<PW == 4, Packed16<T>, Packed8<T>>::type;
+  using Words = typename std::conditional<PW == 4, u32x4, u32x2>::type;
   static constexpr int BLOCKS = (R / VR) * L::CK;
   static constexpr int N = (BLOCKS + NT - 1) / NT;
   static constexpr bool WHOLE = BLOCKS % NT == 0;
-  u32x2 reg[N][8] = {};
+  Words reg[N][8] = {};
   float sum[SUM ? N : 1][VR];
   const T *base;
   int64_t ld, k_end;
@@ -202,7 +204,7 @@ template <typename T, int R, int NT, bool SUM> struct StageR {
       if (!WHOLE && idx >= BLOCKS) continue; // (whole waves)
       const T *p = base + (k0 + chunk * 8) * ld + (row + VR <= rows ? row : rows - VR);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) reg[i][j] = *reinterpret_cast<const Packed8<T> *>(p + j * ld);
+      for (int j = 0; j < 8; ++j) reg[i][j] = *reinterpret_cast<const Piece *>(p + j * ld);
     }
   }
   __device__ void load_any(int64_t k0, int tid) {
@@ -215,14 +217,14 @@ template <typename T, int R, int NT, bool SUM> struct StageR {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int64_t k = k0 + chunk * 8 + j;
-        u32x2 v = {0, 0};
+        Words v = {};
         if (k < k_end && wide) {
-          v = *reinterpret_cast<const Packed8<T> *>(p + j * ld);
+          v = *reinterpret_cast<const Piece *>(p + j * ld);
         } else if (k < k_end && row < rows) {
-          alignas(8) T tmp[VR];
+          alignas(16) T tmp[VR];
 #pragma unroll
           for (int r = 0; r < VR; ++r) tmp[r] = row + r < rows ? p[j * ld + r] : (T)0.0f;
-          v = *reinterpret_cast<const u32x2 *>(tmp);
+          v = *reinterpret_cast<const Words *>(tmp);
         }
         reg[i][j] = v;
       }
@@ -271,6 +273,23 @@ template <typename T, int R, int NT, bool SUM> struct StageR {
       }
     }
   }
+};
+
+// Both operands of that form, in tiles of R rows: one half of the threads stages A, the other B, each with 16-byte loads (64 experts,
+// 1024 -> 2048 f16, the weight's gradient: 360 us with every thread loading 8 bytes of both).
+template <typename T, int R, int NT, bool SUM> struct StagePair {
+  StageR<T, R, NT / 2, SUM, 16> st;
+  bool both;
+  __device__ bool fast() const { return both; }
+  __device__ void load_fast(int64_t k0, int tid) { st.load_fast(k0, tid % (NT / 2)); }
+  __device__ void load_any(int64_t k0, int tid) { st.load_any(k0, tid % (NT / 2)); }
+  __device__ void store(char *lds, int tid) { st.store(lds + tid / (NT / 2) * Tile<T, R>::BYTES, tid % (NT / 2)); }
+};
+struct StageNone {
+  __device__ bool fast() const { return true; }
+  __device__ void load_fast(int64_t, int) {}
+  __device__ void load_any(int64_t, int) {}
+  __device__ void store(char *, int) {}
 };
 
 // ---- the products of one staged pair of tiles -----------------------------------------------------------------------------------
@@ -968,8 +987,9 @@ struct WeightArgs {
   int sum_p;
 };
 
-template <int WHICH, typename A, typename B> __device__ inline auto &pick(A &a, B &b) {
-  if constexpr (WHICH == 1) return a;
+template <bool PAIR, int WHICH, typename A, typename B> __device__ inline auto &pick(A &a, B &b) {
+  if constexpr (PAIR) return a.st;
+  else if constexpr (WHICH == 1) return a;
   else return b;
 }
 // SUMS: column sums of nothing (0), p (1) or q (2) beside the product
@@ -994,11 +1014,20 @@ __global__ __launch_bounds__(64 * WM * WN, 3) void mm_weight_kernel(const Weight
 
   Accum<T, BM, BN, WM, WN> acc;
   acc.clear();
-  StageR<T, BM, NT, SUMS == 1> sa;
-  StageR<T, BN, NT, SUMS == 2> sb;
-  sa.open(P, g.ldp, i0, g.np - i0, r0, r1);
-  sb.open(Q, g.ldq, j0, g.nq - j0, r0, r1);
-  sa.add = sb.add = sums;
+  constexpr bool PAIR = E::PARTS == 1 && BM == 128 && BN == 128;
+  typename std::conditional<PAIR, StagePair<T, BM, NT, SUMS != 0>, StageR<T, BM, NT, SUMS == 1>>::type sa;
+  typename std::conditional<PAIR, StageNone, StageR<T, BN, NT, SUMS == 2>>::type sb;
+  const int half = __builtin_amdgcn_readfirstlane(tid / (NT / 2));
+  if constexpr (PAIR) {
+    sa.st.open(half ? Q : P, half ? g.ldq : g.ldp, half ? j0 : i0, half ? g.nq - j0 : g.np - i0, r0, r1);
+    sa.st.add = sums && half == SUMS - 1;
+    constexpr int VR = 16 / sizeof(T);
+    sa.both = (i0 + BM <= g.np || (g.np > i0 && (g.np - i0) % VR == 0)) && (j0 + BN <= g.nq || (g.nq > j0 && (g.nq - j0) % VR == 0));
+  } else {
+    sa.open(P, g.ldp, i0, g.np - i0, r0, r1);
+    sb.open(Q, g.ldq, j0, g.nq - j0, r0, r1);
+    sa.add = sb.add = sums;
+  }
   const int64_t k_len = r1 - r0;
   staged_products<T, BM, BN, WM, WN, 1>(sa, sb, acc, lds, k_len, tid, wm, wn, lane);
 
@@ -1056,15 +1085,17 @@ __global__ __launch_bounds__(64 * WM * WN, 3) void mm_weight_kernel(const Weight
   if constexpr (SUMS == 0) return;
   if (sums) { // (uniform over the workgroup) column sums: CK threads hold each column's share
     __syncthreads();
-    const int part_id = SUMS == 1 ? tid : (tid + NT / 2) % NT; // (as staged_products numbers the threads of each operand)
+    // (as staged_products and StagePair number the threads of each operand)
+    const int part_id = PAIR ? tid % (NT / 2) : SUMS == 1 ? tid : (tid + NT / 2) % NT;
+    const bool mine = !PAIR || half == SUMS - 1;
     constexpr int R = SUMS == 1 ? BM : BN;
     const int64_t first = SUMS == 1 ? i0 : j0, n = SUMS == 1 ? g.np : g.nq;
-    auto &st = pick<SUMS>(sa, sb);
+    auto &st = pick<PAIR, SUMS>(sa, sb);
     using S = typename std::remove_reference<decltype(st)>::type;
 #pragma unroll
     for (int i = 0; i < S::N; ++i) {
       const int idx = part_id + i * NT;
-      if (idx < S::BLOCKS) {
+      if (mine && idx < S::BLOCKS) {
         const int row = (idx % (R / S::VR)) * S::VR, chunk = idx / (R / S::VR);
 #pragma unroll
         for (int r = 0; r < S::VR; ++r) out[chunk * R + row + r] = st.sum[i][r];
