@@ -11,7 +11,8 @@
 // 2^-26 of it on average - below the float32 rounding of the sum itself - while the bfloat16 cores run 16 times faster than the
 // float32 ones (dense peaks 2.5 PFLOP/s against 0.157): six products there cost less than half of one here.  A split of an infinity
 // (inf - inf) or of a value that rounds up to one is not a number: any non-finite sum is computed again, element by element, in plain
-// float32 (element_again), so infinities and NaN come out as in an ordinary float32 product.
+// float32 (element_again), so infinities and NaN come out as in an ordinary float32 product.  The matrix cores read a bfloat16 below 2^-133
+// as 0, so a factor below 2^-110 keeps an absolute 2^-133 instead of its last bits (float32 itself ends at 2^-149).
 //
 // Layout in LDS.  A tile holds chunks of 8 reduction values (16 bytes) - the operand of one MFMA lane - as
 // [part][chunk][row ^ ((row >> 3) & 7)], each chunk column padded: fragment reads are contiguous, and the writes of both staging forms
@@ -300,35 +301,47 @@ template <typename T, int BM, int BN, int WM, int WN> struct Accum {
   f32x16 acc[FM][FN];
 
   __device__ void clear() {
+    zero(acc);
+  }
+  // into: acc, or for split operands a sum of their own (add) - the six partial products of 16 reduction values, smallest first, so that
+  // the long sum rounds once for a whole step (added to it one by one, K = 4048 came out 1.0e-6 off where a float32 product is 0.6e-6)
+  __device__ static void products(f32x16 (&into)[FM][FN], const typename E::Frag (&a)[E::PARTS][FM], const typename E::Frag (&b)[E::PARTS][FN]) {
+    constexpr int NP = E::PARTS == 1 ? 1 : 6;
+    constexpr int PA[6] = {E::PARTS == 1 ? 0 : 2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) into[i][j] = E::mfma(a[PA[p]][i], b[PB[p]][j], into[i][j]);
+  }
+  static __device__ void zero(f32x16 (&t)[FM][FN]) {
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
       for (int j = 0; j < FN; ++j)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+        for (int e = 0; e < 16; ++e) t[i][j][e] = 0.0f;
   }
-  __device__ void products(const typename E::Frag (&a)[E::PARTS][FM], const typename E::Frag (&b)[E::PARTS][FN]) {
+  __device__ void add(const f32x16 (&t)[FM][FN]) {
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        if constexpr (E::PARTS == 1) {
-          acc[i][j] = E::mfma(a[0][i], b[0][j], acc[i][j]);
-        } else {
-          // the six partial products of 16 reduction values, smallest first, in a sum of their own: the long sum then rounds once for them
-          // (added to it one by one, K = 4048 came out 1.0e-6 off where a float32 product is 0.6e-6)
-          constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
-          f32x16 t;
+      for (int j = 0; j < FN; ++j)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) t[e] = 0.0f;
-#pragma unroll
-          for (int p = 0; p < 6; ++p) t = E::mfma(a[PA[p]][i], b[PB[p]][j], t);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[i][j][e] += t[e];
-        }
-      }
+        for (int e = 0; e < 16; ++e) acc[i][j][e] += t[i][j][e];
   }
   __device__ void step(const char *la, const char *lb, int wm, int wn, int lane) {
+    if constexpr (E::PARTS == 1) {
+      staged(acc, la, lb, wm, wn, lane);
+    } else {
+      f32x16 t[FM][FN];
+      zero(t);
+      staged(t, la, lb, wm, wn, lane);
+      add(t);
+    }
+  }
+  static __device__ void staged(f32x16 (&into)[FM][FN], const char *la, const char *lb, int wm, int wn, int lane) {
     using F = typename E::Frag;
     using LA = Tile<T, BM>;
     using LB = Tile<T, BN>;
@@ -343,7 +356,7 @@ template <typename T, int BM, int BN, int WM, int WN> struct Accum {
 #pragma unroll
         for (int j = 0; j < FN; ++j) b[p][j] = reinterpret_cast<const F *>(lb)[LB::slot(p, chunk, wn * (BN / WN) + j * 32 + lane % 32)];
       }
-      products(a, b);
+      products(into, a, b);
     }
   }
   // element e of a fragment: row 8 * (e / 4) + 4 * (lane / 32) + e % 4, column lane % 32
@@ -515,7 +528,7 @@ int64_t slots_of(int64_t rows, int64_t groups, bool with_ptr, int64_t unit) {
 }
 
 // Workgroups go to the 8 XCDs round robin; tiles that share an operand should share an L2: XCD x takes the x-th eighth of the tiles.
-// (32 bits from here to the tile: a launch has fewer than 2^31 workgroups, and a 64-bit division is some 140 instructions.)
+// (32 bits from here to the tile: a launch has fewer than 2^24 workgroups, and a 64-bit division is some 140 instructions.)
 __device__ inline uint32_t xcd_contiguous(uint32_t block, uint32_t blocks) {
   const uint32_t x = block % 8, q = blocks / 8, r = blocks % 8;
   return x * q + (x < r ? x : r) + block / 8;
@@ -915,6 +928,8 @@ template <typename T, int FM> __global__ __launch_bounds__(512, 2) void mm_few_r
         }
       }
     }
+    f32x16 t[FM][1];
+    if constexpr (E::PARTS == 3) acc.zero(t);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       F a[E::PARTS][FM], b[E::PARTS][1];
@@ -934,8 +949,10 @@ template <typename T, int FM> __global__ __launch_bounds__(512, 2) void mm_few_r
           for (int s = 0; s < 3; ++s) (i < FM ? a[s][i < FM ? i : 0] : b[s][0]) = p[s];
         }
       }
-      acc.products(a, b);
+      if constexpr (E::PARTS == 1) acc.products(acc.acc, a, b);
+      else acc.products(t, a, b);
     }
+    if constexpr (E::PARTS == 3) acc.add(t);
   }
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -994,7 +1011,7 @@ template <bool PAIR, int WHICH, typename A, typename B> __device__ inline auto &
 }
 // SUMS: column sums of nothing (0), p (1) or q (2) beside the product
 template <typename T, int BM, int BN, int WM, int WN, int SUMS>
-__global__ __launch_bounds__(64 * WM * WN, 3) void mm_weight_kernel(const WeightArgs g) {
+__global__ __launch_bounds__(64 * WM * WN, BM == 64 && BN == 64 ? 4 : 3) void mm_weight_kernel(const WeightArgs g) {
   using E = Elem<T>;
   using LA = Tile<T, BM>;
   using LB = Tile<T, BN>;
@@ -1230,7 +1247,7 @@ int launched(const char *name) {
   return GEOT_OK;
 }
 
-constexpr int64_t kMaxBlocks = ((int64_t)1 << 31) - 1;
+constexpr int64_t kMaxBlocks = (((int64_t)1 << 32) - 1) / 512; // (a launch holds fewer than 2^32 threads)
 
 // Reduction values of a workgroup: all of them (k) where the tiles fill the chip, or the reduction is short; else a share such that about
 // two workgroups a CU run, at least four steps each.  (17 rows x 4048 -> 144 f32 in 2 groups: 5 tiles of 127 steps were 192 us.)

@@ -302,6 +302,11 @@ def test_linear_float32_keeps_24_bits():
         if exact:
             assert torch.equal(got, want)
         assert bool(((got - want).abs() <= 2.0 ** -22 * want.abs()).all())
+    # a factor below 2^-110: its parts below the smallest bfloat16, 2^-133, are lost
+    for e in (-140, -127, -115, -100):
+        small = x / x.abs().clamp(min=1e-30) * 2.0 ** e * torch.linspace(1, 2, k, device="cuda")
+        err = (geot.linear(small, torch.eye(k, device="cuda") * 2.0 ** 30).double() - small.double() * 2.0 ** 30).abs()
+        assert bool((err <= 2.0 ** (30 - 133) + 2.0 ** -22 * 2.0 ** 30 * small.double().abs()).all())
 
 
 @gpu
