@@ -21,6 +21,9 @@ Ops in the dispatcher namespace ``geot`` (device key CUDA -- which is what a ROC
     geot::gather_scatter / geot::gather_weight_scatter / geot::csr_gws      (the differentiable ops: defined HERE, in
                                                                              Python, as in the reference; kernels in _C.so)
 
+Beside them, under ``geot_dense``, the operators on dense rows that stand around the aggregations in a layer and that the
+reference leaves to torch.nn: ``linear``, ``segment_matmul``, ``layer_norm`` (csrc/host_dense.cpp; public functions at the end).
+
 Deliberate differences (all documented in DESIGN.md):
 * the output row count still comes from ``index[-1] + 1``, read back from the device and checked on every call
   (part of the reference contract), but the read-back overlaps the kernels and the output is ``torch.empty``: the
