@@ -48,7 +48,7 @@ SYMBOLS = [
     "geot_csr_workspace_bytes", "geot_csr_gws", "geot_coo_to_csr",
     "geot_slab_units", "geot_slab_full_chip", "geot_slab_rows_per_group", "geot_slab_rows_per_group_dtype", "geot_slab_units_for", "geot_slab_rows_per_group_shape", "geot_slab_workspace_bytes", "geot_slab_workspace_bytes_staged", "geot_slab_spmm", "geot_slab_sddmm", "geot_slab_sddmm_staged", "geot_slab_mh_sddmm", "geot_slab_to_plan_order",
     "geot_slab_plan_scratch_bytes", "geot_slab_plan_rows", "geot_slab_plan_groups", "geot_slab_plan_edges",
-    "geot_linear", "geot_linear_keeps_preactivation", "geot_linear_grad_preactivation_workspace_bytes", "geot_linear_grad_preactivation",
+    "geot_linear", "geot_linear_workspace_bytes", "geot_linear_keeps_preactivation", "geot_linear_grad_preactivation_workspace_bytes", "geot_linear_grad_preactivation",
     "geot_linear_grad_input", "geot_linear_grad_input_workspace_bytes", "geot_segment_matmul_workspace_bytes", "geot_segment_matmul_grad_input_workspace_bytes",
     "geot_linear_grad_weight_workspace_bytes", "geot_linear_grad_weight",
     "geot_segment_matmul", "geot_segment_matmul_grad_input", "geot_segment_matmul_grad_weight_workspace_bytes", "geot_segment_matmul_grad_weight",
@@ -272,7 +272,9 @@ def load() -> ctypes.CDLL:
     L.geot_slab_to_plan_order.argtypes = [ctypes.POINTER(SlabPlan), c_vp, c_vp, c_i64, c_int, c_vp]
     L.geot_slab_mh_sddmm.argtypes = [ctypes.POINTER(SlabPlan), c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_int, c_vp, c_sz, c_vp]
     c_f = ctypes.c_float
-    L.geot_linear.argtypes = [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_int, c_vp]
+    L.geot_linear_workspace_bytes.restype = c_sz
+    L.geot_linear_workspace_bytes.argtypes = [c_i64, c_i64, c_i64, c_int]
+    L.geot_linear.argtypes = [c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_int, c_vp, c_sz, c_vp]
     L.geot_linear_keeps_preactivation.argtypes = [c_i64, c_int, c_int, c_int]
     L.geot_linear_grad_preactivation_workspace_bytes.restype = c_sz
     L.geot_linear_grad_preactivation_workspace_bytes.argtypes = [c_i64, c_i64]

@@ -801,8 +801,7 @@ __global__ __launch_bounds__(64 * WM * WN, NBUF == 1 ? 3 : 2) void mm_rows_kerne
   });
 }
 
-// The shares of the reduction, added in their order, and what becomes of a row's sums (no activation or residual: linear splits inside a
-// workgroup, mm_few_rows_kernel).  One wave a row of a tile of 128 rows.
+// The shares of the reduction, added in their order, and what becomes of a row's sums.  A workgroup takes a quarter of a tile's rows.
 template <typename T, int BN, bool BR> __global__ __launch_bounds__(kThreads) void mm_rows_join_kernel(const RowsArgs g, uint32_t shares) {
   constexpr int V = 16 / sizeof(T), TPR = BN / V, RPP = kThreads / TPR;
   const uint32_t slot = blockIdx.x / g.tiles_n, tile = blockIdx.x % g.tiles_n;
@@ -818,31 +817,35 @@ template <typename T, int BN, bool BR> __global__ __launch_bounds__(kThreads) vo
 #pragma unroll
   for (int v = 0; v < V; ++v)
     bias[v] = g.bias && real && v < cols ? as_float(static_cast<const T *>(g.bias)[piece.group * g.bias_group + nc + v]) : 0.0f;
-  for (int64_t row = r0 + threadIdx.x / TPR + (int64_t)blockIdx.y * RPP; row < end; row += (int64_t)gridDim.y * RPP) {
-    float v[V];
+  by_activation(g.act, [&](auto act) {
+    for (int64_t row = r0 + threadIdx.x / TPR + (int64_t)blockIdx.y * RPP; row < end; row += (int64_t)gridDim.y * RPP) {
+      float v[V];
 #pragma unroll
-    for (int c = 0; c < V; ++c) v[c] = 0.0f;
-    if (real) {
+      for (int c = 0; c < V; ++c) v[c] = 0.0f;
+      if (real) {
 #pragma unroll 4
-      for (uint32_t s = 0; s < shares; ++s) {
-        const float *p = g.part + ((int64_t)s * g.groups.rows + row) * g.n + nc;
+        for (uint32_t s = 0; s < shares; ++s) {
+          const float *p = g.part + ((int64_t)s * g.groups.rows + row) * g.n + nc;
 #pragma unroll
-        for (int c = 0; c < V; c += 4) {
-          const u32x4 q = load_cols<float, 4>(p + c, cols - c < 4 ? (cols > c ? cols - c : 0) : 4);
+          for (int c = 0; c < V; c += 4) {
+            const u32x4 q = load_cols<float, 4>(p + c, cols - c < 4 ? (cols > c ? cols - c : 0) : 4);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[c + e] += __uint_as_float(q[e]);
+            for (int e = 0; e < 4; ++e) v[c + e] += __uint_as_float(q[e]);
+          }
+        }
+        if constexpr (Elem<T>::PARTS == 3) {
+          const float *B = static_cast<const float *>(g.b) + piece.group * g.b_group;
+#pragma unroll
+          for (int c = 0; c < V; ++c)
+            if (!finite(v[c]) && c < cols)
+              v[c] = element_again(static_cast<const float *>(g.a) + row * g.lda, 1, B + (BR ? nc + c : (nc + c) * g.ldb), BR ? g.ldb : 1, g.k);
         }
       }
-      if constexpr (Elem<T>::PARTS == 3) {
-        const float *B = static_cast<const float *>(g.b) + piece.group * g.b_group;
-#pragma unroll
-        for (int c = 0; c < V; ++c)
-          if (!finite(v[c]) && c < cols)
-            v[c] = element_again(static_cast<const float *>(g.a) + row * g.lda, 1, B + (BR ? nc + c : (nc + c) * g.ldb), BR ? g.ldb : 1, g.k);
-      }
+      u32x4 ext = {0, 0, 0, 0};
+      if (g.residual) ext = load_cols<T, V>(static_cast<const T *>(g.residual) + row * g.ldr + nc, cols);
+      finish_row<T, V, decltype(act)::value, false>(g, row, nc, cols, v, bias, g.residual != nullptr, ext, none);
     }
-    finish_row<T, V, GEOT_ACT_NONE, false>(g, row, nc, cols, v, bias, false, u32x4{0, 0, 0, 0}, none);
-  }
+  });
 }
 
 // dz = dy act'(z) with z = x W^T + b computed again instead of read: narrow layers are bound by memory, and z costs a write in the forward
@@ -1135,7 +1138,8 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 && BN == 64 ? 4 : 3) void mm
 }
 
 // The chunks of a group, added in their order by 16 threads an element (each every 16th chunk, then the 16 by halves).
-template <typename T> __global__ __launch_bounds__(kThreads) void mm_join_kernel(const WeightArgs g) {
+// WAYS 1: at most 16 chunks, one thread an element (300 rows, 4096 -> 256: 15 of the 16 threads had nothing to add).
+template <typename T, int WAYS> __global__ __launch_bounds__(kThreads) void mm_join_kernel(const WeightArgs g) {
   __shared__ float part[kThreads];
   const int64_t group = blockIdx.y;
   Piece piece;
@@ -1148,26 +1152,30 @@ template <typename T> __global__ __launch_bounds__(kThreads) void mm_join_kernel
   if (len <= g.unit) return;
   const int64_t chunks = (len + g.unit - 1) / g.unit;
   const int64_t size = g.np * g.nq, per_slot = size + (g.colsum ? g.ns : 0);
-  const int lane = threadIdx.x % 16, way = threadIdx.x / 16;
-  for (int64_t base = (int64_t)blockIdx.x * 16; base < per_slot; base += (int64_t)gridDim.x * 16) {
+  constexpr int LANES = kThreads / WAYS;
+  const int lane = threadIdx.x % LANES, way = threadIdx.x / LANES;
+  for (int64_t base = (int64_t)blockIdx.x * LANES; base < per_slot; base += (int64_t)gridDim.x * LANES) {
     const int64_t i = base + lane;
     float s = 0.0f;
     if (i < per_slot) {
 #pragma unroll 4
-      for (int64_t c = way; c < chunks; c += 16) s += g.part[(piece.start + c) * per_slot + i];
+      for (int64_t c = way; c < chunks; c += WAYS) s += g.part[(piece.start + c) * per_slot + i];
     }
-    part[threadIdx.x] = s;
-    __syncthreads();
+    if constexpr (WAYS > 1) {
+      part[threadIdx.x] = s;
+      __syncthreads();
 #pragma unroll
-    for (int h = 128; h >= 16; h /= 2) {
-      if ((int)threadIdx.x < h) part[threadIdx.x] += part[threadIdx.x + h];
+      for (int h = kThreads / 2; h >= LANES; h /= 2) {
+        if ((int)threadIdx.x < h) part[threadIdx.x] += part[threadIdx.x + h];
+        __syncthreads();
+      }
+      s = part[lane];
       __syncthreads();
     }
     if (way == 0 && i < per_slot) {
-      if (i < size) static_cast<T *>(g.out)[group * size + i] = (T)part[lane];
-      else static_cast<T *>(g.colsum)[group * g.ns + i - size] = (T)part[lane];
+      if (i < size) static_cast<T *>(g.out)[group * size + i] = (T)s;
+      else static_cast<T *>(g.colsum)[group * g.ns + i - size] = (T)s;
     }
-    __syncthreads();
   }
 }
 
@@ -1297,10 +1305,15 @@ template <typename T, int FM> int run_few(RowsArgs &g, hipStream_t st) {
   hipLaunchKernelGGL((mm_few_rows_kernel<T, FM>), dim3((unsigned)(tiles_m * g.tiles_n)), dim3(512), 0, st, g);
   return launched("mm_few_rows_kernel");
 }
+// Few tiles and a reduction that eight waves of a workgroup walk in a few steps; a longer one of more than 32 rows is split over
+// workgroups instead (bf16: 100 x 1000 -> 1000 takes 7.9 us so and 15.6 split, 300 x 4096 -> 256 23.6 and 9.5).
+bool takes_few_rows(int64_t rows, bool with_ptr, int64_t n, int64_t k) {
+  return !with_ptr && ((rows + 127) / 128) * ((n + 127) / 128) < 128 && k >= 128 && (rows <= 32 || k <= 2048);
+}
 template <typename T, bool BR> int rows_typed(RowsArgs &g, hipStream_t st) {
   const int64_t tiles = ((g.groups.rows + 127) / 128) * ((g.n + 127) / 128);
-  if constexpr (!BR) {
-    if (!g.groups.ptr && tiles < 128 && g.k >= 128) return g.groups.rows <= 32 ? run_few<T, 1>(g, st) : run_few<T, 2>(g, st);
+  if constexpr (!BR) { // (segment_matmul's gradient comes here too, with groups)
+    if (takes_few_rows(g.groups.rows, g.groups.ptr != nullptr, g.n, g.k)) return g.groups.rows <= 32 ? run_few<T, 1>(g, st) : run_few<T, 2>(g, st);
   }
   // (split operands: two column fragments a wave and their six parts do not fit the registers of three workgroups a CU)
   if (Elem<T>::PARTS == 3 || g.n <= 64) return run_rows<T, 128, 64, 2, 2, BR, 1>(g, st);
@@ -1310,14 +1323,12 @@ template <typename T, bool BR> int rows_typed(RowsArgs &g, hipStream_t st) {
     return run_rows<T, 128, 128, 2, 2, BR, 1>(g, st);
   }
 }
-// (workspace: of the products that may split their reduction over workgroups)
-int rows_product(RowsArgs &g, bool br, int dtype, hipStream_t st, bool may_split = false, void *workspace = nullptr, size_t workspace_bytes = 0) {
+int rows_product(RowsArgs &g, bool br, int dtype, hipStream_t st, void *workspace, size_t workspace_bytes) {
   if (g.groups.rows == 0 || g.n == 0) return GEOT_OK;
-  if (may_split) {
-    const size_t need = rows_workspace(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, g.n, g.k, dtype);
-    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return geot_internal_fail(GEOT_EWORKSPACE, "rows product: workspace too small or misaligned");
-    g.part = need ? static_cast<float *>(workspace) : nullptr;
-  }
+  const bool few = !br && takes_few_rows(g.groups.rows, g.groups.ptr != nullptr, g.n, g.k);
+  const size_t need = few ? 0 : rows_workspace(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, g.n, g.k, dtype);
+  if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return geot_internal_fail(GEOT_EWORKSPACE, "rows product: workspace too small or misaligned");
+  g.part = need ? static_cast<float *>(workspace) : nullptr;
   switch (dtype) {
   case GEOT_F32: return br ? rows_typed<float, true>(g, st) : rows_typed<float, false>(g, st);
   case GEOT_F16: return br ? rows_typed<f16, true>(g, st) : rows_typed<f16, false>(g, st);
@@ -1411,12 +1422,15 @@ template <typename T, int BM, int BN, int WM, int WN> int run_weight(WeightArgs 
   else hipLaunchKernelGGL((mm_weight_kernel<T, BM, BN, WM, WN, 2>), grid, block, 0, st, g);
   if (const int rc = launched("mm_weight_kernel")) return rc;
   if (g.groups.rows > g.unit) { // some group may have several chunks
-    const int64_t per = (g.np * g.nq + (g.colsum ? g.ns : 0) + 15) / 16;
+    const bool few = g.groups.rows <= 16 * g.unit;
+    const int64_t lanes = few ? kThreads : 16, per = (g.np * g.nq + (g.colsum ? g.ns : 0) + lanes - 1) / lanes;
     // (which groups have several chunks only the device knows: few workgroups a group when there are many - 2048 each cost 50 us at 64
     // groups of one chunk)
     int64_t wide = 8192 / g.groups.groups;
     wide = wide < 32 ? 32 : wide > 2048 ? 2048 : wide;
-    hipLaunchKernelGGL((mm_join_kernel<T>), dim3((unsigned)(per < wide ? per : wide), (unsigned)g.groups.groups), dim3(kThreads), 0, st, g);
+    const dim3 join((unsigned)(per < wide ? per : wide), (unsigned)g.groups.groups);
+    if (few) hipLaunchKernelGGL((mm_join_kernel<T, 1>), join, dim3(kThreads), 0, st, g);
+    else hipLaunchKernelGGL((mm_join_kernel<T, 16>), join, dim3(kThreads), 0, st, g);
     return launched(nullptr);
   }
   return GEOT_OK;
@@ -1457,15 +1471,19 @@ bool bad_size(int64_t a, int64_t b, int64_t c) {
 
 extern "C" {
 
+size_t geot_linear_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype) {
+  return bad_size(rows, in, out) || takes_few_rows(rows, false, out, in) ? 0 : rows_workspace(rows, 1, false, out, in, dtype);
+}
+
 int geot_linear(const void *x, int64_t ldx, const void *weight, const void *bias, const void *residual, int64_t ld_residual, void *z, void *y,
-                int64_t rows, int64_t in, int64_t out, int activation, int dtype, void *stream) {
+                int64_t rows, int64_t in, int64_t out, int activation, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
   if (bad_size(rows, in, out) || ldx < 0 || ld_residual < 0) return geot_internal_fail(GEOT_EINVAL, "geot_linear: negative size");
   if (activation < GEOT_ACT_NONE || activation > GEOT_ACT_SILU) return geot_internal_fail(GEOT_EINVAL, "geot_linear: unknown activation");
   if (rows > 0 && out > 0 && (!y || (in > 0 && (!x || !weight)))) return geot_internal_fail(GEOT_EINVAL, "geot_linear: null pointer");
   RowsArgs g{};
   g.a = x; g.lda = ldx; g.b = weight; g.ldb = in; g.bias = bias; g.residual = residual; g.ldr = ld_residual; g.z = z; g.y = y; g.ldy = out;
   g.groups = {nullptr, 1, rows}; g.n = out; g.k = in; g.act = activation;
-  return rows_product(g, false, dtype, static_cast<hipStream_t>(stream));
+  return rows_product(g, false, dtype, static_cast<hipStream_t>(stream), workspace, workspace_bytes);
 }
 
 size_t geot_linear_grad_input_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype) {
@@ -1479,7 +1497,7 @@ int geot_linear_grad_input(const void *dz, const void *weight, void *dx, int64_t
   RowsArgs g{};
   g.a = dz; g.lda = out; g.b = weight; g.ldb = in; g.y = dx; g.ldy = in;
   g.groups = {nullptr, 1, rows}; g.n = in; g.k = out; g.act = GEOT_ACT_NONE;
-  return rows_product(g, true, dtype, static_cast<hipStream_t>(stream), true, workspace, workspace_bytes);
+  return rows_product(g, true, dtype, static_cast<hipStream_t>(stream), workspace, workspace_bytes);
 }
 
 size_t geot_linear_grad_weight_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype) {
@@ -1539,7 +1557,7 @@ int geot_segment_matmul(const void *x, int64_t ldx, const int64_t *ptr, const vo
   RowsArgs g{};
   g.a = x; g.lda = ldx; g.b = weight; g.ldb = out; g.b_group = in * out; g.bias = bias; g.bias_group = out; g.y = y; g.ldy = out;
   g.groups = {ptr, groups, rows}; g.n = out; g.k = in; g.act = GEOT_ACT_NONE;
-  return rows_product(g, true, dtype, static_cast<hipStream_t>(stream), true, workspace, workspace_bytes);
+  return rows_product(g, true, dtype, static_cast<hipStream_t>(stream), workspace, workspace_bytes);
 }
 
 size_t geot_segment_matmul_grad_input_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype) {
@@ -1553,7 +1571,7 @@ int geot_segment_matmul_grad_input(const void *dy, const int64_t *ptr, const voi
   RowsArgs g{};
   g.a = dy; g.lda = out; g.b = weight; g.ldb = out; g.b_group = in * out; g.y = dx; g.ldy = in;
   g.groups = {ptr, groups, rows}; g.n = in; g.k = out; g.act = GEOT_ACT_NONE;
-  return rows_product(g, false, dtype, static_cast<hipStream_t>(stream), true, workspace, workspace_bytes);
+  return rows_product(g, false, dtype, static_cast<hipStream_t>(stream), workspace, workspace_bytes);
 }
 
 size_t geot_segment_matmul_grad_weight_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype) {

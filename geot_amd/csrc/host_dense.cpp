@@ -96,8 +96,9 @@ std::tuple<at::Tensor, at::Tensor> linear_forward_op(const at::Tensor &x_in, con
   at::Tensor z = keep ? at::empty_like(y) : at::empty({0}, x_in.options());
   Rows r{at::Tensor(), 0, 0};
   if (given(residual_in)) r = as_rows(*residual_in);
+  const at::Tensor ws = scratch(x_in, geot_linear_workspace_bytes(x.rows, in, out, dt));
   GEOT_CALL(geot_linear(x.t.data_ptr(), x.ld, w.data_ptr(), data_of(bias), r.t.defined() ? r.t.data_ptr() : nullptr, r.ld, keep ? z.data_ptr() : nullptr,
-                        y.data_ptr(), x.rows, in, out, act, dt, stream_of(x_in)));
+                        y.data_ptr(), x.rows, in, out, act, dt, ws.data_ptr(), ws.numel(), stream_of(x_in)));
   return std::make_tuple(y, z);
 }
 std::tuple<at::Tensor, at::Tensor> linear_train_op(const at::Tensor &x, const at::Tensor &w, const c10::optional<at::Tensor> &bias,

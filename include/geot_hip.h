@@ -388,11 +388,16 @@ int geot_slab_mh_sddmm(const geot_slab_plan *plan, const void *mat_1, const void
  * element's.  No call allocates or synchronises; results do not depend on the launch (no atomics).  float32 products are exact to about
  * 2^-23 of |xy| each (computed on the bfloat16 cores in three parts); a factor below 2^-110 keeps an absolute 2^-133.
  *
+ * Workspaces: ..._workspace_bytes of the call (0 where it needs none - products of few tiles split their reduction over workgroups), 16-byte
+ * aligned, no content expected, free after the call.
+ *
  * geot_linear:  y = act(x weight^T + bias) + residual     x [rows, in], weight [out, in], bias [out] or NULL, residual [rows, out] or
  * NULL, y [rows, out]; z [rows, out] or NULL receives x weight^T + bias (what the backward pass of the activation needs). */
 enum { GEOT_ACT_NONE = 0, GEOT_ACT_RELU = 1, GEOT_ACT_GELU = 2 /* z * Phi(z), the error-function form */, GEOT_ACT_SILU = 3 };
+size_t geot_linear_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype);
 int geot_linear(const void *x, int64_t ldx, const void *weight, const void *bias, const void *residual, int64_t ld_residual, void *z,
-                void *y, int64_t rows, int64_t in, int64_t out, int activation, int dtype, void *stream);
+                void *y, int64_t rows, int64_t in, int64_t out, int activation, int dtype, void *workspace, size_t workspace_bytes,
+                void *stream);
 /* dz = dy act'(z) [rows, out], and the bias's gradient dbias = column sums of dz (before its rounding) [out] or NULL.  z: what geot_linear
  * wrote, or y for relu without a residual (they have one sign), or NULL: computed again from x, weight and bias - what
  * geot_linear_keeps_preactivation says (0: do not keep z) for layers where that moves fewer bytes.  dz may be dy when z is given.
@@ -402,8 +407,7 @@ size_t geot_linear_grad_preactivation_workspace_bytes(int64_t rows, int64_t out)
 int geot_linear_grad_preactivation(const void *dy, const void *z, const void *x, int64_t ldx, const void *weight, const void *bias, void *dz,
                                    void *dbias, int64_t rows, int64_t in, int64_t out, int activation, int dtype, void *workspace,
                                    size_t workspace_bytes, void *stream);
-/* dx = dz weight   [rows, in].  Products of few tiles split their reduction over workgroups; workspaces of these calls: ..._workspace_bytes
- * (0 where none is needed), 16-byte aligned, no content expected, free after the call. */
+/* dx = dz weight   [rows, in] */
 size_t geot_linear_grad_input_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype);
 int geot_linear_grad_input(const void *dz, const void *weight, void *dx, int64_t rows, int64_t in, int64_t out, int dtype, void *workspace,
                            size_t workspace_bytes, void *stream);

@@ -98,7 +98,7 @@ class LinearReference:
 
 
 LINEAR_SHAPES = [(1, 1, 1), (5, 16, 32), (1, 520, 96), (3, 64, 1000), (128, 128, 128), (129, 65, 33), (300, 602, 256), (257, 64, 130), (64, 200, 72),
-                 (200, 7, 128), (1000, 33, 64), (31, 1024, 40), (2, 120, 1990)]
+                 (200, 7, 128), (1000, 33, 64), (31, 1024, 40), (2, 120, 1990), (70, 4100, 48), (700, 24, 80)]
 
 
 # ---- refusals: no GPU needed ------------------------------------------------------------------------------------------------------
@@ -152,10 +152,10 @@ def test_refused_abi_calls():
     """What the C ABI refuses before it touches anything."""
     L = geot._lib.load()
     einval, eworkspace, eunsupported = -1, -2, -4
-    assert L.geot_linear(None, 4, None, None, None, 0, None, None, -1, 4, 4, 0, 0, None) == einval
-    assert L.geot_linear(None, 4, None, None, None, 0, None, None, 2, 4, 4, 0, 0, None) == einval
-    assert L.geot_linear(None, 4, None, None, None, 0, None, None, 0, 4, 4, 9, 0, None) == einval
-    assert L.geot_linear(16, 4, 16, None, None, 0, None, 16, 2, 4, 4, 0, 1, None) == eunsupported       # (float64: refused before any launch)
+    assert L.geot_linear(None, 4, None, None, None, 0, None, None, -1, 4, 4, 0, 0, None, 0, None) == einval
+    assert L.geot_linear(None, 4, None, None, None, 0, None, None, 2, 4, 4, 0, 0, None, 0, None) == einval
+    assert L.geot_linear(None, 4, None, None, None, 0, None, None, 0, 4, 4, 9, 0, None, 0, None) == einval
+    assert L.geot_linear(16, 4, 16, None, None, 0, None, 16, 2, 4, 4, 0, 1, None, 0, None) == eunsupported       # (float64: refused before any launch)
     assert L.geot_segment_matmul(16, 4, 16, 16, None, 16, 2, 65536, 4, 4, 0, None, 0, None) == einval
     need = L.geot_segment_matmul_workspace_bytes(17, 2, 4096, 128, 0)
     assert need > 0 and L.geot_segment_matmul_workspace_bytes(1_000_000, 2, 4096, 128, 0) == 0
