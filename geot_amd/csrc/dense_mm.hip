@@ -676,7 +676,7 @@ __device__ inline void finish_row(const RowsArgs &g, int64_t row, int64_t col, i
 }
 
 // A finished tile: 32 * WM rows at a time through LDS, so that every access to memory is whole rows, V consecutive columns a thread.  What
-// is read beside the sums (the residual, dy) is on its way before the barriers.  a_row(r) / b_col(c): the operands of element_again.
+// is read beside the sums (the residual, dy) is on its way before the barriers.  g.a and B: the operands of element_again.
 template <typename T, int BM, int BN, int WM, int WN, int ACT, bool DZ, bool BR>
 __device__ inline void tile_epilogue(const RowsArgs &g, const Accum<T, BM, BN, WM, WN> &acc, float *out, const T *ext, int64_t ld_ext, const T *B, int64_t r0, int64_t rows,
                                      int64_t nc, int cols, int64_t k_len, const float (&bias)[16 / sizeof(T)], float (&sum)[16 / sizeof(T)], int tid, int wm, int wn, int lane) {
