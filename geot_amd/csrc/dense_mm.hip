@@ -385,6 +385,9 @@ __device__ float element_again(const float *a, int64_t stride_a, const float *b,
 }
 __device__ inline bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 
+// max(z, 0) as a half sum: +inf and NaN stay, -inf becomes NaN (as -inf * 0 does)
+__device__ inline float positive_part(float z) { return fmaf(0.5f, fabsf(z), 0.5f * z); }
+
 // The normal distribution's tail, Phi(-a) = exp(-a^2 / 2) R(a) for a >= 0: R is smooth (Mills' ratio times the density's constant) and
 // is taken as a polynomial in t = 1 / (1 + 0.26 a), fitted by least squares reweighted to equal ripple on [0, 14.2] (3e-8; 4e-7 with its
 // float32 rounding).  The same exponential serves the density in the slope.  erfcf + expf instead bound the kernels by their vector
@@ -393,7 +396,7 @@ struct Normal {
   float tail, bell; // Phi(-|z|), exp(-z^2 / 2)
 };
 __device__ inline Normal normal_of(float z) {
-  // (exp(-200) is 0 in float32, nothing changes behind 20 but inf - inf below; a NaN goes on in z)
+  // (exp(-200) is 0 in float32, nothing changes behind 20 but inf - inf below; a NaN goes on in the caller's z)
   const float a = fminf(fabsf(z), 20.0f);
   const float t = __builtin_amdgcn_rcpf(fmaf(0.26f, a, 1.0f));
   constexpr float half_log2e = 0.72134752044448170f;
@@ -425,8 +428,7 @@ __device__ inline float gelu16(float z) {
   p = fmaf(p, a, 0.45959118008613586f);
   p = fmaf(p, a, 1.1508647203445435f);
   p = fmaf(p, a, 1.0f);
-  // max(z, 0) - a Phi(-a), the maximum as a half sum: NaN stays
-  return fmaf(-a, __builtin_amdgcn_exp2f(-p), fmaf(0.5f, fabsf(z), 0.5f * z));
+  return fmaf(-a, __builtin_amdgcn_exp2f(-p), positive_part(z)); // max(z, 0) - a Phi(-a)
 }
 // gelu'(-a) = exp(-a^2 / 2) (R(a) - a / sqrt(2 pi)), gelu'(z) + gelu'(-z) = 1: degree 7 in a, 2.4e-5 (2^-15.3) absolute
 __device__ inline float gelu_slope16(float z) {
@@ -453,12 +455,12 @@ template <bool EXACT> __device__ inline float logistic(float z) {
   return __builtin_amdgcn_rcpf(1.0f + e);
 }
 // ACT is a compile-time choice inside the loops over elements.  T: float operands take the exact forms.
+// At the infinities: values as the formula gives them (z Phi(z), z / (1 + exp(-z)): +inf, and NaN at -inf).
 template <typename T, int ACT> __device__ inline float activate(float z) {
   if constexpr (ACT == GEOT_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
   else if constexpr (ACT == GEOT_ACT_GELU && sizeof(T) == 2) return gelu16(z);
-  else if constexpr (ACT == GEOT_ACT_GELU) { // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
-    const float y = fmaf(-fabsf(z), normal_of(z).tail, fmaxf(z, 0.0f));
-    return z != z ? z : y;
+  else if constexpr (ACT == GEOT_ACT_GELU) { // z Phi(z) = max(z, 0) - |z| Phi(-|z|); behind 20 the tail is 0, and no infinity may meet it
+    return fmaf(-fminf(fabsf(z), 20.0f), normal_of(z).tail, positive_part(z));
   }
   else if constexpr (ACT == GEOT_ACT_SILU) return z * logistic<sizeof(T) == 4>(z);
   else return z;

@@ -1,0 +1,64 @@
+"""linear, segment_matmul and layer_norm at values and on paths where single numbers matter: infinities, tails, masked places, every kernel.
+
+Tolerances count roundings: u = half a step of the dtype, 2^-23 a step of a float32 sum.
+"""
+import pytest
+import torch
+
+import geot_amd as geot
+
+gpu = pytest.mark.gpu
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+IDS = ["f32", "f16", "bf16"]
+INF, NAN = float("inf"), float("nan")
+# rows, in, out of a product and the kernel it takes: 128-row tiles, few rows (narrow: z computed again in the backward pass; wide: z
+# kept), a reduction split over workgroups
+PATHS = {"tile": (200, 64, 72), "few": (33, 128, 40), "few-kept": (20, 512, 40), "split": (100, 4160, 48)}
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def act64(z, name):
+    if name == "relu":
+        return torch.relu(z)
+    return z * (torch.special.ndtr(z) if name == "gelu" else torch.sigmoid(z)) if name != "none" else z
+
+
+def through_linear(z, path, act):
+    """act(z) of a column of values that the product hands through unchanged: one weight is 1 (two, where z is a pair's sum),
+    the rest is 0."""
+    m, k, n = PATHS[path]
+    rows = z.shape[0]
+    x = torch.zeros(m, k, dtype=z.dtype, device=z.device)
+    x[:rows, :z.shape[1]] = z
+    w = torch.zeros(n, k, dtype=z.dtype, device=z.device)
+    w[:, :z.shape[1]] = 1
+    with torch.no_grad():
+        y = geot.linear(x, w, activation=act)
+    x.requires_grad_()
+    yt = geot.linear(x, w, activation=act)
+    assert torch.equal(yt.nan_to_num(7.0), y.nan_to_num(7.0))
+    assert bool((y[:rows] == y[:rows, :1]).logical_or(torch.isnan(y[:rows, :1])).all())
+    return y[:rows, 0]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("path", PATHS)
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+def test_activations_at_infinities(act, path, dtype):
+    """Infinities, NaN and sums that pass the dtype's range: values as the formula gives them."""
+    big = 60000.0 if dtype == torch.float16 else 1e38
+    pairs = [(INF, 0), (-INF, 0), (NAN, 0), (0.0, 0), (2, 0), (-2, 0), (30, 0), (-30, 0), (1e4, 0), (-1e4, 0), (big, 0), (-big, 0), (big, big), (-big, -big)]
+    z = torch.tensor(pairs, dtype=dtype, device="cuda")
+    y = through_linear(z, path, act)
+    total = z.double().sum(1)
+    want = act64(total, act)
+    over = want.abs() > torch.finfo(dtype).max               # (rounds to an infinity)
+    want = torch.where(over, want.sign() * INF, want)
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.isinf(y), torch.isinf(want)), (y, want)
+    fine = torch.isfinite(want)
+    tol = (half_step(dtype) + 2.0 ** -15) * want.abs() + torch.finfo(dtype).tiny
+    assert bool(((y.double() - want).abs() <= tol)[fine].all()), (y, want)
