@@ -455,7 +455,8 @@ template <bool EXACT> __device__ inline float logistic(float z) {
   return __builtin_amdgcn_rcpf(1.0f + e);
 }
 // ACT is a compile-time choice inside the loops over elements.  T: float operands take the exact forms.
-// At the infinities: values as the formula gives them (z Phi(z), z / (1 + exp(-z)): +inf, and NaN at -inf).
+// At the infinities: values as the formula gives them (z Phi(z), z / (1 + exp(-z)): +inf, and NaN at -inf), slopes as their limits (1 and 0) -
+// a z saved in float16 is infinite from 65520 on, where the value that was passed on can be an ordinary 0.
 template <typename T, int ACT> __device__ inline float activate(float z) {
   if constexpr (ACT == GEOT_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
   else if constexpr (ACT == GEOT_ACT_GELU && sizeof(T) == 2) return gelu16(z);
@@ -470,10 +471,11 @@ template <typename T, int ACT> __device__ inline float activation_slope(float z)
   else if constexpr (ACT == GEOT_ACT_GELU && sizeof(T) == 2) return gelu_slope16(z);
   else if constexpr (ACT == GEOT_ACT_GELU) {
     const Normal n = normal_of(z);
-    return fmaf(z * 0.39894228040143268f, n.bell, z < 0.0f ? n.tail : 1.0f - n.tail);
+    const float c = fminf(fmaxf(z, -20.0f), 20.0f), s = fmaf(c * 0.39894228040143268f, n.bell, z < 0.0f ? n.tail : 1.0f - n.tail);
+    return z != z ? z : s;
   } else if constexpr (ACT == GEOT_ACT_SILU) {
-    const float s = logistic<sizeof(T) == 4>(z);
-    return s * fmaf(z, 1.0f - s, 1.0f);
+    const float s = logistic<sizeof(T) == 4>(z), c = fminf(fmaxf(z, -128.0f), 128.0f); // (s is 0 or 1 behind; a NaN stays in s)
+    return s * fmaf(c, 1.0f - s, 1.0f);
   } else return 1.0f;
 }
 template <int V> using Const = std::integral_constant<int, V>;

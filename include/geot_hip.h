@@ -394,7 +394,7 @@ int geot_slab_mh_sddmm(const geot_slab_plan *plan, const void *mat_1, const void
  * geot_linear:  y = act(x weight^T + bias) + residual     x [rows, in], weight [out, in], bias [out] or NULL, residual [rows, out] or
  * NULL, y [rows, out]; z [rows, out] or NULL receives x weight^T + bias (what the backward pass of the activation needs). */
 /* Activations at the infinities: relu(-inf) = 0, gelu(-inf) and silu(-inf) are NaN (z Phi(z), z / (1 + exp(-z)) in ordinary arithmetic),
- * all three are +inf at +inf. */
+ * all three are +inf at +inf; their slopes there are the limits, 0 and 1. */
 enum { GEOT_ACT_NONE = 0, GEOT_ACT_RELU = 1, GEOT_ACT_GELU = 2 /* z * Phi(z), the error-function form */, GEOT_ACT_SILU = 3 };
 size_t geot_linear_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype);
 int geot_linear(const void *x, int64_t ldx, const void *weight, const void *bias, const void *residual, int64_t ld_residual, void *z,

@@ -2,6 +2,8 @@
 
 Tolerances count roundings: u = half a step of the dtype, 2^-23 a step of a float32 sum.
 """
+import math
+
 import pytest
 import torch
 
@@ -26,9 +28,21 @@ def act64(z, name):
     return z * (torch.special.ndtr(z) if name == "gelu" else torch.sigmoid(z)) if name != "none" else z
 
 
+def slope64(z, name):
+    """With the limits 0 and 1 at the infinities."""
+    c = z.clamp(-1000, 1000)
+    if name == "relu":
+        s = (z > 0).double()
+    elif name == "gelu":
+        s = torch.special.ndtr(c) + c * torch.exp(-c * c / 2) / math.sqrt(2 * math.pi)
+    else:
+        s = torch.sigmoid(c) * (1 + c * torch.sigmoid(-c))
+    return torch.where(torch.isnan(z), z, s)
+
+
 def through_linear(z, path, act):
-    """act(z) of a column of values that the product hands through unchanged: one weight is 1 (two, where z is a pair's sum),
-    the rest is 0."""
+    """act(z) and act'(z) of a column of values that the product hands through unchanged: one weight is 1 (two, where z is a pair's sum),
+    the rest is 0, and one output's gradient is 1."""
     m, k, n = PATHS[path]
     rows = z.shape[0]
     x = torch.zeros(m, k, dtype=z.dtype, device=z.device)
@@ -40,8 +54,11 @@ def through_linear(z, path, act):
     x.requires_grad_()
     yt = geot.linear(x, w, activation=act)
     assert torch.equal(yt.nan_to_num(7.0), y.nan_to_num(7.0))
+    dy = torch.zeros(m, n, dtype=z.dtype, device=z.device)
+    dy[:, 3] = 1
+    (dx,) = torch.autograd.grad(yt, [x], dy)
     assert bool((y[:rows] == y[:rows, :1]).logical_or(torch.isnan(y[:rows, :1])).all())
-    return y[:rows, 0]
+    return y[:rows, 0], dx[:rows, 0]
 
 
 @gpu
@@ -49,11 +66,11 @@ def through_linear(z, path, act):
 @pytest.mark.parametrize("path", PATHS)
 @pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
 def test_activations_at_infinities(act, path, dtype):
-    """Infinities, NaN and sums that pass the dtype's range: values as the formula gives them."""
+    """Infinities, NaN and sums that pass the dtype's range: values as the formula gives them, slopes by their limits."""
     big = 60000.0 if dtype == torch.float16 else 1e38
     pairs = [(INF, 0), (-INF, 0), (NAN, 0), (0.0, 0), (2, 0), (-2, 0), (30, 0), (-30, 0), (1e4, 0), (-1e4, 0), (big, 0), (-big, 0), (big, big), (-big, -big)]
     z = torch.tensor(pairs, dtype=dtype, device="cuda")
-    y = through_linear(z, path, act)
+    y, slope = through_linear(z, path, act)
     total = z.double().sum(1)
     want = act64(total, act)
     over = want.abs() > torch.finfo(dtype).max               # (rounds to an infinity)
@@ -62,3 +79,7 @@ def test_activations_at_infinities(act, path, dtype):
     fine = torch.isfinite(want)
     tol = (half_step(dtype) + 2.0 ** -15) * want.abs() + torch.finfo(dtype).tiny
     assert bool(((y.double() - want).abs() <= tol)[fine].all()), (y, want)
+    want = slope64(total, act)
+    assert torch.equal(torch.isnan(slope), torch.isnan(want)), (slope, want)
+    tol = half_step(dtype) * want.abs() + 2.0 ** -15
+    assert bool(((slope.double() - want).abs() <= tol)[~torch.isnan(want)].all()), (slope, want)
