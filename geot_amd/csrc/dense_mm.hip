@@ -417,30 +417,46 @@ __device__ inline Normal normal_of(float z) {
   return {r * t * bell, bell};
 }
 // 16-bit results: fewer instructions (the exact form's 25 an element were 610 us of vector time in the layer above).  log2 Phi(-a) is close
-// to a parabola: a polynomial of degree 7 in the exponent, 2.7e-5 (2^-15.2) of the value up to a = 6 and falling on behind.
-__device__ inline float gelu16(float z) {
+// to a parabola: a polynomial in the exponent, of degree 7 for float16 (2^-17 of the value up to a = 5.8; behind that it rounds to 0) and 9
+// for bfloat16, whose range holds Phi down to 2^-126 (2^-15 up to a = 10, 2^-13.8 up to 12.9, 0 behind).  Degree 7 for both was 27 %
+// off at -12.
+template <typename T> __device__ inline float gelu16(float z) {
   const float a = fminf(fabsf(z), 16.0f);
-  float p = 1.122847152146278e-06f;
-  p = fmaf(p, a, -4.626810914487578e-05f);
-  p = fmaf(p, a, 0.0008012278121896088f);
-  p = fmaf(p, a, -0.007969655096530914f);
-  p = fmaf(p, a, 0.05281980335712433f);
-  p = fmaf(p, a, 0.45959118008613586f);
-  p = fmaf(p, a, 1.1508647203445435f);
+  float p;
+  if constexpr (std::is_same<T, f16>::value) {
+    p = 1.7826165503720404e-06f;
+    p = fmaf(p, a, -6.053628749214113e-05f);
+    p = fmaf(p, a, 0.0009219465428031981f);
+    p = fmaf(p, a, -0.008472956717014313f);
+    p = fmaf(p, a, 0.053884927183389664f);
+    p = fmaf(p, a, 0.4585457146167755f);
+    p = fmaf(p, a, 1.1512134075164795f);
+  } else {
+    p = 1.8970891524361377e-09f;
+    p = fmaf(p, a, -1.3898932138545206e-07f);
+    p = fmaf(p, a, 4.4754006012226455e-06f);
+    p = fmaf(p, a, -8.38298219605349e-05f);
+    p = fmaf(p, a, 0.0010227881139144301f);
+    p = fmaf(p, a, -0.008678584359586239f);
+    p = fmaf(p, a, 0.05400051549077034f);
+    p = fmaf(p, a, 0.45869940519332886f);
+    p = fmaf(p, a, 1.1510733366012573f);
+  }
   p = fmaf(p, a, 1.0f);
   return fmaf(-a, __builtin_amdgcn_exp2f(-p), positive_part(z)); // max(z, 0) - a Phi(-a)
 }
-// gelu'(-a) = exp(-a^2 / 2) (R(a) - a / sqrt(2 pi)), gelu'(z) + gelu'(-z) = 1: degree 7 in a, 2.4e-5 (2^-15.3) absolute
+// gelu'(-a) = exp(-a^2 / 2) (R(a) - a / sqrt(2 pi)), gelu'(z) + gelu'(-z) = 1, R as in normal_of, of degree 5 in t = 1 / (1 + 0.35 a): 2^-16
+// of the slope up to a = 13.3, and below 2^-18 absolute around its zero at -0.75.  (A polynomial of degree 7 in a for the whole bracket held
+// 2^-15 absolute only: 0.7 % off at -4, 120 times the slope at -14.)
 __device__ inline float gelu_slope16(float z) {
   const float a = fminf(fabsf(z), 16.0f);
-  float q = -4.211963459965773e-05f;
-  q = fmaf(q, a, 0.0009205337846651673f);
-  q = fmaf(q, a, -0.0081043541431427f);
-  q = fmaf(q, a, 0.03846684470772743f);
-  q = fmaf(q, a, -0.1147356703877449f);
-  q = fmaf(q, a, 0.24307765066623688f);
-  q = fmaf(q, a, -0.79688920f);
-  q = fmaf(q, a, 0.4999766945838928f);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.35f, a, 1.0f));
+  float q = -0.09688097983598709f;
+  q = fmaf(q, t, 0.2732522487640381f);
+  q = fmaf(q, t, 0.02117534540593624f);
+  q = fmaf(q, t, 0.1652262806892395f);
+  q = fmaf(q, t, 0.13722974061965942f);
+  q = fmaf(-0.39894228040143268f, a, q * t);
   q *= __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
   return z < 0.0f ? q : 1.0f - q;
 }
@@ -459,7 +475,7 @@ template <bool EXACT> __device__ inline float logistic(float z) {
 // a z saved in float16 is infinite from 65520 on, where the value that was passed on can be an ordinary 0.
 template <typename T, int ACT> __device__ inline float activate(float z) {
   if constexpr (ACT == GEOT_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
-  else if constexpr (ACT == GEOT_ACT_GELU && sizeof(T) == 2) return gelu16(z);
+  else if constexpr (ACT == GEOT_ACT_GELU && sizeof(T) == 2) return gelu16<T>(z);
   else if constexpr (ACT == GEOT_ACT_GELU) { // z Phi(z) = max(z, 0) - |z| Phi(-|z|); behind 20 the tail is 0, and no infinity may meet it
     return fmaf(-fminf(fabsf(z), 20.0f), normal_of(z).tail, positive_part(z));
   }

@@ -22,10 +22,14 @@ def half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
 
+def normal_cdf(z):
+    return torch.special.erfc(z * -math.sqrt(0.5)) / 2       # (torch.special.ndtr is 1 + erf on the GPU: 0 below -8.3)
+
+
 def act64(z, name):
     if name == "relu":
         return torch.relu(z)
-    return z * (torch.special.ndtr(z) if name == "gelu" else torch.sigmoid(z)) if name != "none" else z
+    return z * (normal_cdf(z) if name == "gelu" else torch.sigmoid(z)) if name != "none" else z
 
 
 def slope64(z, name):
@@ -34,7 +38,7 @@ def slope64(z, name):
     if name == "relu":
         s = (z > 0).double()
     elif name == "gelu":
-        s = torch.special.ndtr(c) + c * torch.exp(-c * c / 2) / math.sqrt(2 * math.pi)
+        s = normal_cdf(c) + c * torch.exp(-c * c / 2) / math.sqrt(2 * math.pi)
     else:
         s = torch.sigmoid(c) * (1 + c * torch.sigmoid(-c))
     return torch.where(torch.isnan(z), z, s)
@@ -83,3 +87,34 @@ def test_activations_at_infinities(act, path, dtype):
     assert torch.equal(torch.isnan(slope), torch.isnan(want)), (slope, want)
     tol = half_step(dtype) * want.abs() + 2.0 ** -15
     assert bool(((slope.double() - want).abs() <= tol)[~torch.isnan(want)].all()), (slope, want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("path", ["tile", "few-kept"])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_activation_tails(act, path, dtype):
+    """Values and slopes from -14 to 14, relative to their size.  What a form may be off beside the rounding of its result:
+    float32 gelu: 4e-7 of the tail is its fit, the exponent's products (up to 2^7 of 2^-24 each) the rest: 2^-19; slopes and silu alike.
+    16-bit gelu: 2^-13 of the tail (fits 2^-17 and 2^-15 up to 10, float32 rounding of the exponent behind); slopes 2^-15.  silu in 16 bits
+    rounds z log2(e) once: 14 * 1.45 * 2^-24 * ln 2 = 2^-20.  A float16 result is rounded to half a subnormal step at least; in the
+    other types results below the smallest normal number, and a tail below 2^-126 times 14, may be 0.  Around the zero of gelu's slope (-0.75) the terms that cancel there are of size 0.3."""
+    rows = PATHS[path][0]
+    z = torch.cat([torch.linspace(-14, 14, rows - 4), torch.tensor([-0.75, -0.7518, -12.75, 5.8])])[:rows].to(dtype).cuda()
+    y, slope = through_linear(z[:, None], path, act)
+    z = z.double()
+    fit = {"gelu": 2.0 ** -19 if dtype == torch.float32 else 2.0 ** -13, "silu": 2.0 ** -19}[act]
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 15 * 2.0 ** -126
+    want = act64(z, act)
+    tail = want - z.clamp(min=0)                             # what is computed beside max(z, 0), which is exact
+    tol = half_step(dtype) * want.abs() + 2.0 ** -22 * want.abs() + fit * tail.abs() + tiny
+    off = (y.double() - want).abs() > tol
+    assert not off.any(), (z[off], y[off], want[off])
+    want = slope64(z, act)
+    fit = 2.0 ** -19 if dtype == torch.float32 else 2.0 ** -15
+    size = torch.minimum(want.abs(), (1 - want).abs()) + 0.3 * ((z.abs() > 0.3) & (z.abs() < 1.6))
+    if act == "silu":                                        # s (1 + z (1 - s)): its bracket cancels at -1.28, as large as the two terms together
+        size = torch.sigmoid(z) * (1 + z.abs() * torch.sigmoid(-z))
+    tol = half_step(dtype) * want.abs() + 2.0 ** -22 * want.abs() + fit * size + tiny
+    off = (slope.double() - want).abs() > tol
+    assert not off.any(), (z[off], slope[off], want[off])
