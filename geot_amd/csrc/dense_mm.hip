@@ -483,8 +483,7 @@ template <typename T, int ACT> __device__ inline float activate(float z) {
   else return z;
 }
 template <typename T, int ACT> __device__ inline float activation_slope(float z) {
-  if constexpr (ACT == GEOT_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-  else if constexpr (ACT == GEOT_ACT_GELU && sizeof(T) == 2) return gelu_slope16(z);
+  if constexpr (ACT == GEOT_ACT_GELU && sizeof(T) == 2) return gelu_slope16(z);
   else if constexpr (ACT == GEOT_ACT_GELU) {
     const Normal n = normal_of(z);
     const float c = fminf(fmaxf(z, -20.0f), 20.0f), s = fmaf(c * 0.39894228040143268f, n.bell, z < 0.0f ? n.tail : 1.0f - n.tail);
@@ -493,6 +492,11 @@ template <typename T, int ACT> __device__ inline float activation_slope(float z)
     const float s = logistic<sizeof(T) == 4>(z), c = fminf(fmaxf(z, -128.0f), 128.0f); // (s is 0 or 1 behind; a NaN stays in s)
     return s * fmaf(c, 1.0f - s, 1.0f);
   } else return 1.0f;
+}
+// dy act'(z).  relu's is a choice, not a product: where it is off, an infinite or NaN dy (a masked place) does not come through.
+template <typename T, int ACT> __device__ inline float activation_gradient(float dy, float z) {
+  if constexpr (ACT == GEOT_ACT_RELU) return z > 0.0f ? dy : (z != z ? z : 0.0f);
+  else return dy * activation_slope<T, ACT>(z);
 }
 template <int V> using Const = std::integral_constant<int, V>;
 template <typename F> __device__ __host__ inline void by_activation(int act, F f) {
@@ -680,7 +684,7 @@ __device__ inline void finish_row(const RowsArgs &g, int64_t row, int64_t col, i
   if constexpr (DZ) {
 #pragma unroll
     for (int c = 0; c < V; ++c) {
-      v[c] = as_float(tmp[c]) * activation_slope<T, ACT>(v[c]);
+      v[c] = activation_gradient<T, ACT>(as_float(tmp[c]), v[c]);
       sum[c] += v[c];
     }
   } else {
@@ -1227,7 +1231,7 @@ __global__ __launch_bounds__(kThreads) void act_backward_kernel(const T *dy, con
       }
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float d = as_float(a[v]) * activation_slope<T, ACT>(as_float(b[v]));
+        const float d = activation_gradient<T, ACT>(as_float(a[v]), as_float(b[v]));
         sum[v] += d;
         a[v] = (T)d;
       }

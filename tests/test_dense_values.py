@@ -118,3 +118,29 @@ def test_activation_tails(act, path, dtype):
     tol = half_step(dtype) * want.abs() + 2.0 ** -22 * want.abs() + fit * size + tiny
     off = (slope.double() - want).abs() > tol
     assert not off.any(), (z[off], slope[off], want[off])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("path", PATHS)
+@pytest.mark.parametrize("residual", [False, True], ids=["plain", "skip"])
+def test_relu_keeps_masked_gradients_out(residual, path, dtype):
+    """An infinite or NaN gradient where relu is off reaches nothing but the residual: dx and db are what they are with 0 there."""
+    m, k, n = PATHS[path]
+    g = torch.Generator().manual_seed(1)
+    x, w, b, r, dy = (torch.randn(*s, generator=g).to(dtype).cuda() for s in ((m, k), (n, k), (n,), (m, n), (m, n)))
+    w[5:9] = 0
+    b[5:8] = torch.tensor([-1.0, 0.0, -3.0])
+    leaves = [t.requires_grad_() for t in (x, w, b)] + ([r.requires_grad_()] if residual else [])
+
+    def grads(dy):
+        return torch.autograd.grad(geot.linear(x, w, b, residual=r if residual else None, activation="relu"), leaves, dy)
+
+    clean, dirty = dy.clone(), dy.clone()
+    clean[:, 5:8] = 0
+    dirty[:, 5:8] = torch.tensor([INF, NAN, -INF], dtype=dtype)
+    got = grads(dirty)
+    for a, c in zip(got[:3], grads(clean)[:3]):
+        assert torch.equal(a, c)
+    if residual:
+        assert torch.equal(got[3].nan_to_num(7.0), dirty.nan_to_num(7.0))
