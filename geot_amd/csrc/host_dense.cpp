@@ -56,6 +56,11 @@ std::vector<int64_t> with_width(const at::Tensor &x, int64_t width) {
   return s;
 }
 at::Tensor scratch(const at::Tensor &like, size_t bytes) { return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)); }
+// (a tangent would get lost without a word: the kernels know nothing of it)
+void reverse_mode_only(const char *op, std::initializer_list<const at::Tensor *> ts) {
+  for (const at::Tensor *t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->_fw_grad(/*level=*/0).defined(), op, ": forward-mode gradients (jvp, dual tensors) are not supported");
+}
 bool wants_grad(std::initializer_list<const at::Tensor *> ts) {
   if (!c10::GradMode::is_enabled()) return false;
   for (const at::Tensor *t : ts)
@@ -151,6 +156,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_backward_op(const at::Tens
 
 at::Tensor linear_op(const at::Tensor &x, const at::Tensor &w, const c10::optional<at::Tensor> &bias, const c10::optional<at::Tensor> &residual,
                      c10::string_view activation) {
+  reverse_mode_only("linear", {&x, &w, ptr_of(bias), ptr_of(residual)});
   if (wants_grad({&x, &w, ptr_of(bias), ptr_of(residual)})) {
     static const auto train = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::linear_train", "").typed<decltype(linear_train_op)>();
     return std::get<0>(train.call(x, w, bias, residual, activation));
@@ -222,6 +228,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> segment_matmul_backward_op(const 
 at::Tensor segment_matmul_op(const at::Tensor &x, const at::Tensor &ptr, const at::Tensor &w, const c10::optional<at::Tensor> &bias) {
   static const auto train = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::segment_matmul_train", "").typed<decltype(segment_matmul_forward_op)>();
   static const auto fwd = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::segment_matmul_forward", "").typed<decltype(segment_matmul_forward_op)>();
+  reverse_mode_only("segment_matmul", {&x, &w, ptr_of(bias)});
   return wants_grad({&x, &w, ptr_of(bias)}) ? train.call(x, ptr, w, bias) : fwd.call(x, ptr, w, bias);
 }
 
@@ -279,6 +286,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_backward_op(const at::
 }
 
 at::Tensor layer_norm_op(const at::Tensor &x, const c10::optional<at::Tensor> &w, const c10::optional<at::Tensor> &b, double eps) {
+  reverse_mode_only("layer_norm", {&x, ptr_of(w), ptr_of(b)});
   if (wants_grad({&x, ptr_of(w), ptr_of(b)})) {
     static const auto train = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::layer_norm_train", "").typed<decltype(layer_norm_train_op)>();
     return std::get<0>(train.call(x, w, b, eps));

@@ -607,8 +607,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     """``act(x @ weight.T + bias) + residual`` in one kernel: x [..., in], weight [out, in] (torch.nn.Linear's layout), bias [out],
     residual [..., out]; ``activation``: 'none', 'relu', 'gelu' (the error-function form) or 'silu'.
 
-    float32, float16 or bfloat16, one dtype for all operands; sums in float32, one rounding.  Differentiable in every tensor (the
-    backward pass itself is not).  A training call of a wide layer keeps the pre-activation in the operands' dtype; a narrow one (in <= 256,
+    float32, float16 or bfloat16, one dtype for all operands; sums in float32, one rounding.  Differentiable in every tensor (in reverse
+    mode; the backward pass itself is not).  A training call of a wide layer keeps the pre-activation in the operands' dtype; a narrow one (in <= 256,
     float32 128) computes it again in the backward pass, and 'none', and 'relu' without a residual, do not need it."""
     return torch.ops.geot_dense.linear(x, weight, bias, residual, activation)
 

@@ -18,6 +18,33 @@ INF, NAN = float("inf"), float("nan")
 PATHS = {"tile": (200, 64, 72), "few": (33, 128, 40), "few-kept": (20, 512, 40), "split": (100, 4160, 48)}
 
 
+# ---- refusals: no GPU needed ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("device", ["cpu", "meta"])
+def test_forward_mode_is_refused(device):
+    """A tangent of any input, through dual tensors or torch.func, alone or beside reverse mode: named, never dropped."""
+    import torch.autograd.forward_ad as forward_ad
+    ones = lambda *s: torch.ones(*s, device=device)  # noqa: E731
+    ptr = torch.tensor([0, 1, 4]).to(device)
+    calls = {"linear": (lambda x, w, b, r: geot.linear(x, w, b, residual=r), [ones(4, 6), ones(5, 6), ones(5), ones(4, 5)]),
+             "segment_matmul": (lambda x, w, b: geot.segment_matmul(x, ptr, w, b), [ones(4, 6), ones(2, 6, 5), ones(2, 5)]),
+             "layer_norm": (geot.layer_norm, [ones(4, 6), ones(6), ones(6)])}
+    for name, (f, args) in calls.items():
+        for i, t in enumerate(args):
+            one = lambda v: f(*args[:i], v, *args[i + 1:])  # noqa: E731, B023
+            refused = pytest.raises(NotImplementedError, match=f"{name}: forward-mode gradients .* not supported")
+            with refused, forward_ad.dual_level():
+                one(forward_ad.make_dual(t, torch.ones_like(t)))
+            with refused, forward_ad.dual_level():
+                one(forward_ad.make_dual(t.clone().requires_grad_(), torch.ones_like(t)))
+            with refused:
+                torch.func.jvp(one, (t,), (torch.ones_like(t),))
+            with refused, torch.no_grad():
+                torch.func.jvp(one, (t,), (torch.ones_like(t),))
+            with refused:
+                torch.func.jacfwd(one)(t)
+
+
+# ---- activations ----------------------------------------------------------------------------------------------------------------------
 def half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
