@@ -162,6 +162,18 @@ def _single_user(node) -> Optional[fx.Node]:
     return users[0] if len(users) == 1 else None
 
 
+def _writes_between(first, last) -> bool:
+    """Whether anything strictly between the two nodes may write into a tensor (an exported graph keeps in-place operators) or change a mode:
+    what is computed at ``first`` must not move down to ``last`` then."""
+    node = first.next
+    while node is not last:
+        if node.op == "call_function" and getattr(node.target, "__module__", None) != "_operator":      # (getitem, arithmetic of sizes)
+            if not isinstance(node.target, torch._ops.OpOverload) or node.target._schema.is_mutable:
+                return True
+        node = node.next
+    return False
+
+
 def _dense_operands(*nodes) -> bool:
     """All of one dtype the dense operators take."""
     vals = [n.meta.get("val") for n in nodes if n is not None]
@@ -171,8 +183,8 @@ def _dense_operands(*nodes) -> bool:
 def rewrite_dense(gm: fx.GraphModule) -> int:
     """Rewrite ``aten.linear`` - with the relu / silu / gelu (error-function form) and the addition of a tensor of the result's shape that
     alone consume it - into ``geot_dense::linear``, and ``aten.layer_norm`` over the last dimension into ``geot_dense::layer_norm``, in
-    place; returns the number of rewritten products and normalisations.  Other dtypes, broadcast additions and shared intermediates keep
-    their aten form."""
+    place; returns the number of rewritten products and normalisations.  Other dtypes, broadcast additions, shared intermediates and what an
+    in-place operator stands in front of keep their aten form."""
     graph = gm.graph
     done = 0
     for node in list(graph.nodes):
@@ -184,10 +196,10 @@ def rewrite_dense(gm: fx.GraphModule) -> int:
             last, act, residual = node, "none", None
             nxt = _single_user(last)
             if nxt is not None and nxt.op == "call_function" and nxt.target in _ACTIVATIONS and \
-                    nxt.kwargs.get("approximate", "none") == "none" and len(nxt.args) == 1:
+                    nxt.kwargs.get("approximate", "none") == "none" and len(nxt.args) == 1 and not _writes_between(node, nxt):
                 last, act = nxt, _ACTIVATIONS[nxt.target]
                 nxt = _single_user(last)
-            if nxt is not None and _is(nxt, aten.add.Tensor) and nxt.kwargs.get("alpha", 1) == 1:
+            if nxt is not None and _is(nxt, aten.add.Tensor) and nxt.kwargs.get("alpha", 1) == 1 and not _writes_between(node, nxt):
                 other = nxt.args[1] if nxt.args[0] is last else nxt.args[0]
                 if isinstance(other, fx.Node) and other is not last and _shape(other) == _shape(last) and _dense_operands(x, other):
                     last, residual = nxt, other

@@ -44,6 +44,48 @@ def test_forward_mode_is_refused(device):
                 torch.func.jacfwd(one)(t)
 
 
+class _Writes(torch.nn.Module):
+    """In-place operators between a product and what consumes it: on the product's input, its weight, the skip connection."""
+
+    def __init__(self, where):
+        super().__init__()
+        self.lin, self.where = torch.nn.Linear(6, 6), where
+
+    def forward(self, x):
+        h = x * 2
+        z = self.lin(h)
+        if self.where == "activation":
+            h.add_(1)
+        y = torch.relu(z)
+        if self.where == "addition":
+            h.mul_(3)
+        if self.where == "elsewhere":
+            x = torch.zeros_like(x).view(-1)[:6] + x
+        return y + h, x
+
+
+@pytest.mark.parametrize("where,form", [("activation", ("none", False)), ("addition", ("relu", False)), ("elsewhere", ("relu", True))])
+def test_rewriting_keeps_the_order_of_writes(where, form):
+    """The fused node reads its operands where the last part of it stood: in front of no write that was there before."""
+    from geot_amd.match_replace import pattern_transform
+    torch.manual_seed(0)
+    model, x = _Writes(where), torch.randn(4, 6)
+    ep = pattern_transform(model, (x,), dense=True)
+    nodes = [n for n in ep.graph_module.graph.nodes if n.target == torch.ops.geot_dense.linear.default]
+    assert [(n.args[4], n.args[3] is not None) for n in nodes] == [form]
+
+    def plain_linear(x, w, b, r, act):
+        y = torch.nn.functional.linear(x, w, b)
+        y = torch.relu(y) if act == "relu" else y
+        return y if r is None else y + r
+
+    nodes[0].target = plain_linear                       # (what the node computes, on the CPU)
+    ep.graph_module.recompile()
+    got = ep.graph_module(*[p.detach() for p in model.parameters()], x)
+    for a, b in zip(got, model(x)):
+        assert torch.equal(a, b.detach())
+
+
 # ---- activations ----------------------------------------------------------------------------------------------------------------------
 def half_step(dtype):
     return torch.finfo(dtype).eps / 2
