@@ -25,6 +25,7 @@ with these guarantees the reference's pass does not give:
 """
 from __future__ import annotations
 
+import warnings
 from typing import Optional, Tuple
 
 import torch
@@ -220,6 +221,10 @@ def rewrite_dense(gm: fx.GraphModule) -> int:
         new.meta["val"] = last.meta.get("val")
         last.replace_all_uses_with(new)
         done += 1
+    if any(n.target in (torch.ops.geot_dense.linear.default, torch.ops.geot_dense.layer_norm.default) and n.meta.get("val") is not None and
+           n.meta["val"].device.type == "cpu" for n in graph.nodes):
+        warnings.warn("pattern_transform(dense=True) rewrote products or normalisations of a model that was exported on the CPU: they run on the GPU "
+                      "only (geot_dense::linear, geot_dense::layer_norm refuse CPU tensors)", stacklevel=3)
     if done:
         graph.eliminate_dead_code()
         graph.lint()
@@ -318,7 +323,8 @@ def pattern_transform(model: torch.nn.Module, args, sort_edges: bool = False, st
     ``static_graph``).  ``static_graph=True``: the fused nodes are bound to ``geot_amd.Graph`` handles built here, once, from the example
     inputs' edge list (see :func:`bind_static_graphs` for the promise that goes with it); ``exported.geot_graphs`` lists the handles.
     ``dense=True``: the layers' products and normalisations become ``geot_amd.linear`` / ``geot_amd.layer_norm`` nodes too
-    (:func:`rewrite_dense`); ``exported.geot_dense_nodes`` counts them."""
+    (:func:`rewrite_dense`); ``exported.geot_dense_nodes`` counts them.  Every rewritten node runs on the GPU only, wherever the model was
+    exported (dense nodes of a model on the CPU: a warning)."""
     exported = export(model, args, **kwargs)
     exported.geot_fused_nodes = rewrite_graph(exported.graph_module, sort_edges=sort_edges and not static_graph)
     exported.geot_graphs = bind_static_graphs(exported, args, slab_mode=slab_mode) if static_graph else []

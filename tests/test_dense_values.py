@@ -86,6 +86,18 @@ def test_rewriting_keeps_the_order_of_writes(where, form):
         assert torch.equal(a, b.detach())
 
 
+def test_rewriting_a_model_on_the_cpu_warns():
+    import warnings
+    from geot_amd.match_replace import pattern_transform
+    args = (torch.randn(4, 6),)
+    with pytest.warns(UserWarning, match="run on the GPU only"):
+        pattern_transform(torch.nn.Linear(6, 6), args, dense=True)
+    with warnings.catch_warnings():
+        warnings.filterwarnings("error", message=".*run on the GPU only")
+        pattern_transform(torch.nn.Linear(6, 6), args)                               # (nothing rewritten, nothing to say)
+        pattern_transform(torch.nn.Linear(6, 6).double(), (args[0].double(),), dense=True)
+
+
 # ---- activations ----------------------------------------------------------------------------------------------------------------------
 def half_step(dtype):
     return torch.finfo(dtype).eps / 2
