@@ -94,6 +94,24 @@ def _rows_arg(graph: fx.Graph, dst: fx.Node, before: fx.Node):
         return graph.call_function(aten.sym_size.int, (dst, 0))
 
 
+def _writes_between(first, last) -> bool:
+    """Whether anything strictly between the two nodes may write into a tensor (an exported graph keeps in-place operators) or change a mode:
+    what is computed at ``first`` must not move down to ``last`` then."""
+    node = first.next
+    while node is not last:
+        if node.op == "call_function" and getattr(node.target, "__module__", None) != "_operator":      # (getitem, arithmetic of sizes)
+            if not isinstance(node.target, torch._ops.OpOverload) or node.target._schema.is_mutable:
+                return True
+        node = node.next
+    return False
+
+
+def _may_be_written(node) -> bool:
+    """Whether a user of the node writes into it or takes a view of it (through which others may)."""
+    return any(u.op == "call_function" and isinstance(u.target, torch._ops.OpOverload) and
+               (u.target._schema.is_mutable or any(r.alias_info is not None for r in u.target._schema.returns)) for u in node.users)
+
+
 def rewrite_graph(gm: fx.GraphModule, sort_edges: bool = False) -> int:
     """Rewrite every matching index_add in ``gm`` in place; returns the number of fused nodes."""
     graph = gm.graph
@@ -132,6 +150,9 @@ def rewrite_graph(gm: fx.GraphModule, sort_edges: bool = False) -> int:
                 target = None
         if target is None or args is None:
             continue
+        read = [n for n in (source, *source.args) if _gathered_rows(n) is not None] + [source]
+        if _writes_between(read[0], node) or _may_be_written(dst):
+            continue                    # (the rows, a factor or the zeros may hold something else by now)
         rows = _rows_arg(graph, dst, node)
         with graph.inserting_before(node):
             if sort_edges:
@@ -161,18 +182,6 @@ _DENSE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 def _single_user(node) -> Optional[fx.Node]:
     users = list(node.users)
     return users[0] if len(users) == 1 else None
-
-
-def _writes_between(first, last) -> bool:
-    """Whether anything strictly between the two nodes may write into a tensor (an exported graph keeps in-place operators) or change a mode:
-    what is computed at ``first`` must not move down to ``last`` then."""
-    node = first.next
-    while node is not last:
-        if node.op == "call_function" and getattr(node.target, "__module__", None) != "_operator":      # (getitem, arithmetic of sizes)
-            if not isinstance(node.target, torch._ops.OpOverload) or node.target._schema.is_mutable:
-                return True
-        node = node.next
-    return False
 
 
 def _dense_operands(*nodes) -> bool:

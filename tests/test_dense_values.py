@@ -86,6 +86,25 @@ def test_rewriting_keeps_the_order_of_writes(where, form):
         assert torch.equal(a, b.detach())
 
 
+@pytest.mark.parametrize("where", ["nowhere", "rows", "factor", "zeros", "row of zeros"])
+def test_rewriting_an_aggregation_keeps_the_order_of_writes(where):
+    from geot_amd.match_replace import pattern_transform
+
+    class Aggregate(torch.nn.Module):
+        def forward(self, x, w, row, col):
+            h, f = x * 2, w * 2
+            rows = h.index_select(0, col)
+            out = h.new_zeros(5, 6)
+            scaled = rows * f.unsqueeze(-1)
+            if where != "nowhere":
+                {"rows": h, "factor": f, "zeros": out, "row of zeros": out[0]}[where].add_(1)
+            return out.index_add(0, row, scaled) + h.sum() + f.sum()
+
+    row = torch.tensor([0, 1, 1, 3])
+    ep = pattern_transform(Aggregate(), (torch.randn(5, 6), torch.randn(4), row, row))
+    assert ep.geot_fused_nodes == (where == "nowhere")
+
+
 def test_rewriting_a_model_on_the_cpu_warns():
     import warnings
     from geot_amd.match_replace import pattern_transform
