@@ -1028,13 +1028,17 @@ template <typename T, int FM> __global__ __launch_bounds__(512, 2) void mm_few_r
 struct WeightArgs {
   const void *p, *q;   // [rows, np], [rows, nq]: out(i, j) = sum over rows of p[r, i] q[r, j]
   void *out, *colsum;  // [G, np, nq] in T; column sums of p (sum_p) or q [G, np or nq], may be null
-  float *part;         // partial products of the chunks of groups that have several: [slots][np * nq + (colsum ? ns : 0)]
+  float *part;         // partial products of the chunks of groups that have several: [part_of ..][np * nq + (colsum ? ns : 0)]
   int64_t ldp, ldq, np, nq, ns;
   Groups groups;
   int64_t unit;        // rows of a chunk; with groups 1 << unit_log2
   int unit_log2;
   uint32_t tiles_p, tiles_q;
-  int sum_p;
+  int sum_p, compact;
+  // Where chunk `index` of a group goes that starts at row q0 and has several; `slot`: the chunk's slot of the launch.  compact: a number that
+  // does not grow with the groups.  floor(q0 / unit) + index ascends over all such chunks, and two of them share a value at most where one
+  // group's last chunk meets the next one's first: first chunks take the odd numbers, the others the even ones, all below 2 ceil(rows / unit).
+  __device__ int64_t part_of(int64_t q0, int64_t index, int64_t slot) const { return compact ? 2 * ((q0 >> unit_log2) + index) + (index == 0) : slot; }
 };
 
 template <bool PAIR, int WHICH, typename A, typename B> __device__ inline auto &pick(A &a, B &b) {
@@ -1082,6 +1086,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 && BN == 64 ? 4 : 3) void mm
   staged_products<T, BM, BN, WM, WN, 1>(sa, sb, acc, lds, k_len, tid, wm, wn, lane);
 
   const int64_t per_slot = g.np * g.nq + (g.colsum ? g.ns : 0);
+  float *const part = g.part + g.part_of(piece.begin, piece.index, slot) * per_slot;
   float *out = reinterpret_cast<float *>(lds);
   const int col = (tid % (BN / 4)) * 4;
 #pragma unroll
@@ -1120,7 +1125,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 && BN == 64 ? 4 : 3) void mm
             if (c < cols) o[c] = tmp[c];
         }
       } else {
-        float *o = g.part + slot * per_slot + row * g.nq + cc;
+        float *o = part + row * g.nq + cc;
         if (cols == 4) {
           *reinterpret_cast<Packed16<float> *>(o) = *reinterpret_cast<const u32x4 *>(v);
         } else {
@@ -1156,7 +1161,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 && BN == 64 ? 4 : 3) void mm
       float s = 0.0f;
       for (int k = 0; k < E::BK / 8; ++k) s += out[k * R + c];
       if (whole) static_cast<T *>(g.colsum)[piece.group * g.ns + first + c] = (T)s;
-      else g.part[slot * per_slot + g.np * g.nq + first + c] = s;
+      else part[g.np * g.nq + first + c] = s;
     }
   }
 }
@@ -1183,7 +1188,7 @@ template <typename T, int WAYS> __global__ __launch_bounds__(kThreads) void mm_j
     float s = 0.0f;
     if (i < per_slot) {
 #pragma unroll 4
-      for (int64_t c = way; c < chunks; c += WAYS) s += g.part[(piece.start + c) * per_slot + i];
+      for (int64_t c = way; c < chunks; c += WAYS) s += g.part[g.part_of(piece.begin, c, piece.start + c) * per_slot + i];
     }
     if constexpr (WAYS > 1) {
       part[threadIdx.x] = s;
@@ -1417,7 +1422,9 @@ template <typename T> int preactivation_typed(RowsArgs &g, const void *dy, const
 // of a power of two (piece_of).
 struct WeightPlan {
   int64_t tiles_p, tiles_q, unit, slots;
+  int64_t parts; // partial products that need room (part_of)
   int unit_log2;
+  bool compact;
 };
 WeightPlan weight_plan(int64_t rows, int64_t groups, bool with_ptr, int64_t np, int64_t nq, int dtype) {
   WeightPlan w;
@@ -1436,6 +1443,10 @@ WeightPlan weight_plan(int64_t rows, int64_t groups, bool with_ptr, int64_t np, 
   }
   w.slots = slots_of(rows, groups, with_ptr, w.unit);
   if (w.slots < 1) w.slots = 1;
+  // (64 experts of 1024 x 2048, 32768 rows: 16 numbers of 8.4 MB where the launch has 74 slots)
+  const int64_t compact = 2 * ((rows + w.unit - 1) / w.unit);
+  w.compact = with_ptr && compact < w.slots;
+  w.parts = rows > w.unit ? (w.compact ? compact : w.slots) : 0;
   return w;
 }
 template <typename T, int BM, int BN, int WM, int WN> int run_weight(WeightArgs &g, int64_t slots, hipStream_t st) {
@@ -1474,8 +1485,9 @@ int weight_product(WeightArgs &g, int dtype, void *workspace, size_t workspace_b
   g.tiles_p = (uint32_t)w.tiles_p;
   g.tiles_q = (uint32_t)w.tiles_q;
   g.part = static_cast<float *>(workspace);
-  if (g.groups.rows > w.unit) {
-    const size_t need = (size_t)w.slots * (size_t)(g.np * g.nq + (g.colsum ? g.ns : 0)) * sizeof(float);
+  g.compact = w.compact;
+  if (w.parts > 0) {
+    const size_t need = (size_t)w.parts * (size_t)(g.np * g.nq + (g.colsum ? g.ns : 0)) * sizeof(float);
     if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) return geot_internal_fail(GEOT_EWORKSPACE, "weight gradient: workspace too small or misaligned");
   }
   switch (dtype) {
@@ -1527,7 +1539,7 @@ int geot_linear_grad_input(const void *dz, const void *weight, void *dx, int64_t
 size_t geot_linear_grad_weight_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dtype) {
   if (bad_size(rows, in, out)) return 0;
   const WeightPlan w = weight_plan(rows, 1, false, out, in, dtype);
-  return rows > w.unit ? (size_t)w.slots * (size_t)(in * out + out) * sizeof(float) : 0;
+  return (size_t)w.parts * (size_t)(in * out + out) * sizeof(float);
 }
 
 int geot_linear_grad_weight(const void *dz, const void *x, int64_t ldx, void *dweight, void *dbias, int64_t rows, int64_t in, int64_t out, int dtype,
@@ -1601,7 +1613,7 @@ int geot_segment_matmul_grad_input(const void *dy, const int64_t *ptr, const voi
 size_t geot_segment_matmul_grad_weight_workspace_bytes(int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype) {
   if (bad_size(rows, in, out) || groups < 0 || groups > 65535) return 0;
   const WeightPlan w = weight_plan(rows, groups, true, in, out, dtype);
-  return rows > w.unit ? (size_t)w.slots * (size_t)(in * out + out) * sizeof(float) : 0;
+  return (size_t)w.parts * (size_t)(in * out + out) * sizeof(float);
 }
 
 int geot_segment_matmul_grad_weight(const void *x, int64_t ldx, const int64_t *ptr, const void *dy, void *dweight, void *dbias, int64_t rows, int64_t groups,

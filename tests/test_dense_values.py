@@ -86,6 +86,19 @@ def test_rewriting_keeps_the_order_of_writes(where, form):
         assert torch.equal(a, b.detach())
 
 
+def test_segment_workspace_does_not_grow_with_groups():
+    """Only chunks of groups that have several need room: at fixed rows no number of groups asks for more than twice the chunks of all rows."""
+    L = geot._lib.load()
+    one = (64 * 128 + 128) * 4
+    for rows in (1, 256, 257, 20_000, 1_000_003):
+        for dtype in (0, 2, 3):
+            sizes = [L.geot_segment_matmul_grad_weight_workspace_bytes(rows, groups, 64, 128, dtype) for groups in (1, 16, 256, 4096, 65535)]
+            assert max(sizes) <= 2 * -(-rows // 256) * one and sizes[-1] == sizes[-2], (rows, dtype, sizes)
+    # 256 groups of 4096 x 4096 and 20,000 rows: two chunks of 16384 rows, of which one group could have both
+    need = L.geot_segment_matmul_grad_weight_workspace_bytes(20_000, 256, 4096, 4096, 2)
+    assert need <= 4 * (4096 * 4096 + 4096) * 4
+
+
 @pytest.mark.parametrize("where", ["nowhere", "rows", "factor", "zeros", "row of zeros"])
 def test_rewriting_an_aggregation_keeps_the_order_of_writes(where):
     from geot_amd.match_replace import pattern_transform
@@ -244,3 +257,27 @@ def test_relu_keeps_masked_gradients_out(residual, path, dtype):
         assert torch.equal(a, c)
     if residual:
         assert torch.equal(got[3].nan_to_num(7.0), dirty.nan_to_num(7.0))
+
+
+# ---- every kernel -----------------------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_segment_gradients_of_chunked_groups(dtype):
+    """Groups of one to three chunks of 256 rows beside empty and tiny ones, ends on, before and behind a chunk's border, more groups than
+    chunks: dW and db of every group, twice, bit for bit.  Integers of at most 4 and sums below 2^11 come out exactly in every type."""
+    sizes = [0, 257, 1, 512, 0, 0, 513, 3, 256, 255, 700, 0, 2, 300, 1, 258, 511, 0, 0, 0, 769, 5] + [0, 1] * 20
+    rows = [0]
+    for s in sizes:
+        rows.append(rows[-1] + s)
+    k, n, m = 20, 72, rows[-1] + 9
+    g = torch.Generator().manual_seed(3)
+    x, dy = (torch.randint(-1, 2, s, generator=g).to(dtype).cuda() for s in ((m, k), (m, n)))
+    w, b = torch.zeros(len(sizes), k, n, dtype=dtype, device="cuda", requires_grad=True), torch.zeros(len(sizes), n, dtype=dtype, device="cuda", requires_grad=True)
+    ptr = torch.tensor(rows, device="cuda")
+    runs = [torch.autograd.grad(geot.segment_matmul(x, ptr, w, b), [w, b], dy) for _ in range(2)]
+    for i in range(len(sizes)):
+        lo, hi = rows[i], rows[i + 1]
+        dw, db = x[lo:hi].double().t().contiguous() @ dy[lo:hi].double(), dy[lo:hi].double().sum(0)
+        for run in runs:
+            # (bfloat16 holds whole numbers up to 256; sums of 769 numbers of -1, 0, 1 stay below: 6 standard deviations are 150)
+            assert torch.equal(run[0][i].double(), dw) and torch.equal(run[1][i].double(), db), i
