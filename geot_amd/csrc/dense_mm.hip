@@ -1085,8 +1085,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 && BN == 64 ? 4 : 3) void mm
   const int64_t k_len = r1 - r0;
   staged_products<T, BM, BN, WM, WN, 1>(sa, sb, acc, lds, k_len, tid, wm, wn, lane);
 
-  const int64_t per_slot = g.np * g.nq + (g.colsum ? g.ns : 0);
-  float *const part = g.part + g.part_of(piece.begin, piece.index, slot) * per_slot;
+  const int64_t per_slot = g.np * g.nq + (g.colsum ? g.ns : 0), number = g.part_of(piece.begin, piece.index, slot);
   float *out = reinterpret_cast<float *>(lds);
   const int col = (tid % (BN / 4)) * 4;
 #pragma unroll
@@ -1125,7 +1124,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 && BN == 64 ? 4 : 3) void mm
             if (c < cols) o[c] = tmp[c];
         }
       } else {
-        float *o = part + row * g.nq + cc;
+        float *o = g.part + number * per_slot + row * g.nq + cc;
         if (cols == 4) {
           *reinterpret_cast<Packed16<float> *>(o) = *reinterpret_cast<const u32x4 *>(v);
         } else {
@@ -1161,7 +1160,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 && BN == 64 ? 4 : 3) void mm
       float s = 0.0f;
       for (int k = 0; k < E::BK / 8; ++k) s += out[k * R + c];
       if (whole) static_cast<T *>(g.colsum)[piece.group * g.ns + first + c] = (T)s;
-      else part[g.np * g.nq + first + c] = s;
+      else g.part[number * per_slot + g.np * g.nq + first + c] = s;
     }
   }
 }
@@ -1181,14 +1180,18 @@ template <typename T, int WAYS> __global__ __launch_bounds__(kThreads) void mm_j
   if (len <= g.unit) return;
   const int64_t chunks = (len + g.unit - 1) / g.unit;
   const int64_t size = g.np * g.nq, per_slot = size + (g.colsum ? g.ns : 0);
+  const float *first = g.part + g.part_of(piece.begin, 0, piece.start) * per_slot; // (chunks behind the first: evenly spaced)
+  const float *rest = g.part + (g.compact ? 2 * (piece.begin >> g.unit_log2) : piece.start) * per_slot;
+  const int64_t step = (g.compact ? 2 : 1) * per_slot;
   constexpr int LANES = kThreads / WAYS;
   const int lane = threadIdx.x % LANES, way = threadIdx.x / LANES;
   for (int64_t base = (int64_t)blockIdx.x * LANES; base < per_slot; base += (int64_t)gridDim.x * LANES) {
     const int64_t i = base + lane;
     float s = 0.0f;
     if (i < per_slot) {
+      if (way == 0) s = first[i];
 #pragma unroll 4
-      for (int64_t c = way; c < chunks; c += WAYS) s += g.part[g.part_of(piece.begin, c, piece.start + c) * per_slot + i];
+      for (int64_t c = way == 0 ? WAYS : way; c < chunks; c += WAYS) s += rest[c * step + i];
     }
     if constexpr (WAYS > 1) {
       part[threadIdx.x] = s;
