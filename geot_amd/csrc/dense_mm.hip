@@ -10,8 +10,8 @@
 // weight is above 2^-24 of it: x1y1, x1y2, x2y1, x2y2, x1y3, x3y1.  What is left out (x2y3, x3y2, x3y3) is at most 2^-23 of |xy| and
 // 2^-26 of it on average - below the float32 rounding of the sum itself - while the bfloat16 cores run 16 times faster than the
 // float32 ones (dense peaks 2.5 PFLOP/s against 0.157): six products there cost less than half of one here.  A split of an infinity
-// (inf - inf) or of a value that rounds up to one is not a number: any non-finite sum is computed again, element by element, in plain
-// float32 (element_again), so infinities and NaN come out as in an ordinary float32 product.  The matrix cores read a bfloat16 below 2^-133
+// (inf - inf) or of a value that rounds up to one is not a number: any non-finite sum is computed again in plain
+// float32 (sums_again), so infinities and NaN come out as in an ordinary float32 product.  The matrix cores read a bfloat16 below 2^-133
 // as 0, so a factor below 2^-110 keeps an absolute 2^-133 instead of its last bits (float32 itself ends at 2^-149).
 //
 // Layout in LDS.  A tile holds chunks of 8 reduction values (16 bytes) - the operand of one MFMA lane - as
@@ -299,6 +299,65 @@ struct StageNone {
   __device__ void store(char *, int) {}
 };
 
+__device__ inline bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+template <typename P> __device__ inline P *pointer_of_lane(P *p, int lane) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  return reinterpret_cast<P *>(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
+}
+// A lane's sum that came out non-finite again, in plain float32: the way of an infinity, a NaN or an overflow through a product of split
+// operands.  a[i * stride_a] times b[i * stride_b], i < k; every active lane of the wave takes part, `bad` or not.  A lane walks its first 64
+// terms alone, which ends most NaN; longer reductions go to the whole wave one after the other, every lane taking each n-th term (one
+// infinity in a column of x makes every output's sum over that column's rows non-finite, and a chunk of rows can be all of them: 4096 x 4096
+// weights, 30,000 rows, their gradient 27 ms with one, 7.7 without; lane by lane alone 93).  Fixed order: the same bits every run.
+__device__ inline float sum_again(float v, bool bad, const float *a, int64_t stride_a, const float *b, int64_t stride_b, int64_t k) {
+  constexpr int64_t kAlone = 64;
+  constexpr int U = 8; // terms of a lane in flight
+  bool left = false;
+  if (bad) {
+    const int64_t alone = k < kAlone ? k : kAlone;
+    v = 0.0f;
+    for (int64_t i = 0; i < alone && v == v; ++i) v = fmaf(a[i * stride_a], b[i * stride_b], v);
+    left = k > kAlone && v == v;
+  }
+  const int lane = threadIdx.x % 64;
+  const uint64_t on = __ballot(true);
+  const int64_t helpers = __popcll(on), rank = __popcll(on & (((uint64_t)1 << lane) - 1));
+  for (uint64_t todo = __ballot(left); todo; todo &= todo - 1) {
+    const int src = __builtin_ctzll(todo);
+    const float *pa = pointer_of_lane(a, src), *pb = pointer_of_lane(b, src);
+    float s = 0.0f;
+    for (int64_t i = rank; i < k; i += U * helpers) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t j = i + u * helpers;
+        if (j < k) s = fmaf(pa[j * stride_a], pb[j * stride_b], s);
+      }
+      if (__ballot(s != s)) break;
+    }
+    float total = 0.0f;
+    for (uint64_t h = on; h; h &= h - 1) total += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(s), __builtin_ctzll(h)));
+    v = lane == src ? total : v;
+  }
+  return v;
+}
+// ... of V elements a lane, b's `next` apart
+template <int V>
+__device__ inline void sums_again(float (&v)[V], int cols, const float *a, int64_t stride_a, const float *b, int64_t stride_b, int64_t next, int64_t k) {
+  bool any = false;
+#pragma unroll
+  for (int c = 0; c < V; ++c) any |= c < cols && !finite(v[c]);
+  if (__ballot(any) == 0) return;
+#pragma unroll 1
+  for (int c = 0; c < V; ++c) {
+    float one = v[0];
+#pragma unroll
+    for (int e = 1; e < V; ++e) one = c == e ? v[e] : one;
+    one = sum_again(one, c < cols && !finite(one), a, stride_a, b + c * next, stride_b, k);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = c == e ? one : v[e];
+  }
+}
+
 // ---- the products of one staged pair of tiles -----------------------------------------------------------------------------------
 // WM x WN waves over a BM x BN tile
 template <typename T, int BM, int BN, int WM, int WN> struct Accum {
@@ -375,15 +434,28 @@ template <typename T, int BM, int BN, int WM, int WN> struct Accum {
       for (int e = 0; e < 16; ++e) lds[(wm * 32 + row_of(e, lane)) * (BN + 4) + wn * (BN / WN) + j * 32 + lane % 32] = acc[i][j][e];
   }
   static __device__ int tile_row(int lr, int i) { return (lr / 32) * (BM / WM) + i * 32 + lr % 32; }
+  // Non-finite sums among those that this wave has put there, computed again (sum_again).  Element (row, col) of the tile: a + row * row_a,
+  // b + col * col_b, for rows < `rows`, columns < `cols`.
+  __device__ void again(float *lds, int i, int wm, int wn, int lane, const float *a, int64_t row_a, int64_t stride_a, const float *b, int64_t col_b, int64_t stride_b,
+                        int rows, int cols, int64_t k) const {
+    float any = 0.0f;
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) any = fmaf(acc[i][j][e], 0.0f, any);
+    if (__ballot(any != 0.0f) == 0) return; // (0, or NaN)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); // (the wave's own lanes wrote what is read here)
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int at = lane; at < 32 * (BN / WN); at += 64) {
+      const int lr = wm * 32 + at / (BN / WN), col = wn * (BN / WN) + at % (BN / WN), row = tile_row(lr, i);
+      float &v = lds[lr * (BN + 4) + col];
+      const bool bad = row < rows && col < cols && !finite(v);
+      if (__ballot(bad) == 0) continue;
+      v = sum_again(v, bad, a + row * row_a, stride_a, b + col * col_b, stride_b, k);
+    }
+  }
 };
-
-// One element in plain float32: the way of an infinity, a NaN or an overflow through a product of split operands.  A NaN ends it.
-__device__ float element_again(const float *a, int64_t stride_a, const float *b, int64_t stride_b, int64_t k) {
-  float s = 0.0f;
-  for (int64_t i = 0; i < k && s == s; ++i) s = fmaf(a[i * stride_a], b[i * stride_b], s);
-  return s;
-}
-__device__ inline bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 
 // max(z, 0) as a half sum: +inf and NaN stay, -inf becomes NaN (as -inf * 0 does)
 __device__ inline float positive_part(float z) { return fmaf(0.5f, fabsf(z), 0.5f * z); }
@@ -499,7 +571,8 @@ template <typename T, int ACT> __device__ inline float activation_gradient(float
   else return dy * activation_slope<T, ACT>(z);
 }
 template <int V> using Const = std::integral_constant<int, V>;
-template <typename F> __device__ __host__ inline void by_activation(int act, F f) {
+template <bool ANY = true, typename F> __device__ __host__ inline void by_activation(int act, F f) {
+  if constexpr (!ANY) return f(Const<GEOT_ACT_NONE>());
   switch (act) {
   case GEOT_ACT_RELU: f(Const<GEOT_ACT_RELU>()); break;
   case GEOT_ACT_GELU: f(Const<GEOT_ACT_GELU>()); break;
@@ -700,7 +773,7 @@ __device__ inline void finish_row(const RowsArgs &g, int64_t row, int64_t col, i
 }
 
 // A finished tile: 32 * WM rows at a time through LDS, so that every access to memory is whole rows, V consecutive columns a thread.  What
-// is read beside the sums (the residual, dy) is on its way before the barriers.  g.a and B: the operands of element_again.
+// is read beside the sums (the residual, dy) is on its way before the barriers.  g.a and B: the operands of sums_again.
 template <typename T, int BM, int BN, int WM, int WN, int ACT, bool DZ, bool BR>
 __device__ inline void tile_epilogue(const RowsArgs &g, const Accum<T, BM, BN, WM, WN> &acc, float *out, const T *ext, int64_t ld_ext, const T *B, int64_t r0, int64_t rows,
                                      int64_t nc, int cols, int64_t k_len, const float (&bias)[16 / sizeof(T)], float (&sum)[16 / sizeof(T)], int tid, int wm, int wn, int lane) {
@@ -718,6 +791,11 @@ __device__ inline void tile_epilogue(const RowsArgs &g, const Accum<T, BM, BN, W
     }
     if (i) __syncthreads();
     acc.put(out, i, wm, wn, lane);
+    if constexpr (Elem<T>::PARTS == 3) {
+      const int64_t n0 = nc - col;
+      acc.again(out, i, wm, wn, lane, static_cast<const float *>(g.a) + r0 * g.lda, g.lda, 1, reinterpret_cast<const float *>(B) + (BR ? n0 : n0 * g.ldb), BR ? 1 : g.ldb,
+                BR ? g.ldb : 1, (int)rows, (int)(g.n - n0 < BN ? g.n - n0 : BN), k_len);
+    }
     __syncthreads();
     if (cols > 0) {
 #pragma unroll
@@ -731,13 +809,6 @@ __device__ inline void tile_epilogue(const RowsArgs &g, const Accum<T, BM, BN, W
           const f32x4 q = *reinterpret_cast<const f32x4 *>(out + lr * (BN + 4) + col + c);
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[c + e] = q[e];
-        }
-        if constexpr (Elem<T>::PARTS == 3) {
-#pragma unroll
-          for (int c = 0; c < V; ++c)
-            if (!finite(v[c]) && c < cols)
-              v[c] = element_again(static_cast<const float *>(g.a) + row * g.lda, 1, reinterpret_cast<const float *>(B) + (BR ? nc + c : (nc + c) * g.ldb),
-                                   BR ? g.ldb : 1, k_len);
         }
         finish_row<T, V, ACT, DZ>(g, row, nc, cols, v, bias, ext != nullptr, pre[p], sum);
       }
@@ -819,7 +890,7 @@ __global__ __launch_bounds__(64 * WM * WN, NBUF == 1 ? 3 : 2) void mm_rows_kerne
 #pragma unroll
   for (int v = 0; v < V; ++v)
     bias[v] = g.bias && real && v < cols ? as_float(static_cast<const T *>(g.bias)[piece.group * g.bias_group + nc + v]) : 0.0f;
-  by_activation(g.act, [&](auto act) {
+  by_activation<!BR>(g.act, [&](auto act) { // (products with B laid out that way come without an activation)
     tile_epilogue<T, BM, BN, WM, WN, decltype(act)::value, false, BR>(g, acc, reinterpret_cast<float *>(lds), static_cast<const T *>(g.residual), g.ldr, B, r0, rows, nc, cols,
                                                                      k_len, bias, none, tid, wm, wn, lane);
   });
@@ -841,35 +912,30 @@ template <typename T, int BN, bool BR> __global__ __launch_bounds__(kThreads) vo
 #pragma unroll
   for (int v = 0; v < V; ++v)
     bias[v] = g.bias && real && v < cols ? as_float(static_cast<const T *>(g.bias)[piece.group * g.bias_group + nc + v]) : 0.0f;
-  by_activation(g.act, [&](auto act) {
-    for (int64_t row = r0 + threadIdx.x / TPR + (int64_t)blockIdx.y * RPP; row < end; row += (int64_t)gridDim.y * RPP) {
-      float v[V];
+  for (int64_t row = r0 + threadIdx.x / TPR + (int64_t)blockIdx.y * RPP; row < end; row += (int64_t)gridDim.y * RPP) {
+    float v[V];
 #pragma unroll
-      for (int c = 0; c < V; ++c) v[c] = 0.0f;
-      if (real) {
+    for (int c = 0; c < V; ++c) v[c] = 0.0f;
+    if (real) {
 #pragma unroll 4
-        for (uint32_t s = 0; s < shares; ++s) {
-          const float *p = g.part + ((int64_t)s * g.groups.rows + row) * g.n + nc;
+      for (uint32_t s = 0; s < shares; ++s) {
+        const float *p = g.part + ((int64_t)s * g.groups.rows + row) * g.n + nc;
 #pragma unroll
-          for (int c = 0; c < V; c += 4) {
-            const u32x4 q = load_cols<float, 4>(p + c, cols - c < 4 ? (cols > c ? cols - c : 0) : 4);
+        for (int c = 0; c < V; c += 4) {
+          const u32x4 q = load_cols<float, 4>(p + c, cols - c < 4 ? (cols > c ? cols - c : 0) : 4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[c + e] += __uint_as_float(q[e]);
-          }
-        }
-        if constexpr (Elem<T>::PARTS == 3) {
-          const float *B = static_cast<const float *>(g.b) + piece.group * g.b_group;
-#pragma unroll
-          for (int c = 0; c < V; ++c)
-            if (!finite(v[c]) && c < cols)
-              v[c] = element_again(static_cast<const float *>(g.a) + row * g.lda, 1, B + (BR ? nc + c : (nc + c) * g.ldb), BR ? g.ldb : 1, g.k);
+          for (int e = 0; e < 4; ++e) v[c + e] += __uint_as_float(q[e]);
         }
       }
-      u32x4 ext = {0, 0, 0, 0};
-      if (g.residual) ext = load_cols<T, V>(static_cast<const T *>(g.residual) + row * g.ldr + nc, cols);
-      finish_row<T, V, decltype(act)::value, false>(g, row, nc, cols, v, bias, g.residual != nullptr, ext, none);
+      if constexpr (Elem<T>::PARTS == 3) {
+        const float *B = static_cast<const float *>(g.b) + piece.group * g.b_group;
+        sums_again<V>(v, cols, static_cast<const float *>(g.a) + row * g.lda, 1, B + (BR ? nc : nc * g.ldb), BR ? g.ldb : 1, BR ? 1 : g.ldb, g.k);
+      }
     }
-  });
+    u32x4 ext = {0, 0, 0, 0};
+    if (g.residual) ext = load_cols<T, V>(static_cast<const T *>(g.residual) + row * g.ldr + nc, cols);
+    by_activation<!BR>(g.act, [&](auto act) { finish_row<T, V, decltype(act)::value, false>(g, row, nc, cols, v, bias, g.residual != nullptr, ext, none); });
+  }
 }
 
 // dz = dy act'(z) with z = x W^T + b computed again instead of read: narrow layers are bound by memory, and z costs a write in the forward
@@ -1012,12 +1078,8 @@ template <typename T, int FM> __global__ __launch_bounds__(512, 2) void mm_few_r
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[c + e] += q[e];
       }
-    if constexpr (E::PARTS == 3) {
-#pragma unroll
-      for (int c = 0; c < V; ++c)
-        if (!finite(v[c]) && c < cols)
-          v[c] = element_again(static_cast<const float *>(g.a) + (r0 + lr) * g.lda, 1, static_cast<const float *>(g.b) + (nc + c) * g.ldb, 1, g.k);
-    }
+    if constexpr (E::PARTS == 3)
+      sums_again<V>(v, cols, static_cast<const float *>(g.a) + (r0 + lr) * g.lda, 1, static_cast<const float *>(g.b) + nc * g.ldb, 1, g.ldb, g.k);
     u32x4 ext = {0, 0, 0, 0};
     if (g.residual) ext = load_cols<T, V>(static_cast<const T *>(g.residual) + (r0 + lr) * g.ldr + nc, cols);
     by_activation(g.act, [&](auto act) { finish_row<T, V, decltype(act)::value, false>(g, r0 + lr, nc, cols, v, bias, g.residual != nullptr, ext, none); });
@@ -1092,6 +1154,9 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 && BN == 64 ? 4 : 3) void mm
   for (int i = 0; i < acc.FM; ++i) {
     if (i) __syncthreads();
     acc.put(out, i, wm, wn, lane);
+    if constexpr (E::PARTS == 3)
+      acc.again(out, i, wm, wn, lane, reinterpret_cast<const float *>(P) + r0 * g.ldp + i0, 1, g.ldp, reinterpret_cast<const float *>(Q) + r0 * g.ldq + j0, 1, g.ldq,
+                (int)(g.np - i0 < BM ? g.np - i0 : BM), (int)(g.nq - j0 < BN ? g.nq - j0 : BN), k_len);
     __syncthreads();
     for (int lr = tid / (BN / 4); lr < 32 * WM; lr += NT / (BN / 4)) {
       const int64_t row = i0 + acc.tile_row(lr, i);
@@ -1100,16 +1165,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM == 64 && BN == 64 ? 4 : 3) void mm
       const int64_t cc = j0 + col;
       if (cc >= g.nq) continue;
       const int cols = g.nq - cc < 4 ? (int)(g.nq - cc) : 4;
-      alignas(16) float v[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        v[c] = q[c];
-        if constexpr (E::PARTS == 3) {
-          if (!finite(v[c]) && c < cols)
-            v[c] = element_again(reinterpret_cast<const float *>(P) + r0 * g.ldp + row, g.ldp, reinterpret_cast<const float *>(Q) + r0 * g.ldq + cc + c, g.ldq,
-                                 k_len);
-        }
-      }
+      alignas(16) float v[4] = {q[0], q[1], q[2], q[3]};
       if (whole) {
         T *o = static_cast<T *>(g.out) + (piece.group * g.np + row) * g.nq + cc;
         alignas(16) T tmp[4];

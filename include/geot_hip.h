@@ -387,6 +387,8 @@ int geot_slab_mh_sddmm(const geot_slab_plan *plan, const void *mat_1, const void
  * the distance of two rows in elements (>= the row's width, or 0 for one repeated row), every other operand is dense.  Operands need no alignment beyond their
  * element's.  No call allocates or synchronises; results do not depend on the launch (no atomics).  float32 products are exact to about
  * 2^-23 of |xy| each (computed on the bfloat16 cores in three parts); a factor below 2^-110 keeps an absolute 2^-133.
+ * A float32 sum that comes out non-finite is computed a second time in plain float32 (an infinity in the operands costs time: its row's or
+ * column's sums are read again, a wave a sum).
  *
  * Workspaces: ..._workspace_bytes of the call (0 where it needs none - products of few tiles split their reduction over workgroups), 16-byte
  * aligned, no content expected, free after the call.

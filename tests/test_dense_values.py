@@ -281,3 +281,37 @@ def test_segment_gradients_of_chunked_groups(dtype):
         for run in runs:
             # (bfloat16 holds whole numbers up to 256; sums of 769 numbers of -1, 0, 1 stay below: 6 standard deviations are 150)
             assert torch.equal(run[0][i].double(), dw) and torch.equal(run[1][i].double(), db), i
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n", [(200, 200, 72), (33, 300, 40), (100, 4160, 48), (1500, 70, 130)], ids=["tile", "few", "split", "chunks"])
+def test_nonfinite_sums_of_long_reductions(m, k, n):
+    """float32 sums that end in an infinity or NaN, decided by terms far behind the first: y, dx and dW of linear and segment_matmul have
+    them where float64 arithmetic has, and everything else within the products' bound (6 partial products of 2^-23 steps a term).  Left
+    out: sums whose finite terms pass float32's range in absolute value, of both signs or beside an infinity - a term or a partial sum
+    becomes an infinity of either sign in float32 arithmetic, and it ends in an infinity, NaN or a number as its order has it."""
+    g = torch.Generator().manual_seed(m)
+    x, w, dy = (torch.randn(*s, generator=g).cuda() for s in ((m, k), (n, k), (m, n)))
+    x[3, k - 2], x[5, 1], x[5, k - 1], x[m - 1, k // 2] = INF, INF, -INF, NAN
+    w[n - 1, 2], w[1, k - 3] = -INF, NAN
+    dy[m - 2, n - 2], dy[m // 2, 0], dy[0, 5], dy[m - 3, 5] = INF, NAN, 3e38, 3e38
+    x[0, 0], x[m - 3, 0] = 2.0, 2.0                          # (dW[5, 0]: 2 * 3e38 twice)
+    ptr = torch.tensor([0, m], device="cuda")
+
+    def check(got, a, b, what):
+        want, most = a.double() @ b.double(), torch.finfo(torch.float32).max
+        size = a.double().nan_to_num(0, 0, 0).abs() @ b.double().nan_to_num(0, 0, 0).abs()
+        open_ended = (size > most) & (torch.isinf(want) | (torch.isfinite(want) & (want.abs() < 0.99 * size)))
+        want = torch.where(want.abs() > most, want.sign() * INF, want)
+        got, want, size = got.double()[~open_ended], want[~open_ended], size[~open_ended]
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+        assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)]) and torch.equal(torch.isinf(got), torch.isinf(want)), what
+        off = (got - want).abs() > (6 * a.shape[1] + 16) * 2.0 ** -23 * size
+        assert not (off & torch.isfinite(want)).any(), what
+
+    xg, wg, w3 = x.clone().requires_grad_(), w.clone().requires_grad_(), w.t()[None].contiguous().requires_grad_()
+    for y, weight, flip in ((geot.linear(xg, wg), wg, False), (geot.segment_matmul(xg, ptr, w3), w3, True)):
+        dx, dw = torch.autograd.grad(y, [xg, weight], dy)
+        check(y, x, w.t().contiguous(), "y")
+        check(dx, dy, w, "dx")
+        check(dw[0].t() if flip else dw, dy.t().contiguous(), x, "dw")
