@@ -940,7 +940,10 @@ template <typename T, int BN, bool BR> __global__ __launch_bounds__(kThreads) vo
 
 // dz = dy act'(z) with z = x W^T + b computed again instead of read: narrow layers are bound by memory, and z costs a write in the forward
 // pass and a read here where x, which the weight's gradient reads anyway, is all this needs (2.4 M x 128 -> 256 bf16: 3.8 GB and 850 us
-// for dz from a saved z, 3.1 GB so, and the forward pass writes 1.3 GB less).  z is not rounded on its way.  Column sums of dz - the bias's
+// for dz from a saved z, 3.1 GB so, and the forward pass writes 1.3 GB less).  z is not rounded on its way; dz is, to the
+// operands' type, like the dz of act_backward_kernel: dx and dW take it as a matrix operand, and in float32 its write and two reads would
+// move 3.8 GB more of that layer's 6.9 and double both products.  What it costs: dx and dW 2.4e-3 off in 2-norm where one rounding is 1.7e-3
+// (bfloat16).  Column sums of dz - the bias's
 // gradient - are taken before its rounding, one row of partial sums a row tile.  (One workgroup over several row tiles spilled 70 registers: 2057 us.)
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, 3) void mm_preactivation_kernel(const RowsArgs g, const T *dy, float *part) {

@@ -607,9 +607,13 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     """``act(x @ weight.T + bias) + residual`` in one kernel: x [..., in], weight [out, in] (torch.nn.Linear's layout), bias [out],
     residual [..., out]; ``activation``: 'none', 'relu', 'gelu' (the error-function form) or 'silu'.
 
-    float32, float16 or bfloat16, one dtype for all operands; sums in float32, one rounding.  Differentiable in every tensor (in reverse
-    mode; the backward pass itself is not).  A training call of a wide layer keeps the pre-activation in the operands' dtype; a narrow one (in <= 256,
-    float32 128) computes it again in the backward pass, and 'none', and 'relu' without a residual, do not need it."""
+    float32, float16 or bfloat16, one dtype for all operands; sums in float32, ``out`` rounded once.  Differentiable in every tensor (in
+    reverse mode; the backward pass itself is not).  With 16-bit operands and an activation, the gradient of the pre-activation is rounded to
+    their dtype before the products that make the gradients of x and weight (in 2-norm, two roundings where a float32 one in between would
+    leave one: 2.4e-3 instead of 1.7e-3 for bfloat16, 2.9e-4 instead of 2.1e-4 for float16), the bias's gradient is summed before it.  A
+    training call of a wide layer also keeps the pre-activation in the operands' dtype, and takes the activation's slope there; a narrow one
+    (in <= 256, float32 128) computes it again in the backward pass, unrounded, and 'none', and 'relu' without a residual, do not need it.
+    16-bit gelu is a fit to 2^-15 of the value (2^-13 below -10).  A factor of a float32 product below 2^-110 keeps an absolute 2^-133."""
     return torch.ops.geot_dense.linear(x, weight, bias, residual, activation)
 
 
@@ -619,11 +623,11 @@ def segment_matmul(x: torch.Tensor, ptr: torch.Tensor, weight: torch.Tensor, bia
 
     x [rows, in], ptr int64 [groups + 1] ascending, on the GPU (never read back: the call does not synchronise), weight
     [groups, in, out], bias [groups, out]; float32, float16 or bfloat16.  Groups may be empty; rows in front of ptr[0] and behind ptr[-1]
-    come out 0.  Entries of ptr that do not ascend leave the result unspecified.  Differentiable in x, weight and bias."""
+    come out 0.  Entries of ptr that do not ascend leave the result unspecified.  Differentiable in x, weight and bias, in reverse mode."""
     return torch.ops.geot_dense.segment_matmul(x, ptr, weight, bias)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """Normalisation of the last dimension: ``(x - mean) / sqrt(var + eps) * weight + bias``; weight / bias [x.shape[-1]], of x's dtype or
-    float32.  float32, float16 or bfloat16 rows, statistics in float32.  Differentiable in x, weight and bias."""
+    float32.  float32, float16 or bfloat16 rows, statistics in float32.  Differentiable in x, weight and bias, in reverse mode."""
     return torch.ops.geot_dense.layer_norm(x, weight, bias, eps)
