@@ -28,6 +28,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <cstdio>
 #include <type_traits>
 
 #include "geot_hip.h"
@@ -1369,6 +1370,12 @@ size_t rows_workspace(int64_t rows, int64_t groups, bool with_ptr, int64_t n, in
   const int64_t share = rows_share(rows, groups, with_ptr, n, k, dtype == GEOT_F32);
   return share < k ? (size_t)((k + share - 1) / share) * (size_t)rows * (size_t)n * sizeof(float) : 0;
 }
+template <typename T, int BM, int BN, int WM, int WN, bool BR, int NBUF> int launched_rows(bool split) {
+  char name[96];
+  snprintf(name, sizeof name, "mm_rows_kernel<%s, %d, %d, %d, %d, %s, %d, %s>", std::is_same<T, float>::value ? "float" : std::is_same<T, f16>::value ? "_Float16" : "__bf16",
+           BM, BN, WM, WN, BR ? "true" : "false", NBUF, split ? "true" : "false");
+  return launched(name);
+}
 template <typename T, int BM, int BN, int WM, int WN, bool BR, int NBUF> int run_rows(RowsArgs &g, hipStream_t st) {
   const int64_t tiles_n = (g.n + BN - 1) / BN, slots = slots_of(g.groups.rows, g.groups.groups, g.groups.ptr != nullptr, BM);
   if (tiles_n > kMaxBlocks / 8 || slots > kMaxBlocks / tiles_n) return geot_internal_fail(GEOT_EINVAL, "more tiles than one launch can hold");
@@ -1382,13 +1389,13 @@ template <typename T, int BM, int BN, int WM, int WN, bool BR, int NBUF> int run
       const unsigned shares = (unsigned)((g.k + share - 1) / share);
       g.k_share = share;
       hipLaunchKernelGGL((mm_rows_kernel<T, BM, BN, WM, WN, BR, NBUF, true>), dim3(blocks, shares), dim3(64 * WM * WN), 0, st, g);
-      if (const int rc = launched("mm_rows_kernel")) return rc;
+      if (const int rc = launched_rows<T, BM, BN, WM, WN, BR, NBUF>(true)) return rc;
       hipLaunchKernelGGL((mm_rows_join_kernel<T, BN, BR>), dim3(blocks, 4), dim3(kThreads), 0, st, g, shares);
       return launched(nullptr);
     }
   }
   hipLaunchKernelGGL((mm_rows_kernel<T, BM, BN, WM, WN, BR, NBUF, false>), dim3(blocks), dim3(64 * WM * WN), 0, st, g);
-  return launched("mm_rows_kernel");
+  return launched_rows<T, BM, BN, WM, WN, BR, NBUF>(false);
 }
 template <typename T, int FM> int run_few(RowsArgs &g, hipStream_t st) {
   g.tiles_n = (uint32_t)((g.n + 31) / 32);

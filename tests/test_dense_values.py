@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import geot_amd as geot
+from test_dense_ops import LinearReference, close
 
 gpu = pytest.mark.gpu
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -347,3 +348,73 @@ def test_roundings_of_a_training_step(k, act, dtype):
     assert relative_error(db, dz.sum(0)) <= 1.02 * math.sqrt(1 + kept ** 2) * one
     assert relative_error(dx, dz @ w.double()) <= 1.02 * many
     assert relative_error(dw, dz.t().contiguous() @ x.double()) <= 1.02 * many
+
+
+def _edges_of_tiles(m, tile=256):
+    """Rows to look at: ends of the first and last tiles, both sides of their borders, some between."""
+    g = torch.Generator().manual_seed(m)
+    last = m // tile * tile
+    near = [0, 1, 31, 127, 128, tile - 1, tile, tile + 1, 2 * tile - 1, last - 1]
+    return torch.cat([torch.tensor(near), torch.randint(0, m, (60,), generator=g), torch.arange(last, m)]).unique().cuda()
+
+
+# 16-bit rows and 512 or more values a sum: 256 x 256 tiles, two buffers; reductions of whole steps of 64 and not, odd and even in number
+WIDE = [(66_001, 602, 258), (66_000, 520, 300), (66_301, 576, 256), (66_000, 640, 511)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("m,k,n", WIDE)
+def test_linear_in_large_tiles(m, k, n, dtype):
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x, r = (torch.randn(m, c, generator=g, device="cuda").to(dtype) for c in (k, n))
+    w, b = (torch.randn(n, k, generator=g, device="cuda") * k ** -0.5).to(dtype), torch.randn(n, generator=g, device="cuda").to(dtype)
+    rows = _edges_of_tiles(m)
+    one = 1.02 * torch.finfo(dtype).eps / math.sqrt(12)
+    kind = {torch.float16: "_Float16", torch.bfloat16: "__bf16"}[dtype]
+    for act, bias, res in (("none", None, None), ("gelu", b, r)):
+        y = geot.linear(x, w, bias, residual=res, activation=act)
+        assert geot.hip.last_kernel() == f"mm_rows_kernel<{kind}, 256, 256, 2, 4, false, 2, false>"
+        ref = LinearReference(x[rows], w, bias, None if res is None else r[rows], act)
+        close(y[rows], ref.y, ref.e_y, f"y {act}")
+        assert relative_error(y[rows], ref.y) <= one
+        whole = torch.nn.functional.linear(x, w, bias)       # (every row: no tile left out or written twice; another library's rounding beside)
+        whole = whole if act == "none" else torch.nn.functional.gelu(whole) + r
+        assert float((y.float() - whole.float()).abs().max()) <= 8 * torch.finfo(dtype).eps * float(whole.float().abs().max())
+    # the gradient of the input, where the weight's output index is contiguous
+    w2 = (torch.randn(k, n, generator=g, device="cuda") * k ** -0.5).to(dtype)
+    x2 = torch.zeros(m, n, dtype=dtype, device="cuda")
+    dx = torch.ops.geot_dense.linear_backward(x, x2, w2, None, x2[:0, 0], "none", True, False, False)[0]    # (in this thread, for last_kernel)
+    assert geot.hip.last_kernel() == f"mm_rows_kernel<{kind}, 256, 256, 2, 4, true, 2, false>"
+    ref = LinearReference(x[rows], w2.t(), None, None, "none")
+    close(dx[rows], ref.y, ref.e_y, "dx")
+    assert relative_error(dx[rows], ref.y) <= one
+    whole = x.float() @ w2.float()
+    assert float((dx.float() - whole).abs().max()) <= 8 * torch.finfo(dtype).eps * float(whole.abs().max())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=IDS[1:])
+def test_segment_matmul_in_large_tiles(dtype):
+    """Two groups above 2048 rows and an odd border, rows in front of and behind them: both directions in 256 x 256 tiles."""
+    m, k, n, ptr = 66_000, 520, 602, [3, 30_001, 65_990]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, dy = (torch.randn(m, c, generator=g, device="cuda").to(dtype) for c in (k, n))
+    w = (torch.randn(2, k, n, generator=g, device="cuda") * k ** -0.5).to(dtype)
+    at = torch.tensor(ptr, device="cuda")
+    y = geot.segment_matmul(x, at, w)
+    kind = {torch.float16: "_Float16", torch.bfloat16: "__bf16"}[dtype]
+    assert geot.hip.last_kernel() == f"mm_rows_kernel<{kind}, 256, 256, 2, 4, true, 2, false>"
+    dx = torch.ops.geot_dense.segment_matmul_backward(dy, x, at, w, True, False, False)[0]
+    assert geot.hip.last_kernel() == f"mm_rows_kernel<{kind}, 256, 256, 2, 4, false, 2, false>"
+    for got in (y, dx):
+        assert not got[:3].any() and not got[65_990:].any()
+    one = 1.02 * torch.finfo(dtype).eps / math.sqrt(12)
+    for i, (lo, hi) in enumerate(zip(ptr[:-1], ptr[1:])):
+        rows = _edges_of_tiles(hi - lo) + lo
+        for got, a, b in ((y, x, w[i].t()), (dx, dy, w[i])):
+            ref = LinearReference(a[rows], b, None, None, "none")
+            close(got[rows], ref.y, ref.e_y, "y" if got is y else "dx")
+            assert relative_error(got[rows], ref.y) <= one
+            whole = a[lo:hi].float() @ b.float().t()
+            assert float((got[lo:hi].float() - whole).abs().max()) <= 8 * torch.finfo(dtype).eps * float(whole.abs().max())
