@@ -418,3 +418,157 @@ def test_segment_matmul_in_large_tiles(dtype):
             assert relative_error(got[rows], ref.y) <= one
             whole = a[lo:hi].float() @ b.float().t()
             assert float((got[lo:hi].float() - whole).abs().max()) <= 8 * torch.finfo(dtype).eps * float(whole.abs().max())
+
+
+# ---- float32 products: 24 bits on every path, errors in root mean square -------------------------------------------------------------------
+def _numbers(*shape, seed):
+    """Significands of 24 random bits, exponents spread over 2^-40 .. 2^40."""
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * 2.0 ** torch.randint(-40, 41, shape, generator=g)).cuda()
+
+
+def _ones_and_numbers(n, seed):
+    v = _numbers(n, seed=seed)
+    v[::3] = -0.125
+    return v
+
+
+def _last_place(got, want):
+    """A product of two 24-bit significands: half a step of its rounding, 2^-23 left out of the split product, a step of the sums it passes."""
+    off = (got.double() - want).abs() > 2.0 ** -21.5 * want.abs()
+    assert got.shape == want.shape and not off.any(), (got[off], want[off])
+
+
+# rows, in, out: one and many rows, tiles, few rows (one and two row fragments), a split reduction
+SELECT = [(1, 256, 40), (20, 640, 72), (70, 300, 33), (200, 96, 96), (100, 4160, 48), (300, 64, 200)]
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n", SELECT)
+def test_float32_keeps_24_bits_forward_and_dx(m, k, n):
+    """One entry a row of the weight: every result is one product."""
+    x, w = _numbers(m, k, seed=m), torch.zeros(n, k, device="cuda")
+    at = torch.randint(0, k, (n,), generator=torch.Generator().manual_seed(n)).cuda()
+    v = _ones_and_numbers(n, 3)
+    w[torch.arange(n, device="cuda"), at] = v
+    want = x.double()[:, at] * v.double()
+    ptr = torch.tensor([0, m // 3, m], device="cuda")
+    _last_place(geot.linear(x, w), want)
+    _last_place(geot.segment_matmul(x, ptr, torch.stack([w.t(), w.t()])), want)
+    # dx = dy W with W [k, n] of one entry a column: the same products
+    dy, empty = x, torch.empty(0, device="cuda")
+    w2 = w.t().contiguous()
+    dx = torch.ops.geot_dense.linear_backward(dy, torch.zeros(m, n, device="cuda"), w2, None, empty, "none", True, False, False)[0]
+    _last_place(dx, want)
+    dx = torch.ops.geot_dense.segment_matmul_backward(dy, torch.zeros(m, n, device="cuda"), ptr, torch.stack([w, w]), True, False, False)[0]
+    _last_place(dx, want)
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n", [(1, 5, 7), (100, 64, 64), (2000, 48, 130), (5000, 130, 48), (1500, 70, 64), (900, 200, 300)])
+def test_float32_keeps_24_bits_dw(m, k, n):
+    """One row with an entry for every output: dW is one product each, in one of several chunks of rows."""
+    x, dy = _numbers(m, k, seed=m), torch.zeros(m, n, device="cuda")
+    at = torch.randint(0, m, (n,), generator=torch.Generator().manual_seed(n)).cuda()
+    v = _ones_and_numbers(n, 4)
+    dy[at, torch.arange(n, device="cuda")] = v
+    want = v.double()[:, None] * x.double()[at]
+    dw, db = torch.ops.geot_dense.linear_backward(dy, x, torch.zeros(n, k, device="cuda"), torch.zeros(n, device="cuda"), torch.empty(0, device="cuda"), "none",
+                                                  False, True, True)[1:]
+    _last_place(dw, want)
+    assert torch.equal(db, v)
+    ptr = torch.tensor([0, 0, m, m], device="cuda")
+    dw, db = torch.ops.geot_dense.segment_matmul_backward(dy, x, ptr, torch.zeros(3, k, n, device="cuda"), False, True, True)[1:]
+    _last_place(dw[1].t(), want)
+    assert torch.equal(db[1], v) and not dw[[0, 2]].any() and not db[[0, 2]].any()
+
+
+@gpu
+def test_float32_keeps_24_bits_where_z_is_computed_again():
+    """dz = dy silu'(z) with z = one product: the slope (2^-20 of its size, see above) of a z that lost its third part, 2^-17 of it, shows."""
+    m, k = 400, 96
+    g = torch.Generator().manual_seed(5)
+    x, w = (3 * torch.randn(m, k, generator=g)).cuda(), torch.zeros(k, k, device="cuda")
+    v = (torch.rand(k, generator=g) + 0.5).cuda()
+    w[torch.arange(k, device="cuda"), torch.randperm(k, generator=g).cuda()] = v
+    x.requires_grad_()
+    y = geot.linear(x, w, activation="silu")
+    (dx,) = torch.autograd.grad(y, [x], torch.ones_like(y))
+    z = x.detach().double() @ w.double().t().contiguous()
+    dz = slope64(z, "silu")
+    assert relative_error(dx, dz @ w.double()) <= 2.0 ** -21
+    assert relative_error(y, act64(z, "silu")) <= 2.0 ** -21
+
+
+def rms_bound(k):
+    """Of a float32 product's error over its size, both in root mean square: the long sum rounds once for 16 to 64 values of the reduction (a
+    random walk, every step at most 2^-23 of the sum so far), in between 6 to 24 matrix instructions may truncate, which shrinks a sum by up
+    to 2^-24 each, half of it on average.  Without an operand's third part it is 2^-18.8 and more."""
+    return (12 + 2 * math.sqrt(k / 32)) * 2.0 ** -24
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n", [(1, 256, 512), (20, 520, 200), (70, 1000, 130), (300, 200, 96), (300, 1000, 72), (100, 4160, 48), (1000, 64, 64)])
+def test_float32_errors_in_root_mean_square(m, k, n):
+    g = torch.Generator().manual_seed(m + k + n)
+    x, w, dy = (torch.randn(*s, generator=g).cuda() for s in ((m, k), (n, k), (m, n)))
+    ptr = torch.tensor([0, m], device="cuda")
+    x.requires_grad_()
+    for weight, f in ((w.clone().requires_grad_(), geot.linear), (w.t()[None].contiguous().requires_grad_(), lambda x, w: geot.segment_matmul(x, ptr, w))):
+        y = f(x, weight)
+        dx, dw = torch.autograd.grad(y, [x, weight], dy)
+        x64, w64, dy64 = x.detach().double(), w.double(), dy.double()
+        assert relative_error(y, x64 @ w64.t().contiguous()) <= rms_bound(k)
+        assert relative_error(dx, dy64 @ w64) <= rms_bound(n)
+        assert relative_error(dw if dw.dim() == 2 else dw[0].t(), dy64.t().contiguous() @ x64) <= rms_bound(m)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_many_rows_in_root_mean_square(dtype):
+    """Sums over 70,001 rows: a row left out is 1 / sqrt(70001) = 2^-8 of dW and db, a chunk 2^-4; the bounds are one rounding of the
+    result and the sums' own (float32: rms_bound of all rows)."""
+    m, k, n = 70_001, 40, 24
+    g = torch.Generator().manual_seed(9)
+    x, dy = (torch.randn(m, c, generator=g).to(dtype).cuda() for c in (k, n))
+    bound = rms_bound(m) if dtype == torch.float32 else 1.02 * torch.finfo(dtype).eps / math.sqrt(12)
+    w, b = torch.zeros(n, k, dtype=dtype, device="cuda", requires_grad=True), torch.zeros(n, dtype=dtype, device="cuda", requires_grad=True)
+    dw, db = torch.autograd.grad(geot.linear(x, w, b), [w, b], dy)
+    assert relative_error(dw, dy.double().t().contiguous() @ x.double()) <= bound
+    assert relative_error(db, dy.double().sum(0)) <= bound
+    # relu at z = 0.5: dz = dy through the activation's own column sums
+    half = torch.full((n,), 0.5, dtype=dtype, device="cuda", requires_grad=True)
+    dw, db = torch.autograd.grad(geot.linear(x, w, half, activation="relu"), [w, half], dy)
+    assert relative_error(dw, dy.double().t().contiguous() @ x.double()) <= bound
+    assert relative_error(db, dy.double().sum(0)) <= bound
+    ptr = torch.tensor([1, 30_000, 30_000, 70_000], device="cuda")
+    w3, b3 = torch.zeros(3, k, n, dtype=dtype, device="cuda", requires_grad=True), torch.zeros(3, n, dtype=dtype, device="cuda", requires_grad=True)
+    dw, db = torch.autograd.grad(geot.segment_matmul(x, ptr, w3, b3), [w3, b3], dy)
+    for i, (lo, hi) in enumerate(((1, 30_000), (30_000, 30_000), (30_000, 70_000))):
+        if lo == hi:
+            assert not dw[i].any() and not db[i].any()
+            continue
+        assert relative_error(dw[i], x[lo:hi].double().t().contiguous() @ dy[lo:hi].double()) <= bound
+        assert relative_error(db[i], dy[lo:hi].double().sum(0)) <= bound
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m,d", [(60_011, 24), (3001, 602), (501, 2100), (401, 5000), (301, 9000)])
+def test_layer_norm_in_root_mean_square(m, d, dtype):
+    """y, dx, dw and db: one rounding of the result, and float32 sums of the row (at most 2 sqrt(d / 256) + 12 roundings of 2^-24) and over the
+    rows (as many per partial row, then their join): 64 * 2^-24 holds all.  A row left out of dw or db is 1 / sqrt(m): 2^-8 and more."""
+    g = torch.Generator().manual_seed(d)
+    x, dy, w, b = (torch.randn(*s, generator=g).to(dtype).cuda().requires_grad_() for s in ((m, d), (m, d), (d,), (d,)))
+    bound = 64 * 2.0 ** -24 + (0 if dtype == torch.float32 else 1.02 * torch.finfo(dtype).eps / math.sqrt(12))
+    y = geot.layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], dy.detach())
+    x64, dy64, w64, b64 = (t.detach().double() for t in (x, dy, w, b))
+    var, mean = torch.var_mean(x64, -1, unbiased=False, keepdim=True)
+    s = (var + 1e-5).rsqrt()
+    h = (x64 - mean) * s
+    gw = dy64 * w64
+    assert relative_error(y, h * w64 + b64) <= bound
+    assert relative_error(dx, s * (gw - gw.mean(-1, keepdim=True) - h * (gw * h).mean(-1, keepdim=True))) <= bound
+    assert relative_error(dw, (dy64 * h).sum(0)) <= bound
+    assert relative_error(db, dy64.sum(0)) <= bound
