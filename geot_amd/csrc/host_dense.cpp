@@ -267,7 +267,7 @@ std::tuple<at::Tensor, at::Tensor> layer_norm_train_op(const at::Tensor &x, cons
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_backward_op(const at::Tensor &grad_in, const at::Tensor &x_in, const c10::optional<at::Tensor> &w_in,
-                                                                      const c10::optional<at::Tensor> &b_in, const at::Tensor &stats, bool need_params) {
+                                                                      const c10::optional<at::Tensor> &b_in, const at::Tensor &stats, bool need_x, bool need_params) {
   const auto p = check_norm(x_in, w_in, b_in);
   TORCH_CHECK(grad_in.sizes() == x_in.sizes() && grad_in.scalar_type() == x_in.scalar_type(), "layer_norm: the gradient must have the output's shape and dtype");
   require_gpu("layer_norm", {&grad_in, &x_in, ptr_of(w_in), &stats});
@@ -278,9 +278,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_backward_op(const at::
   const at::Tensor dy = grad_in.contiguous();
   const auto w = dense(w_in);
   const int64_t feat = x_in.size(-1);
-  at::Tensor dx = at::empty(x_in.sizes(), x_in.options()), dw = at::empty({need_params ? feat : 0}, x_in.options().dtype(p)), db = at::empty_like(dw);
+  at::Tensor dx = need_x ? at::empty(x_in.sizes(), x_in.options()) : at::empty({0}, x_in.options()), dw = at::empty({need_params ? feat : 0}, x_in.options().dtype(p)), db = at::empty_like(dw);
   const at::Tensor ws = scratch(x_in, need_params ? geot_layer_norm_backward_workspace_bytes(x.rows, feat) : 0);
-  GEOT_CALL(geot_layer_norm_backward(x.t.data_ptr(), x.ld, data_of(w), stats.data_ptr<float>(), dy.data_ptr(), dx.data_ptr(), need_params ? dw.data_ptr() : nullptr,
+  GEOT_CALL(geot_layer_norm_backward(x.t.data_ptr(), x.ld, data_of(w), stats.data_ptr<float>(), dy.data_ptr(), need_x ? dx.data_ptr() : nullptr, need_params ? dw.data_ptr() : nullptr,
                                      need_params ? db.data_ptr() : nullptr, x.rows, feat, dt, param_code(p), ws.data_ptr(), ws.numel(), stream_of(x_in)));
   return std::make_tuple(dx, dw, db);
 }
@@ -398,7 +398,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
     size_t at = 1; // (inputs that were not given are not counted)
     const bool nx = ctx->needs_input_grad(0), nw = saved[1].defined() && ctx->needs_input_grad(at++), nb = saved[2].defined() && ctx->needs_input_grad(at);
     static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("geot_dense::layer_norm_backward", "").typed<decltype(layer_norm_backward_op)>();
-    auto [dx, dw, db] = op.call(grads[0], saved[0], or_none(saved[1]), or_none(saved[2]), saved[3], nw || nb);
+    auto [dx, dw, db] = op.call(grads[0], saved[0], or_none(saved[1]), or_none(saved[2]), saved[3], nx, nw || nb);
     out[0] = if_needed(nx, dx);
     out[1] = if_needed(nw, dw);
     out[2] = if_needed(nb, db);
@@ -424,7 +424,7 @@ TORCH_LIBRARY_FRAGMENT(geot_dense, m) {
   m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor", layer_norm_op);
   m.def("layer_norm_forward(Tensor x, Tensor? weight, Tensor? bias, float eps, bool save) -> (Tensor, Tensor)");
   m.def("layer_norm_train(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor)");
-  m.def("layer_norm_backward(Tensor grad, Tensor x, Tensor? weight, Tensor? bias, Tensor stats, bool need_params) -> (Tensor, Tensor, Tensor)");
+  m.def("layer_norm_backward(Tensor grad, Tensor x, Tensor? weight, Tensor? bias, Tensor stats, bool need_x, bool need_params) -> (Tensor, Tensor, Tensor)");
 }
 
 // (the CPU key runs the argument checks and then refuses CPU tensors, as the package's other GPU-only operators do)

@@ -118,7 +118,7 @@ __device__ inline float rounded_product(float a, float b) {
 
 struct NormArgs {
   const void *x, *weight, *bias, *dy;
-  void *y, *dx;      // forward / backward result
+  void *y, *dx;      // forward / backward result (dx null where it is not asked for)
   float *stats;      // [3, rows]
   float *part;       // backward: [blocks, 2, feat], null where no parameter gradient is asked for
   int64_t ldx, rows, feat;
@@ -198,6 +198,7 @@ template <typename T, typename P, int L, int EPL> __global__ __launch_bounds__(k
       db[e] += dy[e];
       dy[e] = t;
     }
+    if (!g.dx) continue; // (the parameters' gradients alone)
     all.sum(s, q);
     s *= inv;
     q *= inv;
@@ -374,9 +375,9 @@ template <typename T, typename P> int forward(const NormArgs &g, hipStream_t st)
 }
 template <typename T, typename P> int backward(NormArgs &g, void *dweight, void *dbias, hipStream_t st) {
   const int64_t d = g.feat, blocks = backward_blocks(g.rows, d);
-  if (g.rows > 0 || g.part) {
+  if ((g.rows > 0 && g.dx) || g.part) {
     if (d > kWide) {
-      if (g.rows > 0) hipLaunchKernelGGL((norm_wide_backward_kernel<T, P>), dim3((unsigned)(g.rows < 4096 ? g.rows : 4096)), dim3(kThreads), 0, st, g);
+      if (g.rows > 0 && g.dx) hipLaunchKernelGGL((norm_wide_backward_kernel<T, P>), dim3((unsigned)(g.rows < 4096 ? g.rows : 4096)), dim3(kThreads), 0, st, g);
       if (g.part) hipLaunchKernelGGL((norm_wide_params_kernel<T>), dim3((unsigned)((d + kThreads - 1) / kThreads), (unsigned)blocks), dim3(kThreads), 0, st, g);
     } else {
       NORM_SHAPES(run_backward);
@@ -430,7 +431,7 @@ int geot_layer_norm_backward(const void *x, int64_t ldx, const void *weight, con
                              int64_t rows, int64_t feat, int dtype, int param_dtype, void *workspace, size_t workspace_bytes, void *stream) {
   if (bad(rows, feat, ldx) || (dweight == nullptr) != (dbias == nullptr)) return geot_internal_fail(GEOT_EINVAL, "geot_layer_norm_backward: bad argument");
   if (feat == 0) return GEOT_OK;
-  if (rows > 0 && (!x || !stats || !dy || !dx)) return geot_internal_fail(GEOT_EINVAL, "geot_layer_norm_backward: null pointer");
+  if (rows > 0 && (!x || !stats || !dy)) return geot_internal_fail(GEOT_EINVAL, "geot_layer_norm_backward: null pointer");
   NormArgs g{};
   g.x = x; g.ldx = ldx; g.weight = weight; g.dy = dy; g.dx = dx; g.stats = const_cast<float *>(stats); g.rows = rows; g.feat = feat;
   if (dweight) {

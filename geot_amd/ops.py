@@ -499,10 +499,10 @@ def _(x, weight, bias, eps):
 
 
 @torch.library.register_fake("geot_dense::layer_norm_backward")
-def _(grad, x, weight, bias, stats, need_params):
+def _(grad, x, weight, bias, stats, need_x, need_params):
     dtype = next((p.dtype for p in (weight, bias) if p is not None), x.dtype)
     n = x.shape[-1] if need_params else 0
-    return x.new_empty(x.shape), x.new_empty([n], dtype=dtype), x.new_empty([n], dtype=dtype)
+    return x.new_empty(x.shape if need_x else [0]), x.new_empty([n], dtype=dtype), x.new_empty([n], dtype=dtype)
 
 
 # --------------------------------------------------------------------------------------------------

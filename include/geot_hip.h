@@ -439,7 +439,7 @@ int geot_segment_matmul_grad_weight(const void *x, int64_t ldx, const int64_t *p
 
 /* geot_layer_norm:  y = (x - mean) * rstd * weight + bias over each row of x [rows, feat]; weight / bias [feat] or NULL, of `dtype` or
  * float32 (param_dtype).  stats [3, rows] float32 or NULL receives what the backward pass needs: the mean as two parts whose sum it is, and
- * rstd = 1 / sqrt(var + eps).  dx [rows, feat], dweight / dbias [feat] in param_dtype, both or neither. */
+ * rstd = 1 / sqrt(var + eps).  dx [rows, feat] or NULL, dweight / dbias [feat] in param_dtype, both or neither. */
 int geot_layer_norm(const void *x, int64_t ldx, const void *weight, const void *bias, void *y, float *stats, int64_t rows, int64_t feat,
                     float eps, int dtype, int param_dtype, void *stream);
 size_t geot_layer_norm_backward_workspace_bytes(int64_t rows, int64_t feat);

@@ -572,3 +572,22 @@ def test_layer_norm_in_root_mean_square(m, d, dtype):
     assert relative_error(dx, s * (gw - gw.mean(-1, keepdim=True) - h * (gw * h).mean(-1, keepdim=True))) <= bound
     assert relative_error(dw, (dy64 * h).sum(0)) <= bound
     assert relative_error(db, dy64.sum(0)) <= bound
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("d", [16, 100, 300, 1500, 3000, 5000, 9000])
+def test_layer_norm_parameter_gradients_alone(d, dtype):
+    """The rows need no gradient: none is made, and the parameters' are the same bits."""
+    g = torch.Generator().manual_seed(d)
+    x, dy, w, b = (torch.randn(*s, generator=g).to(dtype).cuda() for s in ((37, d), (37, d), (d,), (d,)))
+    w.requires_grad_(), b.requires_grad_()
+    alone = torch.autograd.grad(geot.layer_norm(x, w, b), [w, b], dy)
+    xg = x.clone().requires_grad_()
+    dx, *both = torch.autograd.grad(geot.layer_norm(xg, w, b), [xg, w, b], dy)
+    assert all(torch.equal(a, c) for a, c in zip(alone, both)) and bool(dx.any())
+    stats = torch.ops.geot_dense.layer_norm_train(x, w, b, 1e-5)[1]
+    none, dw, db = torch.ops.geot_dense.layer_norm_backward(dy, x, w, b, stats, False, True)
+    assert none.numel() == 0 and torch.equal(dw, alone[0]) and torch.equal(db, alone[1])
+    dx2, dw, db = torch.ops.geot_dense.layer_norm_backward(dy, x, w, b, stats, True, False)
+    assert torch.equal(dx2, dx) and dw.numel() == db.numel() == 0
