@@ -1361,9 +1361,13 @@ int64_t rows_share(int64_t rows, int64_t groups, bool with_ptr, int64_t n, int64
   const int64_t bn = f32 || n <= 64 ? 64 : 128, bk = f32 ? 32 : 64;
   const int64_t tiles = ((rows + 127) / 128 + (with_ptr ? (groups < rows ? groups : rows) : 0)) * ((n + bn - 1) / bn);
   if (tiles <= 0 || tiles >= 256 || k < 8 * bk) return k;
+  // (workgroups that find no rows - up to one a group - count against what a launch can hold)
+  const int64_t blocks = slots_of(rows, groups, with_ptr, 128) * ((n + bn - 1) / bn), room = 2 * kMaxBlocks / blocks;
   int64_t shares = (512 + tiles - 1) / tiles;
   const int64_t most = k / (4 * bk);
   shares = shares < most ? shares : most;
+  if (room < 4) return k; // (mm_rows_join_kernel's four a tile)
+  shares = shares < room ? shares : room;
   return ((k + shares - 1) / shares + bk - 1) / bk * bk;
 }
 size_t rows_workspace(int64_t rows, int64_t groups, bool with_ptr, int64_t n, int64_t k, int dtype) {
@@ -1567,9 +1571,11 @@ int weight_product(WeightArgs &g, int dtype, void *workspace, size_t workspace_b
   return geot_internal_fail(GEOT_EUNSUPPORTED, "matrix products take float32, float16 and bfloat16");
 }
 
+// Sizes no operand can have: negative, or matrices of more elements than any memory (the plans' products stay inside 64 bits then)
 bool bad_size(int64_t a, int64_t b, int64_t c) {
-  constexpr int64_t lim = (int64_t)1 << 40;
-  return a < 0 || b < 0 || c < 0 || a > lim || b > lim || c > lim;
+  constexpr int64_t lim = (int64_t)1 << 40, area = (int64_t)1 << 44;
+  const auto large = [&](int64_t m, int64_t n) { return m > 0 && n > area / m; };
+  return a < 0 || b < 0 || c < 0 || a > lim || b > lim || c > lim || large(a, b) || large(a, c) || large(b, c);
 }
 
 } // namespace
@@ -1582,7 +1588,7 @@ size_t geot_linear_workspace_bytes(int64_t rows, int64_t in, int64_t out, int dt
 
 int geot_linear(const void *x, int64_t ldx, const void *weight, const void *bias, const void *residual, int64_t ld_residual, void *z, void *y,
                 int64_t rows, int64_t in, int64_t out, int activation, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
-  if (bad_size(rows, in, out) || ldx < 0 || ld_residual < 0) return geot_internal_fail(GEOT_EINVAL, "geot_linear: negative size");
+  if (bad_size(rows, in, out) || ldx < 0 || ld_residual < 0) return geot_internal_fail(GEOT_EINVAL, "geot_linear: negative or impossible size");
   if (activation < GEOT_ACT_NONE || activation > GEOT_ACT_SILU) return geot_internal_fail(GEOT_EINVAL, "geot_linear: unknown activation");
   if (rows > 0 && out > 0 && (!y || (in > 0 && (!x || !weight)))) return geot_internal_fail(GEOT_EINVAL, "geot_linear: null pointer");
   RowsArgs g{};
@@ -1597,7 +1603,7 @@ size_t geot_linear_grad_input_workspace_bytes(int64_t rows, int64_t in, int64_t 
 
 int geot_linear_grad_input(const void *dz, const void *weight, void *dx, int64_t rows, int64_t in, int64_t out, int dtype, void *workspace, size_t workspace_bytes,
                            void *stream) {
-  if (bad_size(rows, in, out)) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_input: negative size");
+  if (bad_size(rows, in, out)) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_input: negative or impossible size");
   if (rows > 0 && in > 0 && (!dx || (out > 0 && (!dz || !weight)))) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_input: null pointer");
   RowsArgs g{};
   g.a = dz; g.lda = out; g.b = weight; g.ldb = in; g.y = dx; g.ldy = in;
@@ -1613,7 +1619,7 @@ size_t geot_linear_grad_weight_workspace_bytes(int64_t rows, int64_t in, int64_t
 
 int geot_linear_grad_weight(const void *dz, const void *x, int64_t ldx, void *dweight, void *dbias, int64_t rows, int64_t in, int64_t out, int dtype,
                             void *workspace, size_t workspace_bytes, void *stream) {
-  if (bad_size(rows, in, out) || ldx < 0) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_weight: negative size");
+  if (bad_size(rows, in, out) || ldx < 0) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_weight: negative or impossible size");
   if (in > 0 && out > 0 && (!dweight || (rows > 0 && (!dz || !x)))) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_weight: null pointer");
   WeightArgs g{};
   g.p = dz; g.ldp = out; g.np = out; g.q = x; g.ldq = ldx; g.nq = in; g.out = dweight; g.colsum = dbias; g.ns = out; g.sum_p = 1;
@@ -1632,7 +1638,7 @@ size_t geot_linear_grad_preactivation_workspace_bytes(int64_t rows, int64_t out)
 
 int geot_linear_grad_preactivation(const void *dy, const void *z, const void *x, int64_t ldx, const void *weight, const void *bias, void *dz, void *dbias,
                                    int64_t rows, int64_t in, int64_t out, int activation, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
-  if (bad_size(rows, in, out) || ldx < 0) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_preactivation: negative size");
+  if (bad_size(rows, in, out) || ldx < 0) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_preactivation: negative or impossible size");
   if (activation < GEOT_ACT_NONE || activation > GEOT_ACT_SILU) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_preactivation: unknown activation");
   if (rows == 0 || out == 0) return GEOT_OK;
   if (!dy || !dz || (!z && in > 0 && (!x || !weight))) return geot_internal_fail(GEOT_EINVAL, "geot_linear_grad_preactivation: null pointer");
@@ -1657,7 +1663,7 @@ size_t geot_segment_matmul_workspace_bytes(int64_t rows, int64_t groups, int64_t
 
 int geot_segment_matmul(const void *x, int64_t ldx, const int64_t *ptr, const void *weight, const void *bias, void *y, int64_t rows, int64_t groups,
                         int64_t in, int64_t out, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
-  if (bad_size(rows, in, out) || groups < 0 || groups > 65535 || ldx < 0) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul: negative size, or more than 65535 groups");
+  if (bad_size(rows, in, out) || groups < 0 || groups > 65535 || ldx < 0) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul: negative or impossible size, or more than 65535 groups");
   if (rows > 0 && out > 0 && (!y || !ptr || (in > 0 && groups > 0 && (!x || !weight)))) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul: null pointer");
   RowsArgs g{};
   g.a = x; g.lda = ldx; g.b = weight; g.ldb = out; g.b_group = in * out; g.bias = bias; g.bias_group = out; g.y = y; g.ldy = out;
@@ -1671,7 +1677,7 @@ size_t geot_segment_matmul_grad_input_workspace_bytes(int64_t rows, int64_t grou
 
 int geot_segment_matmul_grad_input(const void *dy, const int64_t *ptr, const void *weight, void *dx, int64_t rows, int64_t groups, int64_t in, int64_t out,
                                    int dtype, void *workspace, size_t workspace_bytes, void *stream) {
-  if (bad_size(rows, in, out) || groups < 0 || groups > 65535) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul_grad_input: negative size, or more than 65535 groups");
+  if (bad_size(rows, in, out) || groups < 0 || groups > 65535) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul_grad_input: negative or impossible size, or more than 65535 groups");
   if (rows > 0 && in > 0 && (!dx || !ptr || (out > 0 && groups > 0 && (!dy || !weight)))) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul_grad_input: null pointer");
   RowsArgs g{};
   g.a = dy; g.lda = out; g.b = weight; g.ldb = out; g.b_group = in * out; g.y = dx; g.ldy = in;
@@ -1687,7 +1693,7 @@ size_t geot_segment_matmul_grad_weight_workspace_bytes(int64_t rows, int64_t gro
 
 int geot_segment_matmul_grad_weight(const void *x, int64_t ldx, const int64_t *ptr, const void *dy, void *dweight, void *dbias, int64_t rows, int64_t groups,
                                     int64_t in, int64_t out, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
-  if (bad_size(rows, in, out) || groups < 0 || groups > 65535 || ldx < 0) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul_grad_weight: negative size, or more than 65535 groups");
+  if (bad_size(rows, in, out) || groups < 0 || groups > 65535 || ldx < 0) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul_grad_weight: negative or impossible size, or more than 65535 groups");
   if (groups > 0 && in > 0 && out > 0 && (!ptr || !dweight || (rows > 0 && (!x || !dy)))) return geot_internal_fail(GEOT_EINVAL, "geot_segment_matmul_grad_weight: null pointer");
   WeightArgs g{};
   g.p = x; g.ldp = ldx; g.np = in; g.q = dy; g.ldq = out; g.nq = out; g.out = dweight; g.colsum = dbias; g.ns = out; g.sum_p = 0;

@@ -401,8 +401,8 @@ template <typename F> int by_type(int dtype, int param, F f) {
   return geot_internal_fail(GEOT_EUNSUPPORTED, "layer_norm takes float32, float16 and bfloat16 rows, with parameters of that type or float32");
 }
 bool bad(int64_t rows, int64_t feat, int64_t ldx) {
-  constexpr int64_t lim = (int64_t)1 << 34;
-  return rows < 0 || feat < 0 || ldx < 0 || feat > lim;
+  constexpr int64_t lim = (int64_t)1 << 34, area = (int64_t)1 << 44; // (more elements than any memory)
+  return rows < 0 || feat < 0 || ldx < 0 || feat > lim || rows > area || (feat > 0 && rows > area / feat);
 }
 
 } // namespace

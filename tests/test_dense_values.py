@@ -87,6 +87,36 @@ def test_rewriting_keeps_the_order_of_writes(where, form):
         assert torch.equal(a, b.detach())
 
 
+def test_impossible_sizes_are_refused():
+    """Sizes whose products pass 64 bits: an error code, no division by zero on the way (in a process of its own: a signal would end it)."""
+    import subprocess
+    import sys
+    code = """
+import geot_amd as geot
+L, big = geot._lib.load(), 1 << 40
+for a, b, c in ((1, big, big), (big, big, 1), (big, 1, big), (big, big, big), (1 << 62, 1, 1), (-1, 4, 4)):
+    for dtype in (0, 2, 3):
+        assert L.geot_linear_workspace_bytes(a, b, c, dtype) == L.geot_linear_grad_input_workspace_bytes(a, b, c, dtype) == 0
+        assert L.geot_linear_grad_weight_workspace_bytes(a, b, c, dtype) == 0
+        assert L.geot_segment_matmul_workspace_bytes(a, 3, b, c, dtype) == L.geot_segment_matmul_grad_weight_workspace_bytes(a, 3, b, c, dtype) == 0
+        assert L.geot_linear(16, b, 16, None, None, 0, None, 16, a, b, c, 0, dtype, None, 0, None) == -1
+        assert L.geot_linear_grad_input(16, 16, 16, a, b, c, dtype, None, 0, None) == -1
+        assert L.geot_linear_grad_weight(16, 16, b, 16, 16, a, b, c, dtype, 16, 1 << 62, None) == -1
+        assert L.geot_segment_matmul(16, b, 16, 16, None, 16, a, 3, b, c, dtype, 16, 1 << 62, None) == -1
+        assert L.geot_segment_matmul_grad_weight(16, b, 16, 16, 16, 16, a, 3, b, c, dtype, 16, 1 << 62, None) == -1
+for rows, feat in ((1 << 62, 4), (big, 1 << 20), (4, 1 << 40), (-1, 4)):
+    assert L.geot_layer_norm(16, feat, None, None, 16, None, rows, feat, 1e-5, 0, 0, None) == -1
+    assert L.geot_layer_norm_backward_workspace_bytes(rows, feat) == 0
+    assert L.geot_layer_norm_backward(16, feat, None, 16, 16, 16, None, None, rows, feat, 0, 0, None, 0, None) == -1
+# one row, as many groups as there may be, a long reduction: its shares stay inside one launch (fewer than 2^32 threads)
+need = L.geot_segment_matmul_workspace_bytes(1, 65535, 65536, 1, 2)
+assert 0 < need <= ((1 << 32) // (256 * 65537)) * 4, need
+print("refused")
+"""
+    p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=geot._lib._ROOT)
+    assert p.returncode == 0 and p.stdout.strip() == "refused", (p.returncode, p.stdout, p.stderr[-500:])
+
+
 def test_segment_workspace_does_not_grow_with_groups():
     """Only chunks of groups that have several need room: at fixed rows no number of groups asks for more than twice the chunks of all rows."""
     L = geot._lib.load()
