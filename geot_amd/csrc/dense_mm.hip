@@ -310,7 +310,8 @@ template <typename P> __device__ inline P *pointer_of_lane(P *p, int lane) {
 // terms alone, which ends most NaN; longer reductions go to the whole wave one after the other, every lane taking each n-th term (one
 // infinity in a column of x makes every output's sum over that column's rows non-finite, and a chunk of rows can be all of them: 4096 x 4096
 // weights, 30,000 rows, their gradient 27 ms with one, 7.7 without; lane by lane alone 93).  Fixed order: the same bits every run.
-__device__ inline float sum_again(float v, bool bad, const float *a, int64_t stride_a, const float *b, int64_t stride_b, int64_t k) {
+// A function of its own: inlined, its registers spilled others around the tile kernels' loops (typed nodes f32, x W 81 -> 88 us; 85 so).
+__device__ __attribute__((noinline)) float sum_again(float v, bool bad, const float *a, int64_t stride_a, const float *b, int64_t stride_b, int64_t k) {
   constexpr int64_t kAlone = 64;
   constexpr int U = 8; // terms of a lane in flight
   bool left = false;
