@@ -1409,7 +1409,7 @@ template <typename T, int FM> int run_few(RowsArgs &g, hipStream_t st) {
   return launched("mm_few_rows_kernel");
 }
 // Few tiles and a reduction that eight waves of a workgroup walk in a few steps; a longer one of more than 32 rows is split over
-// workgroups instead (bf16: 100 x 1000 -> 1000 takes 7.9 us so and 15.6 split, 300 x 4096 -> 256 23.6 and 9.5).
+// workgroups instead (bf16: 100 x 1000 -> 1000 takes 7.8 us so and 15.8 split, as its dx is; 300 x 4096 -> 256 23.6 and 18.7).
 bool takes_few_rows(int64_t rows, bool with_ptr, int64_t n, int64_t k) {
   return !with_ptr && ((rows + 127) / 128) * ((n + 127) / 128) < 128 && k >= 128 && (rows <= 32 || k <= 2048);
 }
