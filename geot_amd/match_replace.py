@@ -37,6 +37,7 @@ from . import graph as _graph_ops  # noqa: F401  (registers geot::graph_spmm)
 
 aten = torch.ops.aten
 _ZEROS = {aten.new_zeros.default, aten.zeros.default, aten.zeros_like.default}
+_COPIES = {aten.clone.default, aten.contiguous.default, aten.reshape.default}
 _PASS_THROUGH = {aten.unsqueeze.default, aten.view.default, aten.reshape.default, aten._unsafe_view.default,
                  aten.expand.default, aten.alias.default, aten.contiguous.default, aten.clone.default}
 
@@ -150,8 +151,14 @@ def rewrite_graph(gm: fx.GraphModule, sort_edges: bool = False) -> int:
                 target = None
         if target is None or args is None:
             continue
-        read = [n for n in (source, *source.args) if _gathered_rows(n) is not None] + [source]
-        if _writes_between(read[0], node) or _may_be_written(dst):
+        copies = [source]               # where the replaced nodes read what the fused one reads at the end
+        if weight is not None:
+            copies.append(feat)
+            while fac is not weight:
+                if fac.target in _COPIES:
+                    copies.append(fac)
+                fac = fac.args[0]
+        if _writes_between(next(n for n in graph.nodes if n in copies), node) or _may_be_written(dst):
             continue                    # (the rows, a factor or the zeros may hold something else by now)
         rows = _rows_arg(graph, dst, node)
         with graph.inserting_before(node):
@@ -200,7 +207,7 @@ def rewrite_dense(gm: fx.GraphModule) -> int:
     for node in list(graph.nodes):
         if _is(node, aten.linear.default):
             x, w = node.args[:2]
-            b = node.args[2] if len(node.args) > 2 else None
+            b = node.args[2] if len(node.args) > 2 else node.kwargs.get("bias")
             if not _dense_operands(x, w, b) or len(_shape(w)) != 2:
                 continue
             last, act, residual = node, "none", None

@@ -130,17 +130,21 @@ def test_segment_workspace_does_not_grow_with_groups():
     assert need <= 4 * (4096 * 4096 + 4096) * 4
 
 
-@pytest.mark.parametrize("where", ["nowhere", "rows", "factor", "zeros", "row of zeros"])
+@pytest.mark.parametrize("where", ["nowhere", "rows", "factor", "factor, copied before", "zeros", "row of zeros"])
 def test_rewriting_an_aggregation_keeps_the_order_of_writes(where):
     from geot_amd.match_replace import pattern_transform
 
     class Aggregate(torch.nn.Module):
         def forward(self, x, w, row, col):
             h, f = x * 2, w * 2
+            column = f.unsqueeze(-1)
+            if where.startswith("factor,"):
+                column = column.clone()
+                f.add_(1)
             rows = h.index_select(0, col)
             out = h.new_zeros(5, 6)
-            scaled = rows * f.unsqueeze(-1)
-            if where != "nowhere":
+            scaled = column * rows
+            if where in ("rows", "factor", "zeros", "row of zeros"):
                 {"rows": h, "factor": f, "zeros": out, "row of zeros": out[0]}[where].add_(1)
             return out.index_add(0, row, scaled) + h.sum() + f.sum()
 
