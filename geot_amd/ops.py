@@ -613,7 +613,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     leave one: 2.4e-3 instead of 1.7e-3 for bfloat16, 2.9e-4 instead of 2.1e-4 for float16), the bias's gradient is summed before it.  A
     training call of a wide layer also keeps the pre-activation in the operands' dtype, and takes the activation's slope there; a narrow one
     (in <= 256, float32 128) computes it again in the backward pass, unrounded, and 'none', and 'relu' without a residual, do not need it.
-    16-bit gelu is a fit to 2^-15 of the value (2^-13 below -10).  A factor of a float32 product below 2^-110 keeps an absolute 2^-133."""
+    16-bit gelu is a fit to 2^-15 of the value (2^-13 below -10).  float32 products are taken in three bfloat16 parts, to 2^-23 of each; a factor of a float32 product below 2^-110 keeps an absolute 2^-133."""
     return torch.ops.geot_dense.linear(x, weight, bias, residual, activation)
 
 

@@ -625,3 +625,87 @@ def test_layer_norm_parameter_gradients_alone(d, dtype):
     assert none.numel() == 0 and torch.equal(dw, alone[0]) and torch.equal(db, alone[1])
     dx2, dw, db = torch.ops.geot_dense.layer_norm_backward(dy, x, w, b, stats, True, False)
     assert torch.equal(dx2, dx) and dw.numel() == db.numel() == 0
+
+
+# ---- several at once --------------------------------------------------------------------------------------------------------------------
+def _training_step(path, dtype, seed):
+    m, k, n = PATHS[path]
+    g = torch.Generator().manual_seed(seed)
+    x, w, b, dy = ((torch.randn(*s, generator=g) * c).to(dtype).cuda() for s, c in (((m, k), 1), ((n, k), k ** -0.5), ((n,), 1), ((m, n), 1)))
+    ptr = torch.tensor([0, m // 2, m], device="cuda")
+    w3 = torch.stack([w.t(), w.t() * 0.5]).contiguous()
+    inputs = [x, w, b, w3]
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in inputs]
+        y = geot.layer_norm(geot.linear(*leaves[:3], activation="gelu"))
+        z = geot.segment_matmul(leaves[0], ptr, leaves[3])
+        return [y.detach(), z.detach(), *torch.autograd.grad([y, z], leaves, [dy, dy])]
+
+    return inputs, step
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_two_threads_on_their_own_streams(dtype):
+    """Training steps of every path from two threads at once: the bits of each step alone."""
+    import threading
+    steps = [_training_step(path, dtype, i)[1] for i, path in enumerate(PATHS)]
+    want = [step() for step in steps]
+    torch.cuda.synchronize()
+    errors, done = [], []
+
+    def work(order):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(5):
+                    for i in order:
+                        for a, c in zip(steps[i](), want[i]):
+                            if not torch.equal(a, c):
+                                errors.append(i)
+            stream.synchronize()
+            done.append(True)
+        except Exception as e:  # noqa: BLE001
+            errors.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(order,)) for order in ((0, 1, 2, 3), (3, 1, 0, 2))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(timeout=60)
+    assert not errors and len(done) == 2, errors
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_every_path_in_two_captured_graphs(dtype):
+    """Each path's training step in two graphs with scratch of their own, replayed in turn on new inputs with eager steps between."""
+    for i, path in enumerate(PATHS):
+        pair = [_training_step(path, dtype, 10 * i + j) for j in range(2)]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _, step in pair:
+                step()
+        torch.cuda.current_stream().wait_stream(side)
+        graphs, outs = [], []
+        for _, step in pair:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                outs.append(step())
+            graphs.append(graph)
+        for turn in range(3):
+            g = torch.Generator(device="cuda").manual_seed(turn)
+            for inputs, _ in pair:
+                for t in inputs:
+                    t.copy_(torch.randn(t.shape, generator=g, device="cuda") * 0.1)
+            want = [step() for _, step in pair]
+            for graph in graphs if turn % 2 else graphs[::-1]:
+                graph.replay()
+            torch.cuda.synchronize()
+            for w_, o_ in zip(want, outs):
+                for a, c in zip(w_, o_):
+                    assert torch.equal(a, c), (path, turn)
+            pair[0][1]()
+            torch.cuda.synchronize()
